@@ -222,6 +222,113 @@ lik_status lik_paged_append(
     void* cache, void* scale, void* zero,
     int64_t num_blocks, int64_t block_size, void* stream);
 
+/* Append new tokens of queries, keys and values into a paged cache, rotating
+ * queries and keys by their positions on the way (no reference counterpart;
+ * equals rotating first and lik_paged_append after).
+ *
+ * Channel pair f of n_freqs pairs turns by positions[axis(f)] * inv_freq[f]
+ * radians: (a, b) -> (a cos - b sin, b cos + a sin), rounded once to fp16. The
+ * pair is channels (f, f + n_freqs), or (2 f, 2 f + 1) when interleaved != 0;
+ * channels from 2 n_freqs on pass. positions: int64 [n_axes, n_tokens], up to 4
+ * axes; axis a turns sections[a] consecutive frequencies (host array, sum
+ * n_freqs; may be NULL when n_axes is 1). inv_freq: fp32 [n_freqs], 1 <=
+ * n_freqs <= 64.
+ *
+ * q, q_out [n_tokens, n_heads, 128]; k, v [n_tokens, n_kv_heads, 128] fp16,
+ * tokens *_token_stride elements apart (a multiple of 8; views of a fused
+ * projection), q_out contiguous and, if q is contiguous too, possibly q
+ * itself. slot_mapping as in lik_paged_append: a token whose slot is < 0 or >=
+ * num_blocks * block_size is rotated but not stored; two tokens must not name
+ * the same slot. k_format: 0 fp16 or 1 INT8 per token (k_scale); v_format: a
+ * row_format of lik_paged_append (v_scale, v_zero). Keys are rounded to fp16
+ * before they are quantized. The per-channel INT4 K format is not appended
+ * token by token (see lik_paged_append). */
+lik_status lik_paged_append_rope(
+    int k_format, int v_format, const void* q, int64_t q_token_stride,
+    const void* k, int64_t k_token_stride, const void* v, int64_t v_token_stride,
+    const int64_t* positions, int64_t n_axes, const int64_t* sections,
+    const float* inv_freq, int64_t n_freqs, int interleaved,
+    const int64_t* slot_mapping, void* q_out,
+    int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+    void* k_cache, void* k_scale, void* v_cache, void* v_scale, void* v_zero,
+    int64_t num_blocks, int64_t block_size, void* stream);
+
+/* ---- attention of several query tokens, shared prefixes ---------------- */
+
+/* Bytes of workspace that the two entry points below need on the current
+ * device: n_groups = 0 for lik_attention_paged, else the prefix groups of
+ * lik_attention_shared_prefix. It needs no initialization, holds nothing
+ * between calls, and must be 256-byte aligned; calls that may overlap on the
+ * GPU need different ones. */
+size_t lik_attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t n_groups);
+
+/* Attention of any number of query tokens per sequence over a paged cache (no
+ * reference counterpart): prompts, chunks of prompts and single tokens in one
+ * call. kv_format: 0 fp16, 1 INT8 per token; layouts of
+ * lik_decode_attention_paged.
+ *
+ * q [n_tokens, n_heads, 128] fp16, tokens q_token_stride elements apart (a
+ * multiple of 8); out the same, contiguous. Sequence b owns tokens
+ * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 (int32 [n_seqs + 1], ascending) and
+ * the first context_lens[b] positions of its table (int32 [n_seqs], clamped to
+ * [0, block_size * max_blocks_per_seq]); its queries are the last of those
+ * positions: the i-th of n stands at p = context_lens[b] - n + i.
+ *
+ *   score(p, j) = softmax_scale q.k_j                 (> 0)
+ *   if softcap > 0: score = softcap * tanh(score / softcap)
+ *   if alibi_slopes (fp32 [n_heads]): score -= slope * |p - j|
+ *   visible: j < context_lens[b], j >= first_keys[token] (int32 [n_tokens], may
+ *     be NULL: the start of the token's document), and either
+ *     j < prefix_lens[b] (int32 [n_seqs], may be NULL: a prefix that every query
+ *     of the sequence sees), or j <= p if causal and j > p - window if window > 0
+ *
+ * A row that sees nothing is zero. Rows of no sequence (before
+ * cu_seqlens_q[0], from cu_seqlens_q[n_seqs] on) are left as they are, or set
+ * to zero with zero_tail != 0. Keys and values that no query of a sequence
+ * sees (page ends, what left the window) may hold anything, and the table
+ * entries of pages with none that is seen are not read; a value that some query sees must be
+ * finite. A table entry outside [0, num_blocks) that is reached reads as zero
+ * keys and values, and LIK_ERR_DEVICE_BAD_BLOCK is recorded
+ * (lik_attention_check). Requires n_heads / n_kv_heads <= 128 and fewer than
+ * 2^31 - 128 rows in the cache (num_blocks * n_kv_heads * block_size).
+ * Lengths and offsets are read on the device: a captured call may be replayed
+ * with others. */
+lik_status lik_attention_paged(
+    int kv_format, const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+    const void* k_scale, const void* v_scale, const int32_t* block_tables, const int32_t* context_lens,
+    const int32_t* cu_seqlens_q, void* out,
+    int64_t n_tokens, int64_t n_seqs, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+    int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+    float softmax_scale, int causal, int64_t window, float softcap, const float* alibi_slopes,
+    const int32_t* prefix_lens, const int32_t* first_keys, int zero_tail,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Single-token attention of requests that share prefixes, each prefix read
+ * once for all of its group's requests (no reference counterpart). Requests
+ * cu_groups[g] .. cu_groups[g + 1] - 1 (int32 [n_groups + 1], ascending) attend
+ * over the first prefix_lens[g] positions of row g of prefix_tables (int32
+ * [n_groups, prefix_blocks]) followed by the first context_lens[b] positions of
+ * row b of block_tables (int32 [batch, max_blocks_per_seq]; a length may be 0),
+ * one softmax over both. The request's own positions start a page of their own.
+ * q, out [batch, n_heads, 128]. softcap and alibi_slopes as above, the query
+ * standing at prefix + own length - 1. A request of no group attends to its own
+ * positions only; one without any key is zero. The rest as in
+ * lik_attention_paged. */
+lik_status lik_attention_shared_prefix(
+    int kv_format, const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+    const void* k_scale, const void* v_scale, const int32_t* prefix_tables, const int32_t* prefix_lens,
+    const int32_t* cu_groups, const int32_t* block_tables, const int32_t* context_lens, void* out,
+    int64_t batch, int64_t n_groups, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+    int64_t num_blocks, int64_t block_size, int64_t prefix_blocks, int64_t max_blocks_per_seq,
+    float softmax_scale, float softcap, const float* alibi_slopes,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Read (and clear) the device error word of the two entry points above on the
+ * current device, after the work queued on `stream` (synchronizes it):
+ * *device_error = 0 and LIK_OK when clean, else the code and status of
+ * lik_workspace_check. */
+lik_status lik_attention_check(void* stream, int* device_error);
+
 /* ---- KV quantize / pack --------------------------------------------- */
 /*
  * Source x: [batch, n_kv_heads, n_tokens, head_dim] fp16, contiguous.

@@ -33,11 +33,13 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = {
     "decode.cu": [],
     "quantize.cu": ["-fmad=false"],   # bit-exact quantization: no contraction
+    "rope.cu": ["-fmad=false"],
+    "attention.cu": [],
     "cabi.cu": [],
     "noalloc.cu": [],
     "selftest.cu": [],
 }
-HEADERS = ["lik_device.cuh", "lik_internal.h"]
+HEADERS = ["lik_device.cuh", "lik_quant.cuh", "lik_tcgen05.cuh", "lik_internal.h"]
 
 
 def _nvcc() -> str:

@@ -1,0 +1,1300 @@
+// Attention of any number of query tokens per sequence over a paged KV cache,
+// on tcgen05 (fp16 operands, fp32 scores, softmax state and accumulators).
+//
+//   s = scale q.k             or cap tanh(scale q.k / cap), minus slope |p - j|
+//   out = softmax(s) v        over the visible keys j of the query at position p
+//
+// One kernel serves prompts, chunks of prompts, single tokens and the two key
+// sets (shared prefix, own tokens) of shared-prefix decoding.
+//
+// Unit: the query heads of one KV head (G of them) for up to 2 * floor(128 / G)
+// consecutive tokens of one sequence; row = token * G + head. Keys are walked
+// in tiles of 128 positions. The units' tiles, laid end to end, are split
+// evenly over one CTA per SM, so lengths need not be known on the host and a
+// few long sequences use the whole GPU; every CTA finds its share itself from
+// the lengths in device memory. A unit that several CTAs share leaves
+// unnormalized partial sums, joined by the second kernel in a fixed order.
+//
+// A CTA runs two streams (0, 1) of score tile -> softmax -> weighted sum, each
+// with its own 128 softmax threads, so that one stream's matrix instructions
+// run under the other's exponentials:
+//   wide units (more than 128 rows): stream s holds rows [s], both read every
+//     key tile;
+//   narrow units: both streams hold the same rows and take alternate key
+//     tiles. Units of at most 64 (32) rows are repeated 2 (4) times along the
+//     128 rows of the matrix instruction, and each copy takes the softmax of
+//     its own 64 (32) columns of a tile; a single token's softmax then occupies
+//     all eight warps instead of one. The copies' states are joined at the
+//     unit's end.
+// Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the fp16 weights P
+// overwrite the scores they come from. P V reads P from tensor memory and V as
+// stored ([position, channel], the transposed-operand form).
+//
+// fp16 caches go from the pool to swizzled shared memory by tensor-map copies,
+// one box per run of positions inside a page. INT8 caches arrive as codes and
+// scales; four more warps write fp16(code * scale), the rounding of the
+// dequantizing entry points, into the same swizzled tiles.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "lik_internal.h"
+#include "lik_tcgen05.cuh"
+
+namespace lik {
+
+// Device error word of this file's kernels (zero when the library loads).
+__device__ int g_attention_error;
+
+namespace {
+
+constexpr int kTile = 128;                       // key positions per tile
+constexpr int kTileBytes = kTile * kHeadDim * 2; // one fp16 K or V tile
+constexpr int kHalfTile = kTileBytes / 2;        // its 64-channel half
+constexpr int kRing8 = 3, kRing16 = 5;           // fp16 tiles in flight
+constexpr int kRaw = 4;                          // INT8 tiles in flight
+constexpr int kRawBytes = kTile * kHeadDim + 256;
+constexpr int kSegs = 4;
+constexpr int kScratchBytes = kTileBytes;        // narrow units: the second query tile's space
+constexpr float kLog2e = 1.4426950408889634f;
+// The running maximum is raised only past this many powers of two, so most
+// tiles leave the accumulator alone; weights stay below 2^8 in fp16.
+constexpr float kRaise = 8.0f;
+constexpr uint32_t kPolls = 1u << 20;            // of a microsecond at most each
+
+enum Dest : int { kDirect = 0, kSlot = 1, kRowBuf = 2 };
+
+struct KeySet {
+    const int* cu;      // [n_seq + 1] token offsets; null: token i is sequence i
+    const int* ctx;     // [n_seq] live positions
+    const int* tables;  // [n_seq, width]
+    const int* extra;   // per token: positions that follow the keys (moves p); null: none
+    int n_seq, width, n_ids, causal;
+};
+
+struct Params {
+    KeySet set[2];
+    int n_sets;
+    const int* prefix_lens;
+    const int* first_keys;
+    const float* slopes;
+    int window;
+    float scale, cap;
+    int n_tokens, n_heads, n_kv, group;
+    int num_blocks, block_size, box_rows, total_rows;
+    const __half* k_scale;
+    const __half* v_scale;
+    __half* out;
+    int shared;      // every unit's result goes through the joining kernel
+    int zero_tail;
+    int slot_rows, grid;
+    float* part;     // [2 grid][slot_rows][128]
+    float2* part_ml; // [2 grid][slot_rows] (maximum in powers of two, sum)
+    int4* split;     // [grid] first token, tokens, head, last CTA (-1: none) of the unit split from this CTA on
+    float* rowbuf;   // [2][n_tokens n_heads][128]
+    float2* row_ml;
+    int2* units;     // [(n_ids0 + n_ids1) n_kv] first CTA, last CTA (-1: in rowbuf)
+};
+
+struct Maps {
+    CUtensorMap q[3];  // boxes of 128, 64 and 32 rows' whole tokens
+    CUtensorMap k, v;
+};
+
+struct Segment {
+    int valid, set, seq, head;
+    int tok0, ntok, rep;        // rep 0: wide
+    int ctx, pos0, pfx, fk;     // fk: smallest first key
+    int a0, na, b0, nt;         // key tiles: na from a0, the rest from b0
+    int vlo, vhi;               // positions any row sees: [fk, pfx) and [vlo, vhi]
+    int t0, t1;                 // this CTA's share of the nt tiles
+    int dest;
+    __device__ int tile(int i) const { return i < na ? a0 + i : b0 + i - na; }
+    __device__ bool seen(int j) const { return (j >= vlo && j <= vhi) || (j >= fk && j < pfx); }
+};
+
+struct Misc {
+    uint64_t full[5], empty[5], rfull[kRaw], rempty[kRaw];
+    uint64_t qfull, qempty, sfull[2], pready[2], odone[2], segfull[kSegs], segempty[kSegs], xbar, drain;
+    Segment seg[kSegs];
+    long long scan[17];
+    long long start, count, total;
+    int start_id, start_head, start_off;
+    uint32_t bad[kRaw];
+    int abort;
+    uint32_t tmem;
+};
+static_assert(sizeof(Misc) <= 2048, "the barrier block must fit behind the tiles");
+
+template <int FMT>
+struct Layout {
+    static constexpr int ring = FMT == kF16 ? kRing16 : kRing8;
+    static constexpr int raw = 2 * kTileBytes + ring * kTileBytes;
+    static constexpr int misc = raw + (FMT == kF16 ? 0 : kRaw * kRawBytes);
+    static constexpr int bytes = misc + 2048;
+    static constexpr int threads = FMT == kF16 ? 384 : 512;
+    // registers per thread: launched with `base`, then moved between the
+    // warpgroups; the shares add up to threads * base
+    static constexpr int base = FMT == kF16 ? 168 : 128;
+    static constexpr int softmax_regs = FMT == kF16 ? 208 : 184;
+    static constexpr int other_regs = FMT == kF16 ? 88 : 48;
+    static constexpr int convert_regs = 96;
+    static_assert(2 * softmax_regs + other_regs + (FMT == kF16 ? 0 : convert_regs) <= threads / 128 * base,
+                  "register shares exceed what the block is launched with");
+};
+
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// ---- bounded waits -----------------------------------------------------------
+
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {  // sleeps for a microsecond at most
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity), "r"(1000u)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* abort_flag) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kPolls; ++i) {
+        if (__all_sync(kFull, poll(bar, parity))) return true;
+        if (*reinterpret_cast<volatile int*>(abort_flag)) break;
+    }
+    if ((threadIdx.x & 31) == 0) {
+        *reinterpret_cast<volatile int*>(abort_flag) = 1;
+        atomicCAS(&g_attention_error, 0, static_cast<int>(kDevWaitTimeout));
+    }
+    return false;
+}
+// Whole warp; every lane has observed the phase on return. False: give up
+// (this wait or another one of the CTA ran out).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Misc* m) {
+    if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
+    return wait_slow(bar, parity, &m->abort);
+}
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
+// ---- units -------------------------------------------------------------------
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+__device__ __forceinline__ int cu_at(const KeySet& k, int b, int n_tokens) {
+    return k.cu ? clampi(k.cu[b], 0, n_tokens) : b;
+}
+
+// The key set and the sequence whose unit numbers include `id`; a sequence
+// whose tokens start at c owns the numbers from c / unit + (its index).
+__device__ __forceinline__ int seq_of(const KeySet& k, int id, int unit, int n_tokens) {
+    if (!k.cu) return id;
+    int lo = 0, hi = k.n_seq - 1;  // largest b with cu[b] / unit + b <= id
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cu_at(k, mid, n_tokens) / unit + mid <= id) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Fills the unit `id` (all heads alike); false if no tokens carry this number.
+__device__ bool make_unit(const Params& p, int id, Segment& s) {
+    s.set = id < p.set[0].n_ids ? 0 : 1;
+    const KeySet& k = p.set[s.set];
+    if (s.set) id -= p.set[0].n_ids;
+    if (k.n_seq <= 0) return false;
+    const int per = kTile / p.group, unit = 2 * per;
+    const int b = seq_of(k, id, unit, p.n_tokens);
+    const int c0 = cu_at(k, b, p.n_tokens);
+    const int n = k.cu ? cu_at(k, b + 1, p.n_tokens) - c0 : 1;
+    const int at = k.cu ? (id - (c0 / unit + b)) * unit : 0;
+    if (at < 0 || at >= n) return false;
+    s.seq = b;
+    s.tok0 = c0 + at;
+    s.ntok = min(unit, n - at);
+    s.rep = s.ntok * p.group <= 32 / p.group * p.group   ? 4
+            : s.ntok * p.group <= 64 / p.group * p.group ? 2
+            : s.ntok <= per                              ? 1
+                                                         : 0;
+    s.ctx = static_cast<int>(min(static_cast<long long>(max(k.ctx[b], 0)),
+                                 static_cast<long long>(k.width) * p.block_size));
+    s.pos0 = s.ctx - n + at;
+    s.pfx = p.prefix_lens && s.set == 0 ? min(p.prefix_lens[b], s.ctx) : 0;
+    int fk = 0;
+    if (p.first_keys) {
+        fk = 0x7fffffff;
+        for (int i = 0; i < s.ntok; ++i) fk = min(fk, p.first_keys[s.tok0 + i]);
+        fk = max(fk, 0);
+    }
+    s.fk = fk;
+    s.vlo = p.window > 0 ? max(s.pos0 - p.window + 1, fk) : fk;
+    s.vhi = k.causal ? min(s.pos0 + s.ntok - 1, s.ctx - 1) : s.ctx - 1;
+    s.a0 = s.na = s.b0 = 0;
+    if (s.pfx > fk) {
+        s.a0 = fk / kTile;
+        s.na = (s.pfx - 1) / kTile - s.a0 + 1;
+    }
+    s.nt = s.na;
+    if (s.vhi >= s.vlo) {
+        s.b0 = max(s.vlo / kTile, s.a0 + s.na);
+        s.nt += max(s.vhi / kTile - s.b0 + 1, 0);
+    }
+    return true;
+}
+
+// ---- softmax of one stream -----------------------------------------------------
+
+struct Row {  // what one softmax thread's row sees
+    int lo, hi, fk, pfx;
+    float pos, slope;
+};
+
+__device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
+    return 1.0f - 2.0f * fast_rcp(1.0f + fast_exp2(t * (2.0f * kLog2e)));
+}
+
+// One tile: NC score columns from column c0, keys from j0. `m` is in score
+// units, `sc` turns those into powers of two.
+template <int NC, bool MOD>
+__device__ __forceinline__ bool softmax_tile(const Params& p, Misc* mi, const Row& row, uint32_t s_addr, uint32_t o_addr,
+                                             int c0, int j0, bool first, uint64_t* odone, uint32_t odone_parity,
+                                             float sc, float& m, float& l) {
+    float s[NC];
+#pragma unroll
+    for (int i = 0; i < NC; i += 32) tmem_ld32(s_addr + c0 + i, s + i);
+    tmem_wait_ld();
+    if (MOD) {
+        if (p.cap > 0.f) {
+            const float in = p.scale / p.cap, up = p.cap * kLog2e;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) s[i] = up * tanh_exp(s[i] * in);
+        } else {
+            const float up = p.scale * kLog2e;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) s[i] *= up;
+        }
+        if (p.slopes) {
+            const float from = static_cast<float>(j0) - row.pos;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) s[i] = fmaf(-row.slope, fabsf(from + static_cast<float>(i)), s[i]);
+        }
+    }
+    const int j1 = j0 + NC - 1;
+    const bool whole = (j0 >= row.lo && j1 <= row.hi) || (j0 >= row.fk && j1 < row.pfx);
+    if (__any_sync(kFull, !whole)) {
+        const int lo = row.lo - j0, hi = row.hi - j0, fk = row.fk - j0, pfx = row.pfx - j0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const bool see = (i >= lo && i <= hi) || (i >= fk && i < pfx);
+            s[i] = see ? s[i] : -INFINITY;
+        }
+    }
+    float t[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int i = 4; i < NC; ++i) t[i & 3] = fmaxf(t[i & 3], s[i]);
+    const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+    if (first) {
+        m = top;
+    } else if (__any_sync(kFull, (top - m) * sc > kRaise)) {
+        const float up = fmaxf(m, top);
+        const float a = m == -INFINITY ? 0.f : fast_exp2((m - up) * sc);
+        m = up;
+        l *= a;
+        if (!warp_wait(odone, odone_parity, mi)) return false;
+        tcgen05_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < kHeadDim; c += 32) {
+            float o[32];
+            tmem_ld32(o_addr + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= a;
+            tmem_st32(o_addr + c, o);
+        }
+    }
+    const float ms = m == -INFINITY ? 0.f : -m * sc;
+    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    const float2 sc2 = {sc, sc}, ms2 = {ms, ms};
+#pragma unroll
+    for (int i = 0; i < NC; i += 32) {
+        uint32_t w[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+            float2 x = fma2({s[i + 2 * c], s[i + 2 * c + 1]}, sc2, ms2);
+            x.x = fast_exp2(x.x);
+            x.y = fast_exp2(x.y);
+            sum[c & 1] = add2(sum[c & 1], x);
+            w[c] = pack_f16(x.x, x.y);
+        }
+        tmem_st16(s_addr + (c0 + i) / 2, w);
+    }
+    if (NC < kTile) {  // the other copies' columns weigh nothing in this one
+        const uint32_t z[16] = {};
+#pragma unroll
+        for (int i = 0; i < kTile; i += 32)
+            if (i < c0 || i >= c0 + NC) tmem_st16(s_addr + i / 2, z);
+    }
+    const float2 all = add2(sum[0], sum[1]);
+    l += all.x + all.y;
+    tmem_wait_st();
+    tcgen05_fence_before();
+    return true;
+}
+
+template <int NC, bool MOD>
+__device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Segment& g, const Row& row, int stream,
+                                            uint32_t s_addr, uint32_t o_addr, float sc, uint32_t& tiles, float& m,
+                                            float& l) {
+    const int warp = (threadIdx.x >> 5) & 3;
+    const int c0 = NC == 128 ? 0 : NC == 64 ? (warp >> 1) * 64 : warp * 32;
+    const int step = g.rep ? 2 : 1;
+    const int i0 = g.t0 + (g.rep ? stream : 0);
+#pragma unroll 1
+    for (int i = i0; i < g.t1; i += step) {
+        if (!warp_wait(&mi->sfull[stream], tiles & 1, mi)) return false;
+        tcgen05_fence_after();
+        if (!softmax_tile<NC, MOD>(p, mi, row, s_addr, o_addr, c0, g.tile(i) * kTile + c0, i == i0, &mi->odone[stream],
+                                   (tiles - 1) & 1, sc, m, l))
+            return false;
+        warp_arrive(&mi->pready[stream]);
+        ++tiles;
+    }
+    return true;
+}
+
+__device__ __forceinline__ void store_row(const Params& p, const Segment& g, int tok, int head_row, int unit_row, int c,
+                                          float4 v, float inv) {
+    if (g.dest == kDirect) {
+        uint2 u;
+        u.x = pack_f16(v.x * inv, v.y * inv);
+        u.y = pack_f16(v.z * inv, v.w * inv);
+        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(tok) * p.n_heads + head_row) * kHeadDim + c) = u;
+    } else {
+        const size_t r = g.dest == kSlot
+                             ? static_cast<size_t>(2 * blockIdx.x + (g.t0 == 0)) * p.slot_rows + unit_row
+                             : static_cast<size_t>(g.set) * p.n_tokens * p.n_heads +
+                                   static_cast<size_t>(tok) * p.n_heads + head_row;
+        float* dst = (g.dest == kSlot ? p.part : p.rowbuf) + r * kHeadDim + c;
+        *reinterpret_cast<float4*>(dst) = v;
+    }
+}
+__device__ __forceinline__ void store_ml(const Params& p, const Segment& g, int tok, int head_row, int unit_row, float m,
+                                         float l) {
+    if (g.dest == kSlot)
+        p.part_ml[static_cast<size_t>(2 * blockIdx.x + (g.t0 == 0)) * p.slot_rows + unit_row] = {m, l};
+    else if (g.dest == kRowBuf)
+        p.row_ml[static_cast<size_t>(g.set) * p.n_tokens * p.n_heads + static_cast<size_t>(tok) * p.n_heads +
+                 head_row] = {m, l};
+}
+
+// Barrier of the eight softmax warps.
+__device__ __forceinline__ bool softmax_sync(Misc* mi, uint32_t& phase) {
+    warp_arrive(&mi->xbar);
+    return warp_wait(&mi->xbar, phase++ & 1, mi);
+}
+
+template <bool MOD>
+__device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uint32_t tmem) {
+    const int stream = threadIdx.x >> 7, r_in = threadIdx.x & 127;
+    const uint32_t lane_base = static_cast<uint32_t>(r_in & 96) << 16;
+    const uint32_t s_addr = tmem + lane_base + stream * 128, o_addr = s_addr + 256;
+    const float sc = MOD ? 1.f : p.scale * kLog2e;
+    const int per = kTile / p.group;
+    uint32_t tiles = 0, xphase = 0;
+    for (uint32_t k = 0;; ++k) {
+        const int slot = k % kSegs;
+        if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
+        const Segment& g = mi->seg[slot];
+        if (!g.valid) return;
+        const KeySet& ks = p.set[g.set];
+        const int block = g.rep ? kTile / g.rep : kTile;  // rows of one copy
+        const int rr = r_in & (block - 1);
+        const int tl0 = rr / p.group, hr = g.head * p.group + rr - tl0 * p.group;
+        const int tl = tl0 + (g.rep ? 0 : stream * per);
+        const bool live = tl < g.ntok && rr < block / p.group * p.group;
+        const int tok = g.tok0 + tl;
+        Row row{0, 0x7fffffff, 0, 0, 0.f, 0.f};  // a row that is not live keeps every column: nothing reads it
+        if (live) {
+            const int pos = g.pos0 + tl + (ks.extra ? max(ks.extra[tok], 0) + g.ctx - 1 - (g.pos0 + tl) : 0);
+            row.fk = p.first_keys ? max(p.first_keys[tok], 0) : 0;
+            row.lo = max(p.window > 0 ? max(pos - p.window + 1, 0) : 0, row.fk);
+            row.hi = ks.causal ? min(pos, g.ctx - 1) : g.ctx - 1;
+            row.pfx = g.pfx;
+            row.pos = static_cast<float>(pos);
+            if (MOD && p.slopes) row.slope = p.slopes[hr] * kLog2e;
+        }
+        float m = -INFINITY, l = 0.f;
+        const int mine = g.rep ? (g.t1 - g.t0 - stream + 1) / 2 : g.t1 - g.t0;  // tiles of this stream
+        bool ok;
+        if (g.rep == 4)
+            ok = softmax_run<32, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, m, l);
+        else if (g.rep == 2)
+            ok = softmax_run<64, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, m, l);
+        else
+            ok = softmax_run<128, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, m, l);
+        if (!ok) return;
+        if (mine > 0) {
+            if (!warp_wait(&mi->odone[stream], (tiles - 1) & 1, mi)) return;
+            tcgen05_fence_after();
+        }
+        const float m2 = l > 0.f ? m * sc : -INFINITY;
+        if (g.rep == 0) {
+            const int ur = tl * p.group + hr - g.head * p.group;
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            if (live) store_ml(p, g, tok, hr, ur, m2, l);
+#pragma unroll 1
+            for (int c = 0; c < kHeadDim; c += 32) {
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                if (mine > 0) {
+                    tmem_ld32(o_addr + c, o);
+                    tmem_wait_ld();
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        store_row(p, g, tok, hr, ur, c + i,
+                                  l > 0.f ? float4{o[i], o[i + 1], o[i + 2], o[i + 3]} : float4{0.f, 0.f, 0.f, 0.f}, inv);
+                }
+            }
+        } else {
+            // join the copies and streams: each scales its sums to the row's
+            // common maximum, then 256 threads add the states in order
+            float2* ml = reinterpret_cast<float2*>(smem + kTileBytes);
+            float* data = reinterpret_cast<float*>(smem + kTileBytes + 2048);
+            const int states = 2 * g.rep, rows = g.ntok * p.group;
+            const int state = stream * g.rep + r_in / block;
+            ml[threadIdx.x] = live ? float2{m2, l} : float2{-INFINITY, 0.f};
+            if (!softmax_sync(mi, xphase)) return;
+            float top = -INFINITY;
+            for (int t = 0; t < states; ++t) top = fmaxf(top, ml[t * block + rr].x);
+            const float f = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top);
+            int dc = 128;  // channels per pass: what fits the scratch space
+            while (states * rows * dc * 4 > kScratchBytes - 2048 && dc > 16) dc >>= 1;
+            const int quads = dc / 4;
+            for (int d0 = 0; d0 < kHeadDim; d0 += dc) {
+                for (int c = 0; c < dc; c += 16) {
+                    float o[32];
+                    if (mine > 0) {
+                        tmem_ld16(o_addr + d0 + c, o);
+                        tmem_wait_ld();
+                    }
+                    if (live) {
+                        float4* dst = reinterpret_cast<float4*>(data) + (state * rows + rr) * quads;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float4 v = {0.f, 0.f, 0.f, 0.f};
+                            if (f > 0.f) v = {o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
+                            dst[(c / 4 + i) ^ (rr & 3)] = v;
+                        }
+                    }
+                }
+                if (!softmax_sync(mi, xphase)) return;
+                for (int it = threadIdx.x; it < rows * quads; it += 256) {
+                    const int r = it / quads, c4 = it - r * quads;
+                    float mx = -INFINITY, sum = 0.f;
+                    for (int t = 0; t < states; ++t) mx = fmaxf(mx, ml[t * block + r].x);
+                    float4 v = {0.f, 0.f, 0.f, 0.f};
+                    for (int t = 0; t < states; ++t) {
+                        const float2 e = ml[t * block + r];
+                        if (e.x > -INFINITY) sum += e.y * fast_exp2(e.x - mx);
+                        const float4 a = reinterpret_cast<const float4*>(data)[(t * rows + r) * quads + (c4 ^ (r & 3))];
+                        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                    }
+                    const int tk = r / p.group, h = g.head * p.group + r - tk * p.group;
+                    if (d0 == 0 && c4 == 0) store_ml(p, g, g.tok0 + tk, h, r, mx, sum);
+                    store_row(p, g, g.tok0 + tk, h, r, d0 + 4 * c4, v, sum > 0.f ? 1.f / sum : 0.f);
+                }
+                if (!softmax_sync(mi, xphase)) return;
+            }
+            fence_async_smem();  // the next query tile may be copied over the scratch space
+        }
+        tcgen05_fence_before();
+        warp_arrive(&mi->segempty[slot]);
+    }
+}
+
+// ---- matrix instructions -------------------------------------------------------
+
+template <int FMT>
+__device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_t tmem) {
+    constexpr int ring = Layout<FMT>::ring;
+    constexpr uint32_t id_qk = mma_idesc_f16(128, 128, false), id_pv = mma_idesc_f16(128, 128, true);
+    const int lane = threadIdx.x & 31;
+    const uint32_t q_addr = smem_addr(smem), r_addr = q_addr + 2 * kTileBytes;
+    uint32_t pos = 0, ph[2] = {0, 0};  // ring entries taken; P tiles per stream
+    auto wait_entry = [&](uint32_t e) { return warp_wait(&mi->full[e % ring], (e / ring) & 1, mi); };
+    auto qk = [&](int stream, int qslot, uint32_t e) {
+        tcgen05_fence_after();
+        if (lane == 0) {
+            const uint32_t a = q_addr + qslot * kTileBytes, b = r_addr + (e % ring) * kTileBytes;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t off = (i >> 2) * kHalfTile + (i & 3) * 32;
+                mma_f16_ss(tmem + stream * 128, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), id_qk, i > 0);
+            }
+            mma_commit(&mi->sfull[stream]);
+        }
+        __syncwarp();
+    };
+    auto pv = [&](int stream, uint32_t e, bool first) {
+        tcgen05_fence_after();
+        if (lane == 0) {
+            const uint32_t b = r_addr + (e % ring) * kTileBytes;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                mma_f16_ts(tmem + 256 + stream * 128, tmem + stream * 128 + i * 8, smem_desc(b + i * 2048, kHalfTile, 1024),
+                           id_pv, !first || i > 0);
+            mma_commit(&mi->odone[stream]);
+        }
+        __syncwarp();
+    };
+    auto release = [&](uint32_t e) {
+        if (lane == 0) mma_commit(&mi->empty[e % ring]);
+        __syncwarp();
+    };
+    // fp16 V rows that no row of the unit sees may hold anything (the end of a
+    // page, tokens that left the window): 0 * NaN would reach the sums
+    auto clean = [&](const Segment& g, int tile, uint32_t e) {
+        if (FMT != kF16) return;  // the conversion writes zeros there
+        const int j0 = tile * kTile;
+        if ((j0 >= g.vlo && j0 + kTile - 1 <= g.vhi) || (j0 >= g.fk && j0 + kTile <= g.pfx)) return;
+        unsigned char* v = smem + 2 * kTileBytes + (e % ring) * kTileBytes;
+        for (int i = lane >> 3; i < 2 * kTile; i += 4) {
+            const int r = i >> 1;
+            if (!g.seen(j0 + r))
+                *reinterpret_cast<uint4*>(v + (i & 1) * kHalfTile + r * 128 + (lane & 7) * 16) = uint4{0, 0, 0, 0};
+        }
+        fence_async_smem();
+        __syncwarp();
+    };
+    for (uint32_t k = 0, qk_seg = 0;; ++k) {
+        const int slot = k % kSegs;
+        if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
+        const Segment& g = mi->seg[slot];
+        if (!g.valid) return;
+        const int n = g.t1 - g.t0;
+        if (n > 0) {
+            if (!warp_wait(&mi->qfull, qk_seg++ & 1, mi)) return;
+            if (g.rep == 0) {
+                if (!wait_entry(pos)) return;
+                qk(0, 0, pos);
+                qk(1, 1, pos);
+                release(pos);
+                ++pos;
+                if (n == 1 && lane == 0) mma_commit(&mi->qempty);
+                for (int i = 0; i < n; ++i) {
+                    const uint32_t ve = pos, ke = pos + 1;
+                    const bool more = i + 1 < n;
+                    if (!wait_entry(ve)) return;
+                    clean(g, g.tile(g.t0 + i), ve);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        if (!warp_wait(&mi->pready[s], ph[s]++ & 1, mi)) return;
+                        pv(s, ve, i == 0);
+                        if (more) {
+                            if (s == 0 && !wait_entry(ke)) return;
+                            qk(s, s, ke);
+                        }
+                    }
+                    release(ve);
+                    if (more) {
+                        release(ke);
+                        if (i + 2 == n && lane == 0) mma_commit(&mi->qempty);
+                    }
+                    pos += more ? 2 : 1;
+                }
+            } else {
+                for (int s = 0; s < min(n, 2); ++s) {
+                    if (!wait_entry(pos)) return;
+                    qk(s, 0, pos);
+                    release(pos);
+                    ++pos;
+                }
+                if (n <= 2 && lane == 0) mma_commit(&mi->qempty);
+                for (int i = 0; i < n; ++i) {
+                    const int s = i & 1;
+                    if (!wait_entry(pos)) return;
+                    clean(g, g.tile(g.t0 + i), pos);
+                    if (!warp_wait(&mi->pready[s], ph[s]++ & 1, mi)) return;
+                    pv(s, pos, i < 2);
+                    release(pos);
+                    ++pos;
+                    if (i + 2 < n) {
+                        if (!wait_entry(pos)) return;
+                        qk(s, 0, pos);
+                        release(pos);
+                        ++pos;
+                        if (i + 3 == n && lane == 0) mma_commit(&mi->qempty);
+                    }
+                }
+            }
+        }
+        warp_arrive(&mi->segempty[slot]);
+    }
+}
+
+// ---- copies --------------------------------------------------------------------
+
+// Ring order, shared with the consumers: K of the first L tiles (wide units 1,
+// narrow units 2), then V_i, K_{i + L} for every tile i.
+template <int FMT>
+__device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const Maps& maps) {
+    constexpr int ring = FMT == kF16 ? Layout<FMT>::ring : kRaw;
+    uint64_t* const full = FMT == kF16 ? mi->full : mi->rfull;
+    uint64_t* const empty = FMT == kF16 ? mi->empty : mi->rempty;
+    const int lane = threadIdx.x & 31;
+    const int subs = kTile / p.box_rows;                       // boxes of a tile
+    const int sub = FMT == kF16 ? lane >> 1 : lane;            // this lane's box
+    uint32_t pos = 0, q_seg = 0;  // tiles and query loads so far
+    uint32_t narrow = 0;          // 1 + the last narrow segment
+    for (uint32_t k = 0;; ++k) {
+        const int slot = k % kSegs;
+        if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) break;
+        const Segment& g = mi->seg[slot];
+        if (!g.valid) break;
+        const int n = g.t1 - g.t0;
+        bool ok = true;
+        if (n > 0) {
+            // queries: the last segment's score tiles are done with the first
+            // slot; its epilogue with the scratch space in the second
+            if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
+            if (g.rep == 0 && narrow && k - (narrow - 1) < kSegs &&
+                !warp_wait(&mi->segempty[(narrow - 1) % kSegs], ((narrow - 1) / kSegs) & 1, mi))
+                break;
+            ++q_seg;
+            const int copies = g.rep ? g.rep : 2, block = g.rep ? kTile / g.rep : kTile;
+            const int toks = block / p.group;
+            const CUtensorMap* qm = &maps.q[g.rep == 4 ? 2 : g.rep == 2 ? 1 : 0];
+            if (lane == 0) mbar_arrive_expect_tx(&mi->qfull, static_cast<uint32_t>(copies * toks * p.group * 256));
+            __syncwarp();
+            if (lane < 2 * copies) {
+                const int c = lane >> 1, half = lane & 1;
+                unsigned char* dst = smem + (g.rep ? c * block * 128 : c * kTileBytes) + half * kHalfTile;
+                tma_load_3d(dst, qm, half * 64, g.head * p.group, g.tok0 + (g.rep ? 0 : c * toks), &mi->qfull);
+            }
+            // page of this lane's box in tile i of the list; -2: nothing there is seen
+            auto page = [&](int i) {
+                if (i >= g.t1 || sub >= subs) return -2;
+                const int j = g.tile(i) * kTile + sub * p.box_rows, e = j + p.box_rows - 1;
+                if (!((e >= g.vlo && j <= g.vhi) || (e >= g.fk && j < g.pfx))) return -2;
+                const KeySet& ks = p.set[g.set];
+                return __ldg(ks.tables + static_cast<size_t>(g.seq) * ks.width + j / p.block_size);
+            };
+            auto load = [&](bool v, int i, int pg) {
+                const int st = pos % ring;
+                if (pos >= ring && !warp_wait(&empty[st], (pos / ring - 1) & 1, mi)) return false;
+                ++pos;
+                const bool bad = pg != -2 && (pg < 0 || pg >= p.num_blocks);
+                if (bad) atomicCAS(&g_attention_error, 0, static_cast<int>(kDevBadBlock));
+                const bool there = pg >= 0 && !bad;
+                const int j = g.tile(i) * kTile + sub * p.box_rows;
+                // a row past the end reads as zeros
+                const int row = there ? (pg * p.n_kv + g.head) * p.block_size + j % p.block_size : p.total_rows;
+                const CUtensorMap* map = v ? &maps.v : &maps.k;
+                if (FMT == kF16) {
+                    if (lane == 0) mbar_arrive_expect_tx(&full[st], kTileBytes);
+                    __syncwarp();
+                    if (sub < subs)
+                        tma_load_2d(smem + 2 * kTileBytes + st * kTileBytes + (lane & 1) * kHalfTile +
+                                        sub * p.box_rows * 128,
+                                    map, (lane & 1) * 64, row, &full[st]);
+                } else {
+                    const unsigned here = __ballot_sync(kFull, there && sub < subs);
+                    if (lane == 0) {
+                        mi->bad[st] = ~here;
+                        mbar_arrive_expect_tx(&full[st], kTile * kHeadDim + __popc(here) * p.box_rows * 2);
+                    }
+                    __syncwarp();
+                    if (sub < subs) {
+                        unsigned char* dst = smem + Layout<FMT>::raw + st * kRawBytes;
+                        tma_load_2d(dst + sub * p.box_rows * kHeadDim, map, 0, row, &full[st]);
+                        if (there)
+                            bulk_g2s_plain(dst + kTile * kHeadDim + sub * p.box_rows * 2, (v ? p.v_scale : p.k_scale) + row,
+                                           p.box_rows * 2, &full[st]);
+                    }
+                }
+                __syncwarp();
+                return true;
+            };
+            const int L = g.rep ? 2 : 1;
+            int e0 = page(g.t0), e1 = page(g.t0 + 1), e2 = page(g.t0 + 2);
+            ok = load(false, g.t0, e0);
+            if (ok && L == 2 && n > 1) ok = load(false, g.t0 + 1, e1);
+            for (int i = g.t0; ok && i < g.t1; ++i) {
+                const int e3 = page(i + 3);
+                ok = load(true, i, e0);
+                if (ok && i + L < g.t1) ok = load(false, i + L, L == 2 ? e2 : e1);
+                e0 = e1;
+                e1 = e2;
+                e2 = e3;
+            }
+        }
+        if (!ok) break;
+        if (g.rep) narrow = k + 1;
+        warp_arrive(&mi->segempty[slot]);
+    }
+    // Leave no copy in flight: after an abort nobody else waits for them.
+    if (*reinterpret_cast<volatile int*>(&mi->abort)) {
+        for (uint32_t e = pos > ring ? pos - ring : 0; e < pos; ++e)
+            for (uint32_t i = 0; i < kPolls && !poll(&full[e % ring], (e / ring) & 1); ++i) {}
+        if (q_seg > 0)
+            for (uint32_t i = 0; i < kPolls && !poll(&mi->qfull, (q_seg - 1) & 1); ++i) {}
+    }
+}
+
+// ---- INT8 conversion -------------------------------------------------------------
+
+__device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem) {
+    constexpr int ring = Layout<kI8>::ring;
+    const int t = threadIdx.x & 127;
+    const int c = t & 7, r0 = t >> 3;  // 16 channels of rows r0, r0 + 16, ...
+    uint32_t pos = 0;
+    auto convert = [&](const Segment& g, int tile) {
+        const int st = pos % kRaw, d = pos % ring;
+        if (!warp_wait(&mi->rfull[st], (pos / kRaw) & 1, mi)) return false;
+        if (pos >= ring && !warp_wait(&mi->empty[d], (pos / ring - 1) & 1, mi)) return false;
+        const unsigned char* src = smem + Layout<kI8>::raw + st * kRawBytes;
+        const __half* scale = reinterpret_cast<const __half*>(src + kTile * kHeadDim);
+        unsigned char* dst = smem + 2 * kTileBytes + d * kTileBytes + (c >> 2) * kHalfTile;
+        const uint32_t bad = mi->bad[st];
+        const int j0 = tile * kTile;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + 16 * i;
+            const uint4 w = *reinterpret_cast<const uint4*>(src + r * kHeadDim + c * 16);
+            const half2 s = __half2half2(scale[r]);
+            const bool keep = g.seen(j0 + r) && !((bad >> (r / p.box_rows)) & 1);
+            uint32_t o[8];
+            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                half2 a, b;
+                i8x4_to_h2(in[q], a, b);
+                o[2 * q] = keep ? as_u32(__hmul2(a, s)) : 0u;
+                o[2 * q + 1] = keep ? as_u32(__hmul2(b, s)) : 0u;
+            }
+            unsigned char* line = dst + r * 128;
+            const int x = (c & 3) * 2;
+            *reinterpret_cast<uint4*>(line + ((x ^ (r & 7)) << 4)) = uint4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<uint4*>(line + (((x + 1) ^ (r & 7)) << 4)) = uint4{o[4], o[5], o[6], o[7]};
+        }
+        fence_async_smem();
+        warp_arrive(&mi->rempty[st]);
+        warp_arrive(&mi->full[d]);
+        ++pos;
+        return true;
+    };
+    for (uint32_t k = 0;; ++k) {
+        const int slot = k % kSegs;
+        if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
+        const Segment& g = mi->seg[slot];
+        if (!g.valid) return;
+        const int n = g.t1 - g.t0, L = g.rep ? 2 : 1;
+        for (int i = 0; i < min(n, L); ++i)
+            if (!convert(g, g.tile(g.t0 + i))) return;
+        for (int i = 0; i < n; ++i) {
+            if (!convert(g, g.tile(g.t0 + i))) return;
+            if (i + L < n && !convert(g, g.tile(g.t0 + i + L))) return;
+        }
+        warp_arrive(&mi->segempty[slot]);
+    }
+}
+
+// ---- schedule --------------------------------------------------------------------
+
+// Cost of a unit in tiles (an empty one still writes its rows).
+__device__ __forceinline__ int unit_cost(const Segment& s) { return max(s.nt, 1); }
+
+// CTAs that the tiles are split over: none of them goes without, so the CTAs
+// from a split unit's first to its last all hold a part of it.
+__device__ __forceinline__ long long sharing_ctas(const Params& p, long long total) {
+    return min(static_cast<long long>(p.grid), total);
+}
+
+// This CTA's share [start, start + count) of all units' tiles, and the unit it
+// begins in: a block-wide prefix sum over the unit numbers.
+template <int THREADS>
+__device__ void plan(const Params& p, Misc* mi) {
+    const int n_ids = p.set[0].n_ids + (p.n_sets > 1 ? p.set[1].n_ids : 0);
+    const int chunk = (n_ids + THREADS - 1) / THREADS;
+    const int id0 = threadIdx.x * chunk, id1 = min(id0 + chunk, n_ids);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long mine = 0;
+    Segment s;
+    for (int id = id0; id < id1; ++id)
+        if (make_unit(p, id, s)) mine += unit_cost(s);
+    long long incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long o = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += o;
+    }
+    if (lane == 31) mi->scan[warp] = incl;
+    __syncthreads();
+    long long before = 0, total = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += mi->scan[w];
+        total += mi->scan[w];
+    }
+    total *= p.n_kv;
+    const long long ctas = sharing_ctas(p, total);
+    const long long a = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0;
+    const long long e = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
+    const long long lo = (before + incl - mine) * p.n_kv, hi = (before + incl) * p.n_kv;
+    if (threadIdx.x == 0) {
+        mi->start = a;
+        mi->count = e - a;
+        mi->total = total;
+    }
+    if (e > a && lo <= a && a < hi) {
+        long long at = lo;
+        for (int id = id0; id < id1; ++id) {
+            if (!make_unit(p, id, s)) continue;
+            const int c = unit_cost(s);
+            if (a < at + static_cast<long long>(c) * p.n_kv) {
+                mi->start_id = id;
+                mi->start_head = static_cast<int>((a - at) / c);
+                mi->start_off = static_cast<int>((a - at) % c);
+                break;
+            }
+            at += static_cast<long long>(c) * p.n_kv;
+        }
+    }
+}
+
+__device__ void schedule_role(const Params& p, Misc* mi) {
+    const int lane = threadIdx.x & 31;
+    long long left = mi->count, at = mi->start;
+    const long long total = mi->total;
+    const int n_ids = p.set[0].n_ids + (p.n_sets > 1 ? p.set[1].n_ids : 0);
+    int id = mi->start_id, head = mi->start_head, off = mi->start_off;
+    bool split = false;
+    Segment s;
+    if (left > 0) make_unit(p, id, s);
+    for (uint32_t k = 0;; ++k) {
+        const int slot = k % kSegs;
+        if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
+        if (left <= 0) {
+            if (lane == 0) mi->seg[slot].valid = 0;
+            warp_arrive(&mi->segfull[slot]);
+            break;
+        }
+        const int cost = unit_cost(s);
+        const int n = static_cast<int>(min(left, static_cast<long long>(cost - off)));
+        s.valid = 1;
+        s.head = head;
+        s.t0 = s.nt ? off : 0;
+        s.t1 = s.nt ? off + n : 0;
+        const bool whole = off == 0 && n == cost;
+        s.dest = !whole ? kSlot : p.shared ? kRowBuf : kDirect;
+        if (lane == 0) {
+            mi->seg[slot] = s;
+            if (off == 0) {
+                const long long end = at + cost - 1;  // its last tile's owner finishes the unit
+                const int last = whole ? -1 : static_cast<int>(((end + 1) * sharing_ctas(p, total) - 1) / total);
+                if (p.shared) p.units[static_cast<size_t>(id) * p.n_kv + head] = {static_cast<int>(blockIdx.x), last};
+                if (!whole) p.split[blockIdx.x] = {s.tok0, s.ntok, head, last};
+            }
+        }
+        split |= off == 0 && !whole;
+        warp_arrive(&mi->segfull[slot]);
+        at += n;
+        left -= n;
+        off = 0;
+        if (left > 0 && ++head == p.n_kv) {
+            head = 0;
+            do ++id; while (id < n_ids && !make_unit(p, id, s));
+            if (id >= n_ids) left = 0;
+        }
+    }
+    if (!split && lane == 0) p.split[blockIdx.x] = {0, 0, 0, -1};
+}
+
+template <int FMT, bool MOD>
+__global__ void __launch_bounds__(Layout<FMT>::threads, 1)
+    attention_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+    using Lay = Layout<FMT>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    Misc* mi = reinterpret_cast<Misc*>(smem + Lay::misc);
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        const int readers = FMT == kF16 ? 10 : 14;  // warps that read a segment
+        for (int i = 0; i < Lay::ring; ++i) {
+            mbar_init(&mi->full[i], FMT == kF16 ? 1 : 4);
+            mbar_init(&mi->empty[i], 1);
+        }
+        for (int i = 0; i < kRaw; ++i) {
+            mbar_init(&mi->rfull[i], 1);
+            mbar_init(&mi->rempty[i], 4);
+        }
+        mbar_init(&mi->qfull, 1);
+        mbar_init(&mi->qempty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&mi->sfull[i], 1);
+            mbar_init(&mi->pready[i], 4);
+            mbar_init(&mi->odone[i], 1);
+        }
+        for (int i = 0; i < kSegs; ++i) {
+            mbar_init(&mi->segfull[i], 1);
+            mbar_init(&mi->segempty[i], readers);
+        }
+        mbar_init(&mi->xbar, 8);
+        mbar_init(&mi->drain, 1);
+        mi->abort = 0;
+        fence_barrier_init();
+        tma_prefetch_map(&maps.k);
+        tma_prefetch_map(&maps.v);
+    }
+    if (warp == 9) tmem_alloc(&mi->tmem, 512);
+    grid_dependency_wait();
+    grid_launch_dependents();
+    plan<Lay::threads>(p, mi);
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = mi->tmem;
+
+    if (warp < 8) {
+        regs_inc<Lay::softmax_regs>();
+        softmax_role<MOD>(p, mi, smem, tmem);
+    } else if (warp < 12) {
+        regs_dec<Lay::other_regs>();
+        if (warp == 8) {
+            copy_role<FMT>(p, mi, smem, maps);
+        } else if (warp == 9) {
+            mma_role<FMT>(p, mi, smem, tmem);
+            if (*reinterpret_cast<volatile int*>(&mi->abort)) {  // wait out what is still running
+                if ((threadIdx.x & 31) == 0) mma_commit(&mi->drain);
+                __syncwarp();
+                for (uint32_t i = 0; i < kPolls && !poll(&mi->drain, 0); ++i) {}
+            }
+        } else if (warp == 10) {
+            schedule_role(p, mi);
+        }
+    } else {
+        if constexpr (FMT != kF16) {
+            regs_dec<Lay::convert_regs>();
+            convert_role(p, mi, smem);
+        }
+    }
+    __syncwarp();
+    tcgen05_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tcgen05_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- joining -----------------------------------------------------------------------
+
+// Adds the partial states of one row, this lane's four channels, in CTA order.
+struct Join {
+    float m = -INFINITY, l = 0.f;
+    float4 v = {0.f, 0.f, 0.f, 0.f};
+    __device__ void add(const float2* ml, const float* part, size_t r, int lane) {
+        const float2 e = ml[r];
+        if (e.y <= 0.f) return;
+        const float4 o = *reinterpret_cast<const float4*>(part + r * kHeadDim + lane * 4);
+        const float up = fmaxf(m, e.x);
+        const float a = m == -INFINITY ? 0.f : fast_exp2(m - up), b = fast_exp2(e.x - up);
+        m = up;
+        l = l * a + e.y * b;
+        v = {v.x * a + o.x * b, v.y * a + o.y * b, v.z * a + o.z * b, v.w * a + o.w * b};
+    }
+    __device__ void add_slots(const Params& p, int first, int last, int unit_row, int lane) {
+        for (int c = first; c <= last; ++c)
+            add(p.part_ml, p.part, static_cast<size_t>(2 * c + (c == first)) * p.slot_rows + unit_row, lane);
+    }
+    __device__ void store(const Params& p, size_t row, int lane) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        uint2 u;
+        u.x = pack_f16(v.x * inv, v.y * inv);
+        u.y = pack_f16(v.z * inv, v.w * inv);
+        *reinterpret_cast<uint2*>(p.out + row * kHeadDim + lane * 4) = u;
+    }
+};
+
+// One warp per row of a split unit; blockIdx.x is the CTA the unit starts in.
+__global__ void __launch_bounds__(256) join_split_kernel(const __grid_constant__ Params p) {
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int4 u = p.split[blockIdx.x];
+    if (u.w >= 0) {
+        const int rows = u.y * p.group;
+        for (int r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
+            Join j;
+            j.add_slots(p, blockIdx.x, u.w, r, lane);
+            const int tk = r / p.group;
+            j.store(p, static_cast<size_t>(u.x + tk) * p.n_heads + u.z * p.group + r - tk * p.group, lane);
+        }
+    }
+    if (p.zero_tail) {  // tokens of no sequence
+        const KeySet& k = p.set[0];
+        const long long lo = cu_at(k, 0, p.n_tokens), hi = cu_at(k, k.n_seq, p.n_tokens);
+        const long long pad = (lo + p.n_tokens - hi) * p.n_heads;
+        const long long step = static_cast<long long>(gridDim.x) * gridDim.y * 8;
+        for (long long i = (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * 8 + warp; i < pad; i += step) {
+            const long long row = i < lo * p.n_heads ? i : i + (hi - lo) * p.n_heads;
+            *reinterpret_cast<uint2*>(p.out + row * kHeadDim + lane * 4) = uint2{0, 0};
+        }
+    }
+}
+
+// One warp per (token, query head): the shared prefix's state, then its own.
+__global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ Params p) {
+    grid_dependency_wait();
+    const int lane = threadIdx.x & 31;
+    const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (row >= static_cast<long long>(p.n_tokens) * p.n_heads) return;
+    const int tok = static_cast<int>(row / p.n_heads), hq = static_cast<int>(row - static_cast<long long>(tok) * p.n_heads);
+    const int h = hq / p.group, g = hq - h * p.group;
+    const int unit = 2 * (kTile / p.group);
+    Join j;
+    const KeySet& k = p.set[0];
+    int lo = 0, hi = k.n_seq - 1;  // the group that holds this token
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cu_at(k, mid, p.n_tokens) <= tok) lo = mid; else hi = mid - 1;
+    }
+    const int c0 = cu_at(k, lo, p.n_tokens);
+    if (k.n_seq > 0 && tok >= c0 && tok < cu_at(k, lo + 1, p.n_tokens)) {
+        const int at = (tok - c0) / unit;
+        const int2 u = p.units[static_cast<size_t>(c0 / unit + lo + at) * p.n_kv + h];
+        if (u.y < 0)
+            j.add(p.row_ml, p.rowbuf, row, lane);
+        else
+            j.add_slots(p, u.x, u.y, (tok - c0 - at * unit) * p.group + g, lane);
+    }
+    const int2 u = p.units[static_cast<size_t>(k.n_ids + tok) * p.n_kv + h];
+    if (u.y < 0)
+        j.add(p.row_ml, p.rowbuf, static_cast<size_t>(p.n_tokens) * p.n_heads + row, lane);
+    else
+        j.add_slots(p, u.x, u.y, g, lane);
+    j.store(p, row, lane);
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// cuTensorMapEncodeTiled, looked up in the driver once (the library does not
+// link against it, so it loads on machines without a GPU).
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeFn>(f);
+    }();
+    return fn;
+}
+
+bool encode(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
+            const cuuint64_t* strides, const cuuint32_t* box, bool swizzle, std::string& err) {
+    const cuuint32_t one[3] = {1, 1, 1};
+    const CUresult r = encode_fn()(m, dt, rank, const_cast<void*>(base), dims, strides, box, one,
+                                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) err = "cuTensorMapEncodeTiled failed (" + std::to_string(static_cast<int>(r)) + ")";
+    return r == CUDA_SUCCESS;
+}
+
+struct Plan {  // sizes that the workspace and the launch agree on
+    int per, unit, n_ids0, n_ids1, slot_rows;
+    size_t part, ml, split, rowbuf, row_ml, units, bytes;
+};
+Plan make_plan(int64_t n_tokens, int64_t n_heads, int64_t n_kv, int64_t n_seq0, bool shared, int grid) {
+    Plan w{};
+    const int64_t group = n_heads / n_kv;
+    w.per = static_cast<int>(kTile / group);
+    w.unit = 2 * w.per;
+    w.n_ids0 = static_cast<int>(n_tokens / w.unit + n_seq0);
+    w.n_ids1 = shared ? static_cast<int>(n_tokens) : 0;
+    w.slot_rows = static_cast<int>(std::min<int64_t>(w.unit, n_tokens) * group);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at = align_up(at + bytes, 256);
+        return o;
+    };
+    w.part = take(size_t{2} * grid * w.slot_rows * kHeadDim * 4);
+    w.ml = take(size_t{2} * grid * w.slot_rows * sizeof(float2));
+    w.split = take(size_t{1} * grid * sizeof(int4));
+    if (shared) {
+        const size_t rows = static_cast<size_t>(n_tokens) * n_heads;
+        w.rowbuf = take(2 * rows * kHeadDim * 4);
+        w.row_ml = take(2 * rows * sizeof(float2));
+        w.units = take(static_cast<size_t>(w.n_ids0 + w.n_ids1) * n_kv * sizeof(int2));
+    }
+    w.bytes = at;
+    return w;
+}
+
+template <int FMT, bool MOD>
+lik_status launch(const Maps& maps, const Params& p, cudaStream_t stream, std::string& err) {
+    using Lay = Layout<FMT>;
+    auto kern = attention_kernel<FMT, MOD>;
+    static std::mutex mu;
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!ready[dev & 63]) {
+            cudaFuncAttributes fa;
+            e = cudaFuncGetAttributes(&fa, kern);
+            if (e == cudaSuccess && fa.numRegs != Lay::base) {
+                err = "attention kernel: built with " + std::to_string(fa.numRegs) + " registers, its shares need " +
+                      std::to_string(Lay::base);
+                return LIK_ERR_CUDA;
+            }
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::bytes);
+            if (e == cudaSuccess) ready[dev & 63] = true;
+        }
+    }
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(p.grid);
+        cfg.blockDim = dim3(Lay::threads);
+        cfg.dynamicSmemBytes = Lay::bytes;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, kern, maps, p);
+        if (e == cudaSuccess) {
+            cfg.blockDim = dim3(256);
+            cfg.dynamicSmemBytes = 0;
+            if (p.shared) {
+                const long long rows = static_cast<long long>(p.n_tokens) * p.n_heads;
+                cfg.gridDim = dim3(static_cast<unsigned>((rows + 7) / 8));
+                e = cudaLaunchKernelEx(&cfg, join_rows_kernel, p);
+            } else {
+                cfg.gridDim = dim3(p.grid, static_cast<unsigned>((p.slot_rows + 31) / 32));
+                e = cudaLaunchKernelEx(&cfg, join_split_kernel, p);
+            }
+        }
+    }
+    if (e != cudaSuccess) {
+        err = std::string("attention launch: ") + cudaGetErrorString(e);
+        return LIK_ERR_CUDA;
+    }
+    return LIK_OK;
+}
+
+}  // namespace
+
+size_t attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t n_kv, int64_t n_groups, bool shared,
+                                 int sm_count) {
+    return make_plan(n_tokens, n_heads, n_kv, shared ? n_groups : 0, shared, sm_count).bytes;
+}
+
+void* attention_error_word(std::string& err) {
+    void* a = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&a, g_attention_error);
+    if (e != cudaSuccess) err = std::string("cudaGetSymbolAddress: ") + cudaGetErrorString(e);
+    return e == cudaSuccess ? a : nullptr;
+}
+
+lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::string& err) {
+    DeviceInfo di;
+    if (!device_info(di, err)) return LIK_ERR_CUDA;
+    if (!encode_fn()) {
+        err = "cuTensorMapEncodeTiled not found in the driver";
+        return LIK_ERR_CUDA;
+    }
+    const bool shared = a.prefix_tables != nullptr;
+    const Plan w = make_plan(a.n_tokens, a.n_heads, a.n_kv_heads, shared ? a.n_groups : a.n_seqs, shared, di.sm_count);
+    if (!a.workspace || a.workspace_bytes < w.bytes) {
+        err = "attention workspace of " + std::to_string(w.bytes) + " bytes needed";
+        return LIK_ERR_WORKSPACE;
+    }
+    Params p{};
+    if (shared) {
+        p.set[0] = {a.cu_seqlens, a.prefix_lens, a.prefix_tables, a.context_lens, static_cast<int>(a.n_groups),
+                    static_cast<int>(a.prefix_blocks), w.n_ids0, 0};
+        p.set[1] = {nullptr, a.context_lens, a.block_tables, nullptr, static_cast<int>(a.n_tokens),
+                    static_cast<int>(a.max_blocks), w.n_ids1, 0};
+        p.n_sets = 2;
+    } else {
+        p.set[0] = {a.cu_seqlens, a.context_lens, a.block_tables, nullptr, static_cast<int>(a.n_seqs),
+                    static_cast<int>(a.max_blocks), w.n_ids0, a.causal ? 1 : 0};
+        p.n_sets = 1;
+        p.prefix_lens = a.prefix_lens;
+        p.first_keys = a.first_keys;
+        p.window = static_cast<int>(a.window);
+    }
+    p.slopes = a.alibi_slopes;
+    p.scale = a.softmax_scale;
+    p.cap = a.softcap;
+    p.n_tokens = static_cast<int>(a.n_tokens);
+    p.n_heads = static_cast<int>(a.n_heads);
+    p.n_kv = static_cast<int>(a.n_kv_heads);
+    p.group = p.n_heads / p.n_kv;
+    p.num_blocks = static_cast<int>(a.num_blocks);
+    p.block_size = static_cast<int>(a.block_size);
+    p.box_rows = std::min(kTile, p.block_size & -p.block_size);  // boxes never cross a page
+    p.total_rows = static_cast<int>(a.num_blocks * a.n_kv_heads * a.block_size);
+    p.k_scale = static_cast<const __half*>(a.k_scale);
+    p.v_scale = static_cast<const __half*>(a.v_scale);
+    p.out = static_cast<__half*>(a.out);
+    p.shared = shared;
+    p.zero_tail = a.zero_tail;
+    p.slot_rows = w.slot_rows;
+    p.grid = di.sm_count;
+    unsigned char* ws = static_cast<unsigned char*>(a.workspace);
+    p.part = reinterpret_cast<float*>(ws + w.part);
+    p.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+    p.split = reinterpret_cast<int4*>(ws + w.split);
+    p.rowbuf = reinterpret_cast<float*>(ws + w.rowbuf);
+    p.row_ml = reinterpret_cast<float2*>(ws + w.row_ml);
+    p.units = reinterpret_cast<int2*>(ws + w.units);
+
+    Maps maps;
+    for (int i = 0; i < 3; ++i) {
+        const int toks = (kTile >> i) / p.group;
+        if (toks == 0) {
+            maps.q[i] = maps.q[0];
+            continue;
+        }
+        const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(a.n_heads), static_cast<cuuint64_t>(a.n_tokens)};
+        const cuuint64_t strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(a.q_token_stride) * 2};
+        const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(toks)};
+        if (!encode(&maps.q[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.q, dims, strides, box, true, err)) return LIK_ERR_CUDA;
+    }
+    const bool f16 = a.fmt == kF16;
+    const cuuint64_t dims[2] = {kHeadDim, static_cast<cuuint64_t>(p.total_rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(kHeadDim) * (f16 ? 2 : 1)};
+    const cuuint32_t box[2] = {f16 ? 64u : 128u, static_cast<cuuint32_t>(p.box_rows)};
+    const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    if (!encode(&maps.k, dt, 2, a.k, dims, strides, box, f16, err) || !encode(&maps.v, dt, 2, a.v, dims, strides, box, f16, err))
+        return LIK_ERR_CUDA;
+    const bool mod = p.cap > 0.f || p.slopes;
+    if (f16) return mod ? launch<kF16, true>(maps, p, stream, err) : launch<kF16, false>(maps, p, stream, err);
+    return mod ? launch<kI8, true>(maps, p, stream, err) : launch<kI8, false>(maps, p, stream, err);
+}
+
+}  // namespace lik

@@ -2,6 +2,7 @@
 // dispatch to the kernel launchers. Nothing here allocates device memory.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstring>
 #include <mutex>
 #include <string>
@@ -433,6 +434,167 @@ lik_status lik_decode_attention_paged(int kv_format, const void* q, const void* 
     a.softmax_scale = softmax_scale;
     a.workspace = workspace; a.workspace_bytes = workspace_bytes;
     return run_decode(a, stream);
+}
+
+lik_status lik_paged_append_rope(int k_format, int v_format, const void* q, int64_t q_token_stride, const void* k,
+                                 int64_t k_token_stride, const void* v, int64_t v_token_stride,
+                                 const int64_t* positions, int64_t n_axes, const int64_t* sections,
+                                 const float* inv_freq, int64_t n_freqs, int interleaved, const int64_t* slot_mapping,
+                                 void* q_out, int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                 void* k_cache, void* k_scale, void* v_cache, void* v_scale, void* v_zero,
+                                 int64_t num_blocks, int64_t block_size, void* stream) {
+    if (k_format != kF16 && k_format != kI8) return fail(LIK_ERR_UNSUPPORTED, "k_format must be fp16 or INT8 per token");
+    if (v_format < kF16 || v_format > kI4Asym) return fail(LIK_ERR_INVALID_ARGUMENT, "unknown v_format");
+    if (n_tokens < 0 || num_blocks < 0 || block_size <= 0 || block_size > (1 << 20))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "need n_tokens >= 0, num_blocks >= 0, 0 < block_size <= 2^20");
+    lik_status s = check_heads(n_tokens, n_heads, n_kv_heads, head_dim);
+    if (s != LIK_OK) return s;
+    if (n_freqs < 1 || n_freqs > kHeadDim / 2) return fail(LIK_ERR_INVALID_ARGUMENT, "need 1 <= n_freqs <= 64");
+    if (n_axes < 1 || n_axes > 4) return fail(LIK_ERR_INVALID_ARGUMENT, "need 1 to 4 position axes");
+    if (n_axes > 1 && !sections) return fail(LIK_ERR_INVALID_ARGUMENT, "several position axes need sections");
+    if (sections) {
+        int64_t sum = 0;
+        for (int64_t i = 0; i < n_axes; ++i) {
+            if (sections[i] < 0 || sections[i] > n_freqs) return fail(LIK_ERR_INVALID_ARGUMENT, "section out of range");
+            sum += sections[i];
+        }
+        if (sum != n_freqs) return fail(LIK_ERR_INVALID_ARGUMENT, "sections must sum to n_freqs");
+    }
+    if (n_tokens == 0) return LIK_OK;
+    if (n_tokens > 0x7fffffff || num_blocks > (int64_t{1} << 40))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "too many tokens or blocks");
+    for (const int64_t st : {q_token_stride, k_token_stride, v_token_stride})
+        if (st < 0 || st % 8 != 0) return fail(LIK_ERR_MISALIGNED, "token strides must be multiples of 8 elements");
+    if (!q || !k || !v || !positions || !inv_freq || !slot_mapping || !q_out || !k_cache || !v_cache)
+        return fail(LIK_ERR_INVALID_ARGUMENT, "null tensor pointer");
+    if ((k_format != kF16 && !k_scale) || (v_format != kF16 && !v_scale))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "null scale pointer");
+    if (v_format == kI4Asym && !v_zero) return fail(LIK_ERR_INVALID_ARGUMENT, "null zero-point pointer");
+    for (const void* t : {q, k, v, static_cast<const void*>(q_out), static_cast<const void*>(k_cache),
+                          static_cast<const void*>(v_cache)})
+        if (!aligned16(t)) return fail(LIK_ERR_MISALIGNED, "q, k, v, q_out and the caches must be 16-byte aligned");
+    RopeAppendArgs a;
+    a.q = q; a.k = k; a.v = v;
+    a.positions = positions; a.inv_freq = inv_freq; a.slot_mapping = slot_mapping; a.q_out = q_out;
+    a.k_cache = k_cache; a.v_cache = v_cache; a.k_scale = k_scale; a.v_scale = v_scale; a.v_zero = v_zero;
+    a.q_token_stride = q_token_stride; a.k_token_stride = k_token_stride; a.v_token_stride = v_token_stride;
+    a.n_tokens = n_tokens; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads;
+    a.num_blocks = num_blocks; a.block_size = block_size; a.n_freqs = n_freqs; a.n_axes = n_axes; a.sections = sections;
+    a.k_format = k_format; a.v_format = v_format; a.interleaved = interleaved != 0;
+    std::string err;
+    s = launch_rope_append(a, as_stream(stream), err);
+    return s == LIK_OK ? s : fail(s, err);
+}
+
+size_t lik_attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t n_kv_heads, int64_t n_groups) {
+    DeviceInfo di;
+    std::string err;
+    const int sms = device_info(di, err) ? di.sm_count : 256;
+    if (n_tokens < 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 128 ||
+        n_groups < 0)
+        return kWsErrBytes;
+    return std::max(attention_workspace_bytes(n_tokens, n_heads, n_kv_heads, n_groups, n_groups > 0, sms), kWsErrBytes);
+}
+
+// What both attention entry points check; `a` is filled up to the key sets.
+static lik_status check_attention(const AttentionArgs& a, int64_t head_dim) {
+    lik_status s = check_heads(a.n_tokens, a.n_heads, a.n_kv_heads, head_dim);
+    if (s != LIK_OK) return s;
+    if (a.fmt != kF16 && a.fmt != kI8) return fail(LIK_ERR_UNSUPPORTED, "only fp16 and INT8 caches supported");
+    if (a.n_heads / a.n_kv_heads > 128) return fail(LIK_ERR_UNSUPPORTED, "more than 128 query heads per KV head");
+    if (!(a.softmax_scale > 0.f) || !(a.softmax_scale < 1e30f))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and finite");
+    if (!(a.softcap >= 0.f) || !(a.softcap < 1e30f))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "softcap must be finite and >= 0 (0: none)");
+    if (a.window < 0 || a.window > (int64_t{1} << 30)) return fail(LIK_ERR_INVALID_ARGUMENT, "window out of range");
+    if (a.block_size <= 0 || a.block_size % 16 != 0 || a.block_size > (1 << 20))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "block_size must be a positive multiple of 16");
+    if (a.num_blocks < 1 || a.num_blocks > 0x7fffff7f / a.block_size / a.n_kv_heads)
+        return fail(LIK_ERR_INVALID_ARGUMENT, "need num_blocks >= 1 and fewer than 2^31 - 128 cache rows");
+    for (const int64_t w : {a.max_blocks, a.prefix_blocks})
+        if (w < 0 || w > (int64_t{1} << 30) / a.block_size)
+            return fail(LIK_ERR_INVALID_ARGUMENT, "block tables must span at most 2^30 positions");
+    if (a.n_seqs < 0 || a.n_groups < 0 || a.n_tokens > (int64_t{1} << 30) / a.n_heads || a.n_seqs > (int64_t{1} << 24) ||
+        a.n_groups > (int64_t{1} << 24))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "too many tokens or sequences");
+    if (a.q_token_stride < 0 || a.q_token_stride % 8 != 0 || a.q_token_stride > (int64_t{1} << 38))
+        return fail(LIK_ERR_MISALIGNED, "q_token_stride must be a multiple of 8 elements");
+    if (a.n_tokens > 1 && a.q_token_stride < a.n_heads * kHeadDim)
+        return fail(LIK_ERR_INVALID_ARGUMENT, "q_token_stride below n_heads * head_dim");
+    if (a.n_tokens == 0) return LIK_OK;
+    if (!a.q || !a.k || !a.v || !a.out || !a.cu_seqlens) return fail(LIK_ERR_INVALID_ARGUMENT, "null tensor pointer");
+    if (a.fmt == kI8 && (!a.k_scale || !a.v_scale)) return fail(LIK_ERR_INVALID_ARGUMENT, "null scale pointer");
+    for (const void* t : {a.q, a.k, a.v, static_cast<const void*>(a.out), a.k_scale, a.v_scale})
+        if (!aligned16(t)) return fail(LIK_ERR_MISALIGNED, "q, out, caches and scales must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(a.workspace) & 255)
+        return fail(LIK_ERR_MISALIGNED, "the workspace must be 256-byte aligned");
+    return LIK_OK;
+}
+
+static lik_status run_attention(const AttentionArgs& a, int64_t head_dim, void* stream) {
+    lik_status s = check_attention(a, head_dim);
+    if (s != LIK_OK || a.n_tokens == 0) return s;
+    std::string err;
+    s = launch_attention(a, as_stream(stream), err);
+    return s == LIK_OK ? s : fail(s, err);
+}
+
+lik_status lik_attention_paged(int kv_format, const void* q, int64_t q_token_stride, const void* k_cache,
+                               const void* v_cache, const void* k_scale, const void* v_scale,
+                               const int32_t* block_tables, const int32_t* context_lens, const int32_t* cu_seqlens_q,
+                               void* out, int64_t n_tokens, int64_t n_seqs, int64_t n_heads, int64_t n_kv_heads,
+                               int64_t head_dim, int64_t num_blocks, int64_t block_size, int64_t max_blocks_per_seq,
+                               float softmax_scale, int causal, int64_t window, float softcap,
+                               const float* alibi_slopes, const int32_t* prefix_lens, const int32_t* first_keys,
+                               int zero_tail, void* workspace, size_t workspace_bytes, void* stream) {
+    if (n_tokens > 0 && n_seqs > 0 && (!context_lens || (max_blocks_per_seq > 0 && !block_tables)))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "null block table or lengths");
+    AttentionArgs a;
+    a.fmt = kv_format;
+    a.q = q; a.k = k_cache; a.v = v_cache; a.k_scale = k_scale; a.v_scale = v_scale; a.out = out;
+    a.cu_seqlens = cu_seqlens_q; a.context_lens = context_lens; a.block_tables = block_tables;
+    a.prefix_lens = prefix_lens; a.first_keys = first_keys; a.alibi_slopes = alibi_slopes;
+    a.n_tokens = n_tokens; a.n_seqs = n_seqs; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads;
+    a.q_token_stride = q_token_stride;
+    a.num_blocks = num_blocks; a.block_size = block_size; a.max_blocks = max_blocks_per_seq;
+    a.window = window; a.causal = causal != 0; a.zero_tail = zero_tail != 0;
+    a.softmax_scale = softmax_scale; a.softcap = softcap;
+    a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+    return run_attention(a, head_dim, stream);
+}
+
+lik_status lik_attention_shared_prefix(int kv_format, const void* q, int64_t q_token_stride, const void* k_cache,
+                                       const void* v_cache, const void* k_scale, const void* v_scale,
+                                       const int32_t* prefix_tables, const int32_t* prefix_lens,
+                                       const int32_t* cu_groups, const int32_t* block_tables,
+                                       const int32_t* context_lens, void* out, int64_t batch, int64_t n_groups,
+                                       int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t num_blocks,
+                                       int64_t block_size, int64_t prefix_blocks, int64_t max_blocks_per_seq,
+                                       float softmax_scale, float softcap, const float* alibi_slopes, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    if (n_groups < 1 && batch > 0) return fail(LIK_ERR_INVALID_ARGUMENT, "need at least one prefix group");
+    if (batch > 0 && (!prefix_tables || !prefix_lens || !block_tables || !context_lens))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "null block table or lengths");
+    AttentionArgs a;
+    a.fmt = kv_format;
+    a.q = q; a.k = k_cache; a.v = v_cache; a.k_scale = k_scale; a.v_scale = v_scale; a.out = out;
+    a.cu_seqlens = cu_groups; a.context_lens = context_lens; a.block_tables = block_tables;
+    a.prefix_tables = prefix_tables; a.prefix_lens = prefix_lens; a.alibi_slopes = alibi_slopes;
+    a.n_tokens = batch; a.n_seqs = batch; a.n_groups = n_groups; a.n_heads = n_heads; a.n_kv_heads = n_kv_heads;
+    a.q_token_stride = q_token_stride;
+    a.num_blocks = num_blocks; a.block_size = block_size; a.max_blocks = max_blocks_per_seq;
+    a.prefix_blocks = prefix_blocks;
+    a.softmax_scale = softmax_scale; a.softcap = softcap;
+    a.workspace = workspace; a.workspace_bytes = workspace_bytes;
+    return run_attention(a, head_dim, stream);
+}
+
+lik_status lik_attention_check(void* stream, int* device_error) {
+    if (!device_error) return fail(LIK_ERR_INVALID_ARGUMENT, "device_error must be given");
+    std::string err;
+    void* word = attention_error_word(err);
+    if (!word) return fail(LIK_ERR_CUDA, err);
+    return check_error_word(word, sizeof(int), as_stream(stream), device_error);
 }
 
 }  // extern "C"

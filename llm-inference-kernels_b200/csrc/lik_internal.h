@@ -36,6 +36,60 @@ struct DecodeArgs {
     size_t workspace_bytes = 0;
 };
 
+// lik_attention_paged (prefix_tables null) and lik_attention_shared_prefix.
+struct AttentionArgs {
+    int fmt = kF16;  // kF16 or kI8
+    const void* q = nullptr;
+    const void* k = nullptr;
+    const void* v = nullptr;
+    const void* k_scale = nullptr;
+    const void* v_scale = nullptr;
+    void* out = nullptr;
+    const int* cu_seqlens = nullptr;    // tokens of each sequence, or requests of each prefix group
+    const int* context_lens = nullptr;
+    const int* block_tables = nullptr;
+    const int* prefix_tables = nullptr;
+    const int* prefix_lens = nullptr;   // visible prefix per sequence, or keys of each prefix group
+    const int* first_keys = nullptr;
+    const float* alibi_slopes = nullptr;
+    int64_t n_tokens = 0, n_seqs = 0, n_groups = 0;
+    int64_t n_heads = 0, n_kv_heads = 0, q_token_stride = 0;
+    int64_t num_blocks = 0, block_size = 0, max_blocks = 0, prefix_blocks = 0;
+    int64_t window = 0;
+    bool causal = true, zero_tail = false;
+    float softmax_scale = 0.f, softcap = 0.f;
+    void* workspace = nullptr;
+    size_t workspace_bytes = 0;
+};
+// lik_paged_append_rope
+struct RopeAppendArgs {
+    const void* q = nullptr;
+    const void* k = nullptr;
+    const void* v = nullptr;
+    const int64_t* positions = nullptr;  // [n_axes, n_tokens]
+    const float* inv_freq = nullptr;
+    const int64_t* slot_mapping = nullptr;
+    void* q_out = nullptr;
+    void* k_cache = nullptr;
+    void* v_cache = nullptr;
+    void* k_scale = nullptr;
+    void* v_scale = nullptr;
+    void* v_zero = nullptr;
+    int64_t q_token_stride = 0, k_token_stride = 0, v_token_stride = 0;
+    int64_t n_tokens = 0, n_heads = 0, n_kv_heads = 0;
+    int64_t num_blocks = 0, block_size = 0, n_freqs = 0, n_axes = 1;
+    const int64_t* sections = nullptr;   // [n_axes], on the host
+    int k_format = kF16, v_format = kF16;
+    bool interleaved = false;
+};
+lik_status launch_rope_append(const RopeAppendArgs& a, cudaStream_t stream, std::string& err);
+
+size_t attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t n_kv, int64_t n_groups, bool shared,
+                                 int sm_count);
+lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::string& err);
+// Device address of the attention kernels' error word on the current device.
+void* attention_error_word(std::string& err);
+
 // Device properties cached per device ordinal.
 struct DeviceInfo {
     int sm_count = 0;

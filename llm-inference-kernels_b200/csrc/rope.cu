@@ -1,0 +1,245 @@
+// Append to a paged cache with the position rotation on the way.
+//
+//   angle = position[axis(f)] * inv_freq[f]
+//   (a, b) -> (a cos - b sin, b cos + a sin)
+//
+// over the channel pairs f of the first 2 r channels (r = number of
+// frequencies): (f, f + r), or (2f, 2f + 1) when interleaved; the other
+// channels pass. Frequencies belong to position axes in consecutive sections
+// (one axis: text; three: time, height, width of images and video).
+//
+// Queries are written rotated to their own tensor, keys rotated into the K
+// cache and values as they are into the V cache: fp16 rows, or INT8 / INT4
+// rows quantized per token from the fp16-rounded values, so the cache holds
+// what rotating first and appending after would leave there.
+//
+// Bound by memory: every row is read and written once. One block holds 32
+// (token, head) rows of 128 channels, an 8-lane group each; the block's first
+// threads work out its token's cosines and sines while the rows arrive.
+// Angles take a 64-bit product and range reduction: positions of 10^5 and more
+// leave no correct digits in fp32 at the highest frequencies.
+// Built with -fmad=false: the products round like separate operations.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "lik_device.cuh"
+#include "lik_internal.h"
+#include "lik_quant.cuh"
+
+namespace lik {
+
+namespace {
+
+constexpr int kMaxFreqs = kHeadDim / 2;
+constexpr int kRows = 32;  // rows of a block
+
+struct RopeParams {
+    const __half* q;
+    const __half* k;
+    const __half* v;
+    const long long* pos;  // [axes, n_tokens]
+    const float* inv_freq;
+    const long long* slots;
+    __half* q_out;
+    uint8_t* k_cache;
+    uint8_t* v_cache;
+    __half* k_scale;
+    __half* v_scale;
+    __half* v_zero;
+    long long q_stride, k_stride, v_stride;  // elements between tokens
+    long long n_tokens, n_slots;
+    int n_heads, n_kv, block_size, freqs;
+    int k_format, v_format;
+    int section_end[4];
+};
+
+enum Pairs : int { kHalves = 0, kNeighbours = 1, kHalvesAny = 2 };
+
+__device__ __forceinline__ void rotate2(uint32_t& x, uint32_t& y, float2 c0, float2 c1) {  // two (a, b) pairs
+    const float2 a = __half22float2(as_h2(x)), b = __half22float2(as_h2(y));
+    x = as_u32(__floats2half2_rn(__fsub_rn(__fmul_rn(a.x, c0.x), __fmul_rn(b.x, c0.y)),
+                                 __fsub_rn(__fmul_rn(a.y, c1.x), __fmul_rn(b.y, c1.y))));
+    y = as_u32(__floats2half2_rn(__fadd_rn(__fmul_rn(b.x, c0.x), __fmul_rn(a.x, c0.y)),
+                                 __fadd_rn(__fmul_rn(b.y, c1.x), __fmul_rn(a.y, c1.y))));
+}
+__device__ __forceinline__ uint32_t rotate1(uint32_t x, float2 c) {  // one (a, b) pair
+    const float2 a = __half22float2(as_h2(x));
+    return as_u32(__floats2half2_rn(__fsub_rn(__fmul_rn(a.x, c.x), __fmul_rn(a.y, c.y)),
+                                    __fadd_rn(__fmul_rn(a.y, c.x), __fmul_rn(a.x, c.y))));
+}
+
+__device__ __forceinline__ void store_cache_row(int format, const Raw16& raw, long long row, uint8_t* cache,
+                                                __half* scale, __half* zero, int l, unsigned mask) {
+    switch (format) {
+        case kF16: {
+            uint4* dst = reinterpret_cast<uint4*>(cache + row * (kHeadDim * 2)) + 2 * l;
+            dst[0] = raw.a;
+            dst[1] = raw.b;
+            break;
+        }
+        case kI8: quant_row<kTokI8>(raw, row, cache, scale, zero, l, mask); break;
+        case kI4Sym: quant_row<kTokI4Sym>(raw, row, cache, scale, zero, l, mask); break;
+        default: quant_row<kTokI4Asym>(raw, row, cache, scale, zero, l, mask); break;
+    }
+}
+
+// PAIRS kHalves: the frequencies fill whole 16-byte chunks (r a multiple of
+// 8), so lane l < r / 8 holds chunks l and l + r / 8, both halves of its pairs;
+// the other lanes hold the chunks that pass. kHalvesAny (any r) and
+// kNeighbours: lane l holds channels 16 l .. 16 l + 15.
+template <int PAIRS>
+__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeParams p) {
+    __shared__ float2 turn[kMaxFreqs];  // cosine, sine
+    const long long tok = blockIdx.x;
+    const int l = threadIdx.x & 7;
+    const unsigned mask = 0xFFu << (threadIdx.x & 24);
+    const int row = blockIdx.y * kRows + (threadIdx.x >> 3);
+    const int kind = row < p.n_heads ? 0 : row < p.n_heads + p.n_kv ? 1 : 2;
+    const bool here = row < p.n_heads + 2 * p.n_kv;
+    const int head = kind == 0 ? row : row - p.n_heads - (kind == 2 ? p.n_kv : 0);
+    const __half* src = kind == 0   ? p.q + tok * p.q_stride
+                        : kind == 1 ? p.k + tok * p.k_stride
+                                    : p.v + tok * p.v_stride;
+    src += static_cast<size_t>(head) * kHeadDim;
+    const int c = p.freqs / 8;
+    int x0 = 2 * l, x1 = 2 * l + 1;  // the 16-byte chunks this lane holds
+    if (PAIRS == kHalves && kind != 2 && l < c) {
+        x0 = l;
+        x1 = l + c;
+    }
+    Raw16 raw{};
+    if (here) {
+        raw.a = reinterpret_cast<const uint4*>(src)[x0];
+        raw.b = reinterpret_cast<const uint4*>(src)[x1];
+    }
+    const long long slot = p.slots[tok];
+    if (threadIdx.x < p.freqs) {
+        const int f = threadIdx.x;
+        const int axis = (f >= p.section_end[0]) + (f >= p.section_end[1]) + (f >= p.section_end[2]);
+        constexpr double per_turn = 0.15915494309189533577;  // 1 / (2 pi)
+        const double turns = static_cast<double>(p.pos[axis * p.n_tokens + tok]) * static_cast<double>(p.inv_freq[f]) *
+                             per_turn;
+        float s, co;
+        sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &co);
+        turn[f] = {co, s};
+    }
+    __syncthreads();
+    if (!here) return;  // whole 8-lane groups leave together
+    if (kind != 2) {
+        uint32_t* a = reinterpret_cast<uint32_t*>(&raw.a);
+        uint32_t* b = reinterpret_cast<uint32_t*>(&raw.b);
+        if (PAIRS == kHalves) {
+            if (l < c) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rotate2(a[i], b[i], turn[8 * l + 2 * i], turn[8 * l + 2 * i + 1]);
+            }
+        } else if (PAIRS == kNeighbours) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (8 * l + i < p.freqs) a[i] = rotate1(a[i], turn[8 * l + i]);
+                if (8 * l + 4 + i < p.freqs) b[i] = rotate1(b[i], turn[8 * l + 4 + i]);
+            }
+        } else {
+            __half h[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int ch = 16 * l + i, f = ch < p.freqs ? ch : ch - p.freqs;
+                h[i] = src[ch];
+                if (ch >= 2 * p.freqs) continue;
+                const float x = __half2float(h[i]), y = __half2float(src[ch < p.freqs ? ch + p.freqs : f]);
+                const float2 t = turn[f];
+                h[i] = __float2half_rn(ch < p.freqs ? __fsub_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y))
+                                                    : __fadd_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y)));
+            }
+            __syncwarp(mask);  // q may be rotated in place: nobody writes before all have read
+            raw = *reinterpret_cast<const Raw16*>(h);
+        }
+    }
+    if (kind == 0) {
+        uint4* dst = reinterpret_cast<uint4*>(p.q_out + (tok * p.n_heads + head) * kHeadDim);
+        dst[x0] = raw.a;
+        dst[x1] = raw.b;
+        return;
+    }
+    if (slot < 0 || slot >= p.n_slots) return;  // a token that is not kept
+    const long long blk = slot / p.block_size;
+    const long long drow = (blk * p.n_kv + head) * p.block_size + (slot - blk * p.block_size);
+    if (kind == 2) {
+        store_cache_row(p.v_format, raw, drow, p.v_cache, p.v_scale, p.v_zero, l, mask);
+        return;
+    }
+    if (PAIRS == kHalves && p.k_format != kF16) {
+        // bring the row into 16 consecutive channels per lane: chunk x sits in
+        // lane x (first half), x - c (second half) or x / 2 (passing chunks)
+        const uint32_t a[4] = {raw.a.x, raw.a.y, raw.a.z, raw.a.w}, b[4] = {raw.b.x, raw.b.y, raw.b.z, raw.b.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int x = 2 * l + j;
+            const int from = x < c ? x : x < 2 * c ? x - c : x >> 1;
+            const bool second = x < c ? false : x < 2 * c ? true : (x & 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t u = __shfl_sync(mask, a[i], from, 8), w = __shfl_sync(mask, b[i], from, 8);
+                o[4 * j + i] = second ? w : u;
+            }
+        }
+        raw.a = {o[0], o[1], o[2], o[3]};
+        raw.b = {o[4], o[5], o[6], o[7]};
+    } else if (PAIRS == kHalves) {
+        uint4* dst = reinterpret_cast<uint4*>(p.k_cache + drow * (kHeadDim * 2));
+        dst[x0] = raw.a;
+        dst[x1] = raw.b;
+        return;
+    }
+    store_cache_row(p.k_format, raw, drow, p.k_cache, p.k_scale, nullptr, l, mask);
+}
+
+}  // namespace
+
+lik_status launch_rope_append(const RopeAppendArgs& a, cudaStream_t stream, std::string& err) {
+    RopeParams p{};
+    p.q = static_cast<const __half*>(a.q);
+    p.k = static_cast<const __half*>(a.k);
+    p.v = static_cast<const __half*>(a.v);
+    p.pos = reinterpret_cast<const long long*>(a.positions);
+    p.inv_freq = a.inv_freq;
+    p.slots = reinterpret_cast<const long long*>(a.slot_mapping);
+    p.q_out = static_cast<__half*>(a.q_out);
+    p.k_cache = static_cast<uint8_t*>(a.k_cache);
+    p.v_cache = static_cast<uint8_t*>(a.v_cache);
+    p.k_scale = static_cast<__half*>(a.k_scale);
+    p.v_scale = static_cast<__half*>(a.v_scale);
+    p.v_zero = static_cast<__half*>(a.v_zero);
+    p.q_stride = a.q_token_stride;
+    p.k_stride = a.k_token_stride;
+    p.v_stride = a.v_token_stride;
+    p.n_tokens = a.n_tokens;
+    p.n_slots = a.num_blocks * a.block_size;
+    p.n_heads = static_cast<int>(a.n_heads);
+    p.n_kv = static_cast<int>(a.n_kv_heads);
+    p.block_size = static_cast<int>(a.block_size);
+    p.freqs = static_cast<int>(a.n_freqs);
+    p.k_format = a.k_format;
+    p.v_format = a.v_format;
+    int end = 0;
+    for (int i = 0; i < 4; ++i) {
+        end = i < a.n_axes - 1 ? end + static_cast<int>(a.sections[i]) : kMaxFreqs;
+        p.section_end[i] = end;
+    }
+    const dim3 grid(static_cast<unsigned>(a.n_tokens), static_cast<unsigned>((p.n_heads + 2 * p.n_kv + kRows - 1) / kRows));
+    if (a.interleaved)
+        rope_append_kernel<kNeighbours><<<grid, 256, 0, stream>>>(p);
+    else if (p.freqs % 8 == 0)
+        rope_append_kernel<kHalves><<<grid, 256, 0, stream>>>(p);
+    else
+        rope_append_kernel<kHalvesAny><<<grid, 256, 0, stream>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        err = std::string("rotating append launch: ") + cudaGetErrorString(e);
+        return LIK_ERR_CUDA;
+    }
+    return LIK_OK;
+}
+
+}  // namespace lik

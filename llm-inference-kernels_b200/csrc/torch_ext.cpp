@@ -65,6 +65,9 @@ void check_device_errors() {
             lik_workspace_check(kv.second.data_ptr(), kv.second.numel(), kv.first.second, &code);
         if (st != LIK_OK) msg += std::string(msg.empty() ? "" : "; ") + lik_status_string(st) + ": " + lik_last_error();
     }
+    int code = 0;
+    const lik_status st = lik_attention_check(cur_stream(), &code);
+    if (st != LIK_OK) msg += std::string(msg.empty() ? "" : "; ") + lik_status_string(st) + ": " + lik_last_error();
     TORCH_CHECK(msg.empty(), "decode kernel reported a device-side error (workspace reset): ", msg);
 }
 
@@ -527,6 +530,203 @@ void paged_append(torch::Tensor x, torch::Tensor slot_mapping, torch::Tensor cac
                 "paged_append");
 }
 
+// [n_tokens, heads, 128] fp16 whose heads lie together; tokens may lie apart
+// (a slice of a fused projection). Returns the elements between tokens.
+int64_t token_rows(const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+    TORCH_CHECK(t.scalar_type() == torch::kHalf && t.dim() == 3 && t.size(2) == 128, name,
+                " must be fp16 [n_tokens, heads, 128]");
+    TORCH_CHECK(t.stride(2) == 1 && (t.size(1) <= 1 || t.stride(1) == 128), name,
+                ": the heads of a token must lie together");
+    const int64_t st = t.size(0) > 1 ? t.stride(0) : t.size(1) * 128;
+    TORCH_CHECK(st >= t.size(1) * 128 && st % 8 == 0, name, ": tokens must lie a multiple of 8 elements apart, without overlap");
+    return st;
+}
+
+// fp16 rows or codes and scale (and zero) of a paged cache -> row format
+int cache_format(const at::Tensor& cache, const c10::optional<torch::Tensor>& scale,
+                 const c10::optional<torch::Tensor>& zero, const char* name) {
+    check_cuda(cache, name);
+    TORCH_CHECK(cache.dim() == 4, name, " must be [num_blocks, n_kv_heads, block_size, row]");
+    for (const auto* t : {&scale, &zero}) {
+        if (!t->has_value()) continue;
+        const auto& u = **t;
+        check_cuda(u, "scale / zero");
+        TORCH_CHECK(u.scalar_type() == torch::kHalf && u.dim() == 3 && u.size(0) == cache.size(0) &&
+                        u.size(1) == cache.size(1) && u.size(2) == cache.size(2),
+                    "scale / zero must be fp16 [num_blocks, n_kv_heads, block_size]");
+        check_same_device(cache, u);
+    }
+    if (cache.scalar_type() == torch::kHalf) {
+        TORCH_CHECK(cache.size(3) == 128, name, ": fp16 cache rows must be 128 wide");
+        TORCH_CHECK(!scale.has_value() && !zero.has_value(), name, ": an fp16 cache has no scales");
+        return 0;
+    }
+    TORCH_CHECK(cache.scalar_type() == torch::kInt8, name, " must be fp16 or int8 codes");
+    TORCH_CHECK(scale.has_value(), name, ": a quantized cache needs its per-token scale");
+    if (cache.size(3) == 128) {
+        TORCH_CHECK(!zero.has_value(), name, ": an INT8 cache has no zero points");
+        return 1;
+    }
+    TORCH_CHECK(cache.size(3) == 64, name, ": packed INT4 rows must be 64 bytes");
+    return zero.has_value() ? 3 : 2;
+}
+
+void* opt_ptr(const c10::optional<torch::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+torch::Tensor paged_append_rope(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor positions,
+                                torch::Tensor inv_freq, torch::Tensor slot_mapping, torch::Tensor k_cache,
+                                torch::Tensor v_cache, c10::optional<torch::Tensor> k_scale,
+                                c10::optional<torch::Tensor> v_scale, c10::optional<torch::Tensor> v_zero,
+                                c10::optional<std::vector<int64_t>> sections, bool interleaved) {
+    const int64_t qs = token_rows(q, "q"), ks = token_rows(k, "k"), vs = token_rows(v, "v");
+    TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == q.size(0), "q, k and v must have the same tokens, k and v the same heads");
+    TORCH_CHECK(k.size(1) > 0 && q.size(1) % k.size(1) == 0, "n_heads must be a multiple of n_kv_heads");
+    const int64_t axes = sections.has_value() ? static_cast<int64_t>(sections->size()) : 1;
+    check_cuda(positions, "positions");
+    check_cuda(inv_freq, "inv_freq");
+    check_cuda(slot_mapping, "slot_mapping");
+    TORCH_CHECK(positions.scalar_type() == torch::kInt64 &&
+                    ((positions.dim() == 1 && axes == 1) || (positions.dim() == 2 && positions.size(0) == axes)) &&
+                    positions.size(-1) == q.size(0),
+                "positions must be int64 [n_tokens], or [axes, n_tokens] with one section per axis");
+    TORCH_CHECK(inv_freq.scalar_type() == torch::kFloat && inv_freq.dim() == 1, "inv_freq must be fp32 [rotated channels / 2]");
+    TORCH_CHECK(slot_mapping.scalar_type() == torch::kInt64 && slot_mapping.dim() == 1 &&
+                    slot_mapping.size(0) == q.size(0),
+                "slot_mapping must be int64 [n_tokens]");
+    const int kf = cache_format(k_cache, k_scale, c10::nullopt, "k_cache");
+    const int vf = cache_format(v_cache, v_scale, v_zero, "v_cache");
+    TORCH_CHECK(kf <= 1, "k_cache must be fp16 or INT8 per token (INT4 K is quantized by groups of tokens)");
+    for (int i = 0; i < 3; ++i)
+        TORCH_CHECK(k_cache.size(i) == v_cache.size(i), "k_cache and v_cache must have the same blocks");
+    TORCH_CHECK(k_cache.size(1) == k.size(1), "the caches must have k's head count");
+    for (auto* t : {&k, &v, &positions, &inv_freq, &slot_mapping, &k_cache, &v_cache}) check_same_device(q, *t);
+    const c10::cuda::CUDAGuard guard(q.device());
+    auto out = torch::empty({q.size(0), q.size(1), 128}, q.options());
+    ok_or_throw(lik_paged_append_rope(kf, vf, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+                                      positions.data_ptr<int64_t>(), axes, sections.has_value() ? sections->data() : nullptr,
+                                      inv_freq.data_ptr<float>(), inv_freq.size(0), interleaved,
+                                      slot_mapping.data_ptr<int64_t>(), out.data_ptr(), q.size(0), q.size(1), k.size(1), 128,
+                                      k_cache.data_ptr(), opt_ptr(k_scale), v_cache.data_ptr(), opt_ptr(v_scale),
+                                      opt_ptr(v_zero), k_cache.size(0), k_cache.size(2), cur_stream()),
+                "paged_append_rope");
+    return out;
+}
+
+// ------------------------------------------- several query tokens, shared prefixes
+
+void check_int32(const at::Tensor& t, const at::Tensor& q, std::initializer_list<int64_t> shape, const char* name) {
+    check_cuda(t, name);
+    check_same_device(q, t);
+    TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.sizes() == at::IntArrayRef(shape), name, " must be int32 ",
+                at::IntArrayRef(shape));
+}
+
+struct AttnCommon {
+    int64_t q_stride;
+    int fmt;
+    torch::Tensor out;
+    const float* slopes;
+};
+AttnCommon attention_common(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                            const c10::optional<torch::Tensor>& k_scale, const c10::optional<torch::Tensor>& v_scale,
+                            const c10::optional<torch::Tensor>& alibi_slopes, const c10::optional<torch::Tensor>& out) {
+    AttnCommon c;
+    c.q_stride = token_rows(q, "q");
+    c.fmt = cache_format(k_cache, k_scale, c10::nullopt, "k_cache");
+    TORCH_CHECK(cache_format(v_cache, v_scale, c10::nullopt, "v_cache") == c.fmt && k_cache.sizes() == v_cache.sizes(),
+                "k_cache and v_cache must have the same shape and format");
+    TORCH_CHECK(c.fmt <= 1, "only fp16 and INT8 caches supported");
+    TORCH_CHECK(k_cache.size(1) > 0 && q.size(1) % k_cache.size(1) == 0, "n_heads must be a multiple of n_kv_heads");
+    check_same_device(q, k_cache);
+    check_same_device(q, v_cache);
+    c.slopes = nullptr;
+    if (alibi_slopes.has_value()) {
+        check_cuda(*alibi_slopes, "alibi_slopes");
+        check_same_device(q, *alibi_slopes);
+        TORCH_CHECK(alibi_slopes->scalar_type() == torch::kFloat && alibi_slopes->dim() == 1 &&
+                        alibi_slopes->size(0) == q.size(1),
+                    "alibi_slopes must be fp32 [n_heads]");
+        c.slopes = alibi_slopes->data_ptr<float>();
+    }
+    if (out.has_value()) {
+        check_cuda(*out, "out");
+        check_same_device(q, *out);
+        TORCH_CHECK(out->scalar_type() == torch::kHalf && out->sizes() == q.sizes(), "out must be fp16 with q's shape");
+        c.out = *out;
+    } else {
+        c.out = torch::empty(q.sizes(), q.options());
+    }
+    return c;
+}
+// A workspace of this call alone: it comes from the caching allocator, so
+// captured graphs own theirs and calls on different streams share nothing.
+torch::Tensor attention_workspace(const at::Tensor& q, int64_t n_kv, int64_t groups) {
+    const size_t b = lik_attention_workspace_bytes(q.size(0), q.size(1), n_kv, groups);
+    return torch::empty({static_cast<int64_t>(b)}, q.options().dtype(torch::kUInt8));
+}
+
+torch::Tensor paged_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor block_tables,
+                              torch::Tensor context_lens, torch::Tensor cu_seqlens_q, double softmax_scale,
+                              c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale, bool causal,
+                              int64_t window, double softcap, c10::optional<torch::Tensor> alibi_slopes,
+                              c10::optional<torch::Tensor> prefix_lens, c10::optional<torch::Tensor> first_keys,
+                              c10::optional<torch::Tensor> out) {
+    const c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::optional<c10::Device>(q.device()) : c10::nullopt);
+    const AttnCommon c = attention_common(q, k_cache, v_cache, k_scale, v_scale, alibi_slopes, out);
+    TORCH_CHECK(context_lens.dim() == 1 && block_tables.dim() == 2, "context_lens must be int32 [n_seqs], block_tables int32 "
+                "[n_seqs, max_blocks_per_seq]");
+    const int64_t n = context_lens.size(0);
+    check_int32(context_lens, q, {n}, "context_lens");
+    check_int32(block_tables, q, {n, block_tables.size(1)}, "block_tables");
+    check_int32(cu_seqlens_q, q, {n + 1}, "cu_seqlens_q");
+    if (prefix_lens.has_value()) check_int32(*prefix_lens, q, {n}, "prefix_lens");
+    if (first_keys.has_value()) check_int32(*first_keys, q, {q.size(0)}, "first_keys");
+    const torch::Tensor ws = attention_workspace(q, k_cache.size(1), 0);
+    ok_or_throw(lik_attention_paged(c.fmt, q.data_ptr(), c.q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                    opt_ptr(k_scale), opt_ptr(v_scale), block_tables.data_ptr<int32_t>(),
+                                    context_lens.data_ptr<int32_t>(), cu_seqlens_q.data_ptr<int32_t>(), c.out.data_ptr(),
+                                    q.size(0), n, q.size(1), k_cache.size(1), 128, k_cache.size(0), k_cache.size(2),
+                                    block_tables.size(1), static_cast<float>(softmax_scale), causal, window,
+                                    static_cast<float>(softcap), c.slopes, static_cast<const int32_t*>(opt_ptr(prefix_lens)),
+                                    static_cast<const int32_t*>(opt_ptr(first_keys)), !out.has_value(), ws.data_ptr(),
+                                    ws.numel(), cur_stream()),
+                "paged_attention");
+    return c.out;
+}
+
+torch::Tensor paged_shared_prefix_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache,
+                                            torch::Tensor prefix_tables, torch::Tensor prefix_lens,
+                                            torch::Tensor cu_groups, torch::Tensor block_tables,
+                                            torch::Tensor context_lens, double softmax_scale,
+                                            c10::optional<torch::Tensor> k_scale, c10::optional<torch::Tensor> v_scale,
+                                            double softcap, c10::optional<torch::Tensor> alibi_slopes,
+                                            c10::optional<torch::Tensor> out) {
+    const c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::optional<c10::Device>(q.device()) : c10::nullopt);
+    const AttnCommon c = attention_common(q, k_cache, v_cache, k_scale, v_scale, alibi_slopes, out);
+    TORCH_CHECK(prefix_lens.dim() == 1 && prefix_tables.dim() == 2 && block_tables.dim() == 2,
+                "prefix_lens must be int32 [n_groups], prefix_tables int32 [n_groups, blocks], block_tables int32 "
+                "[batch, max_blocks_per_seq]");
+    const int64_t n = q.size(0), g = prefix_lens.size(0);
+    TORCH_CHECK(g > 0, "need at least one prefix group");
+    check_int32(prefix_lens, q, {g}, "prefix_lens");
+    check_int32(prefix_tables, q, {g, prefix_tables.size(1)}, "prefix_tables");
+    check_int32(cu_groups, q, {g + 1}, "cu_groups");
+    check_int32(block_tables, q, {n, block_tables.size(1)}, "block_tables");
+    check_int32(context_lens, q, {n}, "context_lens");
+    const torch::Tensor ws = attention_workspace(q, k_cache.size(1), g);
+    ok_or_throw(lik_attention_shared_prefix(c.fmt, q.data_ptr(), c.q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                            opt_ptr(k_scale), opt_ptr(v_scale), prefix_tables.data_ptr<int32_t>(),
+                                            prefix_lens.data_ptr<int32_t>(), cu_groups.data_ptr<int32_t>(),
+                                            block_tables.data_ptr<int32_t>(), context_lens.data_ptr<int32_t>(),
+                                            c.out.data_ptr(), n, g, q.size(1), k_cache.size(1), 128, k_cache.size(0),
+                                            k_cache.size(2), prefix_tables.size(1), block_tables.size(1),
+                                            static_cast<float>(softmax_scale), static_cast<float>(softcap), c.slopes,
+                                            ws.data_ptr(), ws.numel(), cur_stream()),
+                "paged_shared_prefix_attention");
+    return c.out;
+}
+
 // ---------------------------------------------------------------- dequantize
 
 std::tuple<torch::Tensor, torch::Tensor> dequant_out(const torch::Tensor& codes, int64_t s) {
@@ -639,6 +839,26 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "Append new K or V tokens into a paged cache at slot_mapping (fp16 copy or per-token quantize)",
           py::arg("x"), py::arg("slot_mapping"), py::arg("cache"), py::arg("scale") = py::none(),
           py::arg("zero") = py::none());
+    m.def("paged_append_rope", &paged_append_rope,
+          "Rotate q and k by their positions (sections: one run of frequencies per position axis), append k and v into "
+          "a paged cache at slot_mapping, return the rotated q",
+          py::arg("q"), py::arg("k"), py::arg("v"), py::arg("positions"), py::arg("inv_freq"), py::arg("slot_mapping"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(),
+          py::arg("v_zero") = py::none(), py::arg("sections") = py::none(), py::arg("interleaved") = false);
+    m.def("paged_attention", &paged_attention,
+          "Attention of any number of query tokens per sequence over a paged fp16 or INT8 cache, with causal, window, "
+          "prefix and document masks, capped scores and distance bias",
+          py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("block_tables"), py::arg("context_lens"),
+          py::arg("cu_seqlens_q"), py::arg("softmax_scale"), py::arg("k_scale") = py::none(),
+          py::arg("v_scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0, py::arg("softcap") = 0.0,
+          py::arg("alibi_slopes") = py::none(), py::arg("prefix_lens") = py::none(),
+          py::arg("first_keys") = py::none(), py::arg("out") = py::none());
+    m.def("paged_shared_prefix_attention", &paged_shared_prefix_attention,
+          "Decode attention of requests that share prefixes: each group's prefix is read once for all its requests",
+          py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("prefix_tables"), py::arg("prefix_lens"),
+          py::arg("cu_groups"), py::arg("block_tables"), py::arg("context_lens"), py::arg("softmax_scale"),
+          py::arg("k_scale") = py::none(), py::arg("v_scale") = py::none(), py::arg("softcap") = 0.0,
+          py::arg("alibi_slopes") = py::none(), py::arg("out") = py::none());
     m.def("dequantize_int8", &dequantize_int8, "INT8 per-token KV -> fp16 K, V (first seqlen positions)",
           py::arg("k_q"), py::arg("k_scale"), py::arg("v_q"), py::arg("v_scale"), py::arg("seqlen") = -1);
     m.def("dequantize_int4", &dequantize_int4,

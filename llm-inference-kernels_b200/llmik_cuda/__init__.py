@@ -13,7 +13,15 @@ failures raise ``RuntimeError``):
     decode_attention_int4(q, k_q, k_scale, v_q, v_scale, group_size, softmax_scale, seqlen=-1)
 
 plus the asymmetric INT4 KIVI format (``*_asym``) and in-place append
-quantizers (``*_into``) that write new tokens into a preallocated cache.
+quantizers (``*_into``) that write new tokens into a preallocated cache, and
+the paged-cache operators of a serving step:
+
+    paged_append(x, slot_mapping, cache, scale=None, zero=None)
+    paged_append_rope(q, k, v, positions, inv_freq, slot_mapping, k_cache, v_cache, ...) -> rotated q
+    paged_decode_attention(q, k_cache, v_cache, block_tables, context_lens, softmax_scale, max_context_len, ...)
+    paged_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, softmax_scale, ...)
+    paged_shared_prefix_attention(q, k_cache, v_cache, prefix_tables, prefix_lens, cu_groups, block_tables,
+                                  context_lens, softmax_scale, ...)
 
 The ops run only on the CUDA library ``libllmik_b200.so`` built by
 ``build.py``; importing this package without the built extension raises
@@ -54,6 +62,9 @@ dequantize_int8 = _C.dequantize_int8
 paged_decode_attention = _C.paged_decode_attention
 dequantize_int4 = _C.dequantize_int4
 paged_append = _C.paged_append
+paged_append_rope = _C.paged_append_rope
+paged_attention = _C.paged_attention
+paged_shared_prefix_attention = _C.paged_shared_prefix_attention
 check_device_errors = _C.check_device_errors
 
 LIBRARY_PATH = _os.path.join(_here, "libllmik_b200.so")
@@ -64,5 +75,5 @@ __all__ = [
     "quantize_k_per_channel_groupwise_int4_asym", "quantize_v_per_token_int4_asym",
     "decode_attention_int4_asym", "quantize_per_token_into", "quantize_v_per_token_int4_into",
     "quantize_k_per_channel_groupwise_int4_into", "dequantize_int8", "dequantize_int4", "paged_decode_attention", "paged_append",
-    "check_device_errors", "LIBRARY_PATH",
+    "paged_append_rope", "paged_attention", "paged_shared_prefix_attention", "check_device_errors", "LIBRARY_PATH",
 ]

@@ -49,6 +49,14 @@ SIGNATURES = {
     "lik_decode_attention_paged": (_int, [_int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
                                           _i64, _i64, _i64, _i64, _i64, _f, _p, _sz, _p]),
     "lik_paged_append": (_int, [_int, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p]),
+    "lik_paged_append_rope": (_int, [_int, _int, _p, _i64, _p, _i64, _p, _i64, _p, _i64, C.POINTER(_i64), _p, _i64, _int,
+                                     _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p]),
+    "lik_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "lik_attention_paged": (_int, [_int, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                                   _i64, _i64, _i64, _f, _int, _i64, _f, _p, _p, _p, _int, _p, _sz, _p]),
+    "lik_attention_shared_prefix": (_int, [_int, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
+                                           _i64, _i64, _i64, _i64, _i64, _i64, _f, _f, _p, _p, _sz, _p]),
+    "lik_attention_check": (_int, [_p, C.POINTER(_int)]),
     "lik_dequantize_int8": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "lik_dequantize_int4": (_int, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "lik_dequantize_int4_asym": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
