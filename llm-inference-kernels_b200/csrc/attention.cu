@@ -53,16 +53,15 @@ namespace {
 constexpr int kTile = 128;                       // key positions per tile
 constexpr int kTileBytes = kTile * kHeadDim * 2; // one fp16 K or V tile
 constexpr int kHalfTile = kTileBytes / 2;        // its 64-channel half
-constexpr int kRing8 = 3, kRing16 = 5;           // fp16 tiles in flight
-constexpr int kRaw = 4;                          // INT8 tiles in flight
+constexpr int kRing8 = 3, kRing16 = 4;           // fp16 tiles in flight
+constexpr int kRaw = 3;                          // INT8 tiles in flight
 constexpr int kRawBytes = kTile * kHeadDim + 256;
 constexpr int kSegs = 4;
-constexpr int kScratchBytes = kTileBytes;        // narrow units: the second query tile's space
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum is raised only past this many powers of two, so most
 // tiles leave the accumulator alone; weights stay below 2^8 in fp16.
 constexpr float kRaise = 8.0f;
-constexpr uint32_t kPolls = 1u << 20;            // of a microsecond at most each
+constexpr uint32_t kPolls = 1u << 18;            // a poll sleeps for a few microseconds at most
 
 enum Dest : int { kDirect = 0, kSlot = 1, kRowBuf = 2 };
 
@@ -117,7 +116,7 @@ struct Segment {
 
 struct Misc {
     uint64_t full[5], empty[5], rfull[kRaw], rempty[kRaw];
-    uint64_t qfull, qempty, sfull[2], pready[2], odone[2], segfull[kSegs], segempty[kSegs], xbar, drain;
+    uint64_t qfull, qempty, sfull[2], pready[2][2], odone[2][2], segfull[kSegs], segempty[kSegs], xbar, drain;
     Segment seg[kSegs];
     long long scan[17];
     long long start, count, total;
@@ -132,7 +131,10 @@ template <int FMT>
 struct Layout {
     static constexpr int ring = FMT == kF16 ? kRing16 : kRing8;
     static constexpr int raw = 2 * kTileBytes + ring * kTileBytes;
-    static constexpr int misc = raw + (FMT == kF16 ? 0 : kRaw * kRawBytes);
+    // results on their way out, see softmax_role
+    static constexpr int stage = raw + (FMT == kF16 ? 0 : kRaw * kRawBytes);
+    static constexpr int stage_bytes = FMT == kF16 ? 32768 : 16384;
+    static constexpr int misc = stage + stage_bytes;
     static constexpr int bytes = misc + 2048;
     static constexpr int threads = FMT == kF16 ? 384 : 512;
     // registers per thread: launched with `base`, then moved between the
@@ -156,21 +158,10 @@ __device__ __forceinline__ void regs_dec() {
 
 // ---- bounded waits -----------------------------------------------------------
 
-__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {  // sleeps for a microsecond at most
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(1000u)
-        : "memory");
-    return done != 0;
-}
 __device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* abort_flag) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kPolls; ++i) {
-        if (__all_sync(kFull, poll(bar, parity))) return true;
+        if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
         if (*reinterpret_cast<volatile int*>(abort_flag)) break;
     }
     if ((threadIdx.x & 31) == 0) {
@@ -264,99 +255,186 @@ struct Row {  // what one softmax thread's row sees
 __device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
     return 1.0f - 2.0f * fast_rcp(1.0f + fast_exp2(t * (2.0f * kLog2e)));
 }
+// tanh on [-0.8, 0.8] as an odd polynomial of degree 9, minimax in the absolute
+// error (3.5e-7): Remez exchange on tanh(t) / t over t^2, weighted by t.
+constexpr float kTanhNear = 0.8f;
+__device__ __forceinline__ float2 tanh_near(float2 t) {
+    const float2 y = mul2(t, t);
+    float2 r = fma2({0.01146465539932251f, 0.01146465539932251f}, y, {-0.04826131463050842f, -0.04826131463050842f});
+    r = fma2(r, y, {0.13186219334602356f, 0.13186219334602356f});
+    r = fma2(r, y, {-0.3331742584705353f, -0.3331742584705353f});
+    r = fma2(r, y, {0.9999951124191284f, 0.9999951124191284f});
+    return mul2(r, t);
+}
 
-// One tile: NC score columns from column c0, keys from j0. `m` is in score
-// units, `sc` turns those into powers of two.
-template <int NC, bool MOD>
-__device__ __forceinline__ bool softmax_tile(const Params& p, Misc* mi, const Row& row, uint32_t s_addr, uint32_t o_addr,
-                                             int c0, int j0, bool first, uint64_t* odone, uint32_t odone_parity,
-                                             float sc, float& m, float& l) {
-    float s[NC];
+// 2^x on the multiply-add pipe for x = 64 u - 56, u in [0, 1]: x splits into an
+// integer, added to the exponent, and a rest in [-1/2, 1/2], whose power is a
+// cubic, minimax in the relative error (7.5e-5, Remez exchange); the weights it
+// gives are rounded to fp16 (4.9e-4). The exponential unit alone takes as long
+// for a tile as its matrix instructions, so a part of the weights come from here.
+__device__ __forceinline__ float2 exp2_cubic(float2 u) {
+    constexpr float magic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, kept in the low bits
+    const float2 t = fma2(u, {64.f, 64.f}, {magic - 56.f, magic - 56.f});
+    const float2 back = fma2(t, {-1.f, -1.f}, {magic - 56.f, magic - 56.f});
+    const float2 r = fma2(u, {64.f, 64.f}, back);
+    float2 e = fma2({0.0551716685295105f, 0.0551716685295105f}, r, {0.2426111251115799f, 0.2426111251115799f});
+    e = fma2(e, r, {0.6932609677314758f, 0.6932609677314758f});
+    e = fma2(e, r, {0.9999280571937561f, 0.9999280571937561f});
+    return {__int_as_float(__float_as_int(e.x) + (__float_as_int(t.x) << 23)),
+            __int_as_float(__float_as_int(e.y) + (__float_as_int(t.y) << 23))};
+}
+__device__ __forceinline__ float fma_sat(float a, float b, float c) {
+    float d;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo .. hi of a word
+    const uint32_t from = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo;
+    const uint32_t to = hi >= 31 ? ~0u : hi < 0 ? 0u : (2u << hi) - 1u;
+    return from & to;
+}
+
+// One step: the softmax of W score columns at s_addr, keys from j0, into W fp16
+// weights at p_addr. `m` is in score units, `sc` turns those into powers of
+// two. The weights are worked out with the maximum so far while the step's own
+// is still being found; only where that turns out to be too low (the first
+// step of a unit, rarely later) the maximum is raised and they are worked out
+// again. On its own the search would hold up every step by a quarter.
+template <int W, bool MOD>
+__device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Row& row, uint32_t s_addr, uint32_t p_addr,
+                                             uint32_t o_addr, int j0, bool have_sums, uint64_t* odone,
+                                             uint32_t odone_parity, float sc, float& m, float& l) {
+    float s[W];
 #pragma unroll
-    for (int i = 0; i < NC; i += 32) tmem_ld32(s_addr + c0 + i, s + i);
+    for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
     tmem_wait_ld();
+    const int j1 = j0 + W - 1;
     if (MOD) {
         if (p.cap > 0.f) {
             const float in = p.scale / p.cap, up = p.cap * kLog2e;
+            const float2 in2 = {in, in}, up2 = {up, up};
+            float least = s[0], most = s[0];
 #pragma unroll
-            for (int i = 0; i < NC; ++i) s[i] = up * tanh_exp(s[i] * in);
+            for (int i = 1; i < W; ++i) {
+                least = fminf(least, s[i]);
+                most = fmaxf(most, s[i]);
+            }
+            if (__all_sync(kFull, fmaxf(most, -least) * in <= kTanhNear)) {
+#pragma unroll
+                for (int i = 0; i < W; i += 2) {
+                    const float2 t = mul2(tanh_near(mul2({s[i], s[i + 1]}, in2)), up2);
+                    s[i] = t.x;
+                    s[i + 1] = t.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) s[i] = up * tanh_exp(s[i] * in);
+            }
         } else {
             const float up = p.scale * kLog2e;
 #pragma unroll
-            for (int i = 0; i < NC; ++i) s[i] *= up;
+            for (int i = 0; i < W; i += 2) {
+                const float2 t = mul2({s[i], s[i + 1]}, {up, up});
+                s[i] = t.x;
+                s[i + 1] = t.y;
+            }
         }
         if (p.slopes) {
             const float from = static_cast<float>(j0) - row.pos;
+            if (__all_sync(kFull, from + static_cast<float>(W - 1) <= 0.f)) {  // no key behind the query
+                const float2 up = {row.slope, row.slope}, two = {2.f, 2.f};
+                float2 d = {from, from + 1.f};
 #pragma unroll
-            for (int i = 0; i < NC; ++i) s[i] = fmaf(-row.slope, fabsf(from + static_cast<float>(i)), s[i]);
+                for (int i = 0; i < W; i += 2) {
+                    const float2 t = fma2(up, d, {s[i], s[i + 1]});
+                    s[i] = t.x;
+                    s[i + 1] = t.y;
+                    d = add2(d, two);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) s[i] = fmaf(-row.slope, fabsf(from + static_cast<float>(i)), s[i]);
+            }
         }
     }
-    const int j1 = j0 + NC - 1;
     const bool whole = (j0 >= row.lo && j1 <= row.hi) || (j0 >= row.fk && j1 < row.pfx);
     if (__any_sync(kFull, !whole)) {
-        const int lo = row.lo - j0, hi = row.hi - j0, fk = row.fk - j0, pfx = row.pfx - j0;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const bool see = (i >= lo && i <= hi) || (i >= fk && i < pfx);
-            s[i] = see ? s[i] : -INFINITY;
+        for (int i = 0; i < W; i += 32) {
+            const int j = j0 + i;
+            const uint32_t see = bits_between(row.lo - j, row.hi - j) | bits_between(row.fk - j, row.pfx - 1 - j);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) s[i + c] = (see >> c) & 1u ? s[i + c] : -INFINITY;
         }
     }
-    float t[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-    for (int i = 4; i < NC; ++i) t[i & 3] = fmaxf(t[i & 3], s[i]);
-    const float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-    if (first) {
-        m = top;
-    } else if (__any_sync(kFull, (top - m) * sc > kRaise)) {
-        const float up = fmaxf(m, top);
-        const float a = m == -INFINITY ? 0.f : fast_exp2((m - up) * sc);
-        m = up;
-        l *= a;
-        if (!warp_wait(odone, odone_parity, mi)) return false;
-        tcgen05_fence_after();
+    const float2 sc2 = {sc, sc};
+    const float sc_u = sc * (1.f / 64.f);
 #pragma unroll 1
-        for (int c = 0; c < kHeadDim; c += 32) {
-            float o[32];
-            tmem_ld32(o_addr + c, o);
-            tmem_wait_ld();
+    for (;;) {
+        const float ms = m == -INFINITY ? 0.f : -m * sc, ms_u = (ms + 56.f) * (1.f / 64.f);
+        const float2 ms2 = {ms, ms};
+        float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t w[W / 2];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= a;
-            tmem_st32(o_addr + c, o);
-        }
-    }
-    const float ms = m == -INFINITY ? 0.f : -m * sc;
-    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-    const float2 sc2 = {sc, sc}, ms2 = {ms, ms};
-#pragma unroll
-    for (int i = 0; i < NC; i += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-            float2 x = fma2({s[i + 2 * c], s[i + 2 * c + 1]}, sc2, ms2);
-            x.x = fast_exp2(x.x);
-            x.y = fast_exp2(x.y);
+        for (int c = 0; c < W / 2; ++c) {
+            const float a = s[2 * c], b = s[2 * c + 1];
+            float2 x;
+            if (c % 8 == 1 || c % 8 == 4 || c % 8 == 6) {  // 3 of 8 pairs: measured beside 2 and 4
+                x = exp2_cubic({fma_sat(a, sc_u, ms_u), fma_sat(b, sc_u, ms_u)});
+            } else {
+                x = fma2({a, b}, sc2, ms2);
+                x.x = fast_exp2(x.x);
+                x.y = fast_exp2(x.y);
+            }
+            most[c & 3] = max3(most[c & 3], a, b);
             sum[c & 1] = add2(sum[c & 1], x);
             w[c] = pack_f16(x.x, x.y);
         }
-        tmem_st16(s_addr + (c0 + i) / 2, w);
-    }
-    if (NC < kTile) {  // the other copies' columns weigh nothing in this one
-        const uint32_t z[16] = {};
+        const float top = fmaxf(max3(most[0], most[1], most[2]), most[3]);
+        if (!__any_sync(kFull, (top - m) * sc > kRaise)) {
 #pragma unroll
-        for (int i = 0; i < kTile; i += 32)
-            if (i < c0 || i >= c0 + NC) tmem_st16(s_addr + i / 2, z);
+            for (int i = 0; i < W / 2; i += 16) tmem_st16(p_addr + i, w + i);
+            const float2 all = add2(sum[0], sum[1]);
+            l += all.x + all.y;
+            return true;
+        }
+        const float up = fmaxf(m, top);
+        const float f = m == -INFINITY ? 0.f : fast_exp2((m - up) * sc);
+        m = up;
+        l *= f;
+        if (have_sums) {
+            if (odone && !warp_wait(odone, odone_parity, mi)) return false;
+            tcgen05_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < kHeadDim; c += 32) {
+                float o[32];
+                tmem_ld32(o_addr + c, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] *= f;
+                tmem_st32(o_addr + c, o);
+            }
+        }
     }
-    const float2 all = add2(sum[0], sum[1]);
-    l += all.x + all.y;
-    tmem_wait_st();
-    tcgen05_fence_before();
-    return true;
 }
 
+// All of a stream's tiles of a segment. NC: the columns of a tile this copy of
+// the rows works on; 128 go in two steps, the first one's weights being
+// multiplied with V while the second is worked out. A tile's scores are there
+// only after the products of the tile before, so the sums can be scaled at once
+// in a tile's first step and after the first half's product in its second.
+// `tiles` and `halves` count the tiles, and those in two steps, so far.
 template <int NC, bool MOD>
 __device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Segment& g, const Row& row, int stream,
-                                            uint32_t s_addr, uint32_t o_addr, float sc, uint32_t& tiles, float& m,
-                                            float& l) {
+                                            uint32_t s_addr, uint32_t o_addr, float sc, uint32_t& tiles, uint32_t& halves,
+                                            float& m, float& l) {
+    constexpr int W = NC == 128 ? 64 : NC;
     const int warp = (threadIdx.x >> 5) & 3;
     const int c0 = NC == 128 ? 0 : NC == 64 ? (warp >> 1) * 64 : warp * 32;
     const int step = g.rep ? 2 : 1;
@@ -364,39 +442,39 @@ __device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Seg
 #pragma unroll 1
     for (int i = i0; i < g.t1; i += step) {
         if (!warp_wait(&mi->sfull[stream], tiles & 1, mi)) return false;
-        tcgen05_fence_after();
-        if (!softmax_tile<NC, MOD>(p, mi, row, s_addr, o_addr, c0, g.tile(i) * kTile + c0, i == i0, &mi->odone[stream],
-                                   (tiles - 1) & 1, sc, m, l))
-            return false;
-        warp_arrive(&mi->pready[stream]);
         ++tiles;
+        tcgen05_fence_after();
+        const int j0 = g.tile(i) * kTile + c0;
+#pragma unroll 1
+        for (int c = 0; c < NC; c += W) {
+            if (!softmax_step<W, MOD>(p, mi, row, s_addr + c0 + c, s_addr + (c0 + c) / 2, o_addr, j0 + c, i > i0 || c > 0,
+                                      c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1, sc, m, l))
+                return false;
+            if (NC < kTile) {  // the other copies' columns weigh nothing in this one
+                const uint32_t z[16] = {};
+#pragma unroll
+                for (int k = 0; k < kTile; k += 32)
+                    if (k < c0 || k >= c0 + NC) tmem_st16(s_addr + k / 2, z);
+            }
+            tmem_wait_st();
+            tcgen05_fence_before();
+            warp_arrive(&mi->pready[stream][NC < kTile || c > 0]);
+        }
+        if (NC == kTile) ++halves;
     }
     return true;
 }
 
-__device__ __forceinline__ void store_row(const Params& p, const Segment& g, int tok, int head_row, int unit_row, int c,
-                                          float4 v, float inv) {
-    if (g.dest == kDirect) {
-        uint2 u;
-        u.x = pack_f16(v.x * inv, v.y * inv);
-        u.y = pack_f16(v.z * inv, v.w * inv);
-        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(tok) * p.n_heads + head_row) * kHeadDim + c) = u;
-    } else {
-        const size_t r = g.dest == kSlot
-                             ? static_cast<size_t>(2 * blockIdx.x + (g.t0 == 0)) * p.slot_rows + unit_row
-                             : static_cast<size_t>(g.set) * p.n_tokens * p.n_heads +
-                                   static_cast<size_t>(tok) * p.n_heads + head_row;
-        float* dst = (g.dest == kSlot ? p.part : p.rowbuf) + r * kHeadDim + c;
-        *reinterpret_cast<float4*>(dst) = v;
-    }
+// Where row (tok, query head hr) of the segment goes: a row of out, of the
+// CTA's partial sums (`ur` its row in the unit) or of the whole units' sums.
+__device__ __forceinline__ uint32_t dest_row(const Params& p, const Segment& g, int tok, int hr, int ur) {
+    const uint32_t r = static_cast<uint32_t>(tok) * p.n_heads + hr;
+    if (g.dest == kDirect) return r;
+    if (g.dest == kSlot) return (2 * blockIdx.x + (g.t0 == 0)) * p.slot_rows + ur;
+    return static_cast<uint32_t>(g.set) * p.n_tokens * p.n_heads + r;
 }
-__device__ __forceinline__ void store_ml(const Params& p, const Segment& g, int tok, int head_row, int unit_row, float m,
-                                         float l) {
-    if (g.dest == kSlot)
-        p.part_ml[static_cast<size_t>(2 * blockIdx.x + (g.t0 == 0)) * p.slot_rows + unit_row] = {m, l};
-    else if (g.dest == kRowBuf)
-        p.row_ml[static_cast<size_t>(g.set) * p.n_tokens * p.n_heads + static_cast<size_t>(tok) * p.n_heads +
-                 head_row] = {m, l};
+__device__ __forceinline__ void store_ml(const Params& p, const Segment& g, uint32_t row, float m, float l) {
+    if (g.dest != kDirect) (g.dest == kSlot ? p.part_ml : p.row_ml)[row] = {m, l};
 }
 
 // Barrier of the eight softmax warps.
@@ -405,14 +483,66 @@ __device__ __forceinline__ bool softmax_sync(Misc* mi, uint32_t& phase) {
     return warp_wait(&mi->xbar, phase++ & 1, mi);
 }
 
-template <bool MOD>
+// Writes this warp's 32 rows of a stream's sums, times `f`, as fp16 or fp32
+// rows of 128 channels; `row_at` is this lane's row, ~0 for none.
+template <int FMT, bool HALF>
+__device__ __forceinline__ void store_wide(unsigned char* stage, unsigned char* base, uint32_t o_addr, bool any,
+                                           uint32_t row_at, float f) {
+    constexpr int bytes = Layout<FMT>::stage_bytes / 256;  // of a row per pass
+    constexpr int lanes = bytes / 16, cols = HALF ? bytes / 2 : bytes / 4;
+    const int lane = threadIdx.x & 31;
+    unsigned char* const mine = stage + (threadIdx.x >> 5) * 32 * bytes;
+#pragma unroll 1
+    for (int c = 0; c < kHeadDim; c += cols) {
+        float o[cols];
+#pragma unroll
+        for (int i = 0; i < cols; ++i) o[i] = 0.f;
+        if (any) {
+            if constexpr (cols == 16) {
+                tmem_ld16(o_addr + c, o);
+            } else {
+#pragma unroll
+                for (int i = 0; i < cols; i += 32) tmem_ld32(o_addr + c + i, o + i);
+            }
+            tmem_wait_ld();
+        }
+#pragma unroll
+        for (int i = 0; i < lanes; ++i) {
+            uint4 u;
+            if constexpr (HALF) {
+                u = {pack_f16(o[8 * i] * f, o[8 * i + 1] * f), pack_f16(o[8 * i + 2] * f, o[8 * i + 3] * f),
+                     pack_f16(o[8 * i + 4] * f, o[8 * i + 5] * f), pack_f16(o[8 * i + 6] * f, o[8 * i + 7] * f)};
+            } else {
+                u = {__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]),
+                     __float_as_uint(o[4 * i + 3])};
+            }
+            *reinterpret_cast<uint4*>(mine + lane * bytes + ((i ^ (lane & (lanes - 1))) << 4)) = u;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < lanes; ++i) {
+            const int r = i * (32 / lanes) + lane / lanes, x = lane & (lanes - 1);
+            const uint32_t at = __shfl_sync(kFull, row_at, r);
+            const uint4 u = *reinterpret_cast<const uint4*>(mine + r * bytes + ((x ^ (r & (lanes - 1))) << 4));
+            if (at != ~0u)
+                *reinterpret_cast<uint4*>(base + (static_cast<size_t>(at) * kHeadDim + c) * (HALF ? 2 : 4) + x * 16) = u;
+        }
+        __syncwarp();
+    }
+}
+
+// Results leave through shared memory, so that a warp writes whole runs of a
+// row instead of 16 bytes of 32 rows (a quarter of the time for a wide unit).
+template <int FMT, bool MOD>
 __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uint32_t tmem) {
     const int stream = threadIdx.x >> 7, r_in = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>(r_in & 96) << 16;
     const uint32_t s_addr = tmem + lane_base + stream * 128, o_addr = s_addr + 256;
     const float sc = MOD ? 1.f : p.scale * kLog2e;
     const int per = kTile / p.group;
-    uint32_t tiles = 0, xphase = 0;
+    unsigned char* const stage = smem + Layout<FMT>::stage;
+    uint32_t tiles = 0, halves = 0, xphase = 0;
+    bool wide_before = false;
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
@@ -439,42 +569,33 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
         const int mine = g.rep ? (g.t1 - g.t0 - stream + 1) / 2 : g.t1 - g.t0;  // tiles of this stream
         bool ok;
         if (g.rep == 4)
-            ok = softmax_run<32, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, m, l);
+            ok = softmax_run<32, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, halves, m, l);
         else if (g.rep == 2)
-            ok = softmax_run<64, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, m, l);
+            ok = softmax_run<64, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, halves, m, l);
         else
-            ok = softmax_run<128, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, m, l);
+            ok = softmax_run<128, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, halves, m, l);
         if (!ok) return;
         if (mine > 0) {
-            if (!warp_wait(&mi->odone[stream], (tiles - 1) & 1, mi)) return;
+            if (!warp_wait(&mi->odone[stream][1], (tiles - 1) & 1, mi)) return;
             tcgen05_fence_after();
         }
+        if (m == -INFINITY) l = 0.f;
         const float m2 = l > 0.f ? m * sc : -INFINITY;
         if (g.rep == 0) {
-            const int ur = tl * p.group + hr - g.head * p.group;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
-            if (live) store_ml(p, g, tok, hr, ur, m2, l);
-#pragma unroll 1
-            for (int c = 0; c < kHeadDim; c += 32) {
-                float o[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.f;
-                if (mine > 0) {
-                    tmem_ld32(o_addr + c, o);
-                    tmem_wait_ld();
-                }
-                if (live) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        store_row(p, g, tok, hr, ur, c + i,
-                                  l > 0.f ? float4{o[i], o[i + 1], o[i + 2], o[i + 3]} : float4{0.f, 0.f, 0.f, 0.f}, inv);
-                }
-            }
+            const uint32_t row_at = live ? dest_row(p, g, tok, hr, tl * p.group + hr - g.head * p.group) : ~0u;
+            if (live) store_ml(p, g, row_at, m2, l);
+            if (g.dest == kDirect)
+                store_wide<FMT, true>(stage, reinterpret_cast<unsigned char*>(p.out), o_addr, mine > 0, row_at,
+                                      l > 0.f ? 1.f / l : 0.f);
+            else
+                store_wide<FMT, false>(stage, reinterpret_cast<unsigned char*>(g.dest == kSlot ? p.part : p.rowbuf),
+                                       o_addr, mine > 0, row_at, 1.f);
         } else {
             // join the copies and streams: each scales its sums to the row's
             // common maximum, then 256 threads add the states in order
-            float2* ml = reinterpret_cast<float2*>(smem + kTileBytes);
-            float* data = reinterpret_cast<float*>(smem + kTileBytes + 2048);
+            if (wide_before && !softmax_sync(mi, xphase)) return;  // the staging space was the warps' own
+            float2* ml = reinterpret_cast<float2*>(stage);
+            float4* data = reinterpret_cast<float4*>(stage + 2048);
             const int states = 2 * g.rep, rows = g.ntok * p.group;
             const int state = stream * g.rep + r_in / block;
             ml[threadIdx.x] = live ? float2{m2, l} : float2{-INFINITY, 0.f};
@@ -482,23 +603,29 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
             float top = -INFINITY;
             for (int t = 0; t < states; ++t) top = fmaxf(top, ml[t * block + rr].x);
             const float f = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top);
-            int dc = 128;  // channels per pass: what fits the scratch space
-            while (states * rows * dc * 4 > kScratchBytes - 2048 && dc > 16) dc >>= 1;
-            const int quads = dc / 4;
+            int dc = 128;  // channels per pass: what fits the scratch space (states * rows <= 256)
+            while (states * rows * dc * 4 > Layout<FMT>::stage_bytes - 2048) dc >>= 1;
+            const int quads = dc / 4, spread = min(quads, 8) - 1;
+            float4* const mine_at = data + (state * rows + rr) * quads;
             for (int d0 = 0; d0 < kHeadDim; d0 += dc) {
-                for (int c = 0; c < dc; c += 16) {
+                for (int c = 0; c < dc; c += 32) {
                     float o[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.f;
                     if (mine > 0) {
-                        tmem_ld16(o_addr + d0 + c, o);
+                        tmem_ld32(o_addr + ((d0 + c) & ~31), o);
                         tmem_wait_ld();
                     }
                     if (live) {
-                        float4* dst = reinterpret_cast<float4*>(data) + (state * rows + rr) * quads;
+                        const int skip = ((d0 + c) & 31) / 4, n = min(quads, 8);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float4 v = {0.f, 0.f, 0.f, 0.f};
-                            if (f > 0.f) v = {o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
-                            dst[(c / 4 + i) ^ (rr & 3)] = v;
+                        for (int i = 0; i < 8; ++i) {
+                            const int x = i - skip;
+                            if (x >= 0 && x < n) {
+                                float4 v = {o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
+                                if (f == 0.f) v = {0.f, 0.f, 0.f, 0.f};
+                                mine_at[(c / 4 + x) ^ (rr & spread)] = v;
+                            }
                         }
                     }
                 }
@@ -511,17 +638,24 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
                     for (int t = 0; t < states; ++t) {
                         const float2 e = ml[t * block + r];
                         if (e.x > -INFINITY) sum += e.y * fast_exp2(e.x - mx);
-                        const float4 a = reinterpret_cast<const float4*>(data)[(t * rows + r) * quads + (c4 ^ (r & 3))];
+                        const float4 a = data[(t * rows + r) * quads + (c4 ^ (r & spread))];
                         v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
                     }
-                    const int tk = r / p.group, h = g.head * p.group + r - tk * p.group;
-                    if (d0 == 0 && c4 == 0) store_ml(p, g, g.tok0 + tk, h, r, mx, sum);
-                    store_row(p, g, g.tok0 + tk, h, r, d0 + 4 * c4, v, sum > 0.f ? 1.f / sum : 0.f);
+                    const int tk = r / p.group;
+                    const uint32_t at = dest_row(p, g, g.tok0 + tk, g.head * p.group + r - tk * p.group, r);
+                    if (d0 == 0 && c4 == 0) store_ml(p, g, at, mx, sum);
+                    const size_t e = static_cast<size_t>(at) * kHeadDim + d0 + 4 * c4;
+                    if (g.dest == kDirect) {
+                        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                        *reinterpret_cast<uint2*>(p.out + e) = {pack_f16(v.x * inv, v.y * inv), pack_f16(v.z * inv, v.w * inv)};
+                    } else {
+                        *reinterpret_cast<float4*>((g.dest == kSlot ? p.part : p.rowbuf) + e) = v;
+                    }
                 }
                 if (!softmax_sync(mi, xphase)) return;
             }
-            fence_async_smem();  // the next query tile may be copied over the scratch space
         }
+        wide_before = g.rep == 0;
         tcgen05_fence_before();
         warp_arrive(&mi->segempty[slot]);
     }
@@ -535,48 +669,60 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
     constexpr uint32_t id_qk = mma_idesc_f16(128, 128, false), id_pv = mma_idesc_f16(128, 128, true);
     const int lane = threadIdx.x & 31;
     const uint32_t q_addr = smem_addr(smem), r_addr = q_addr + 2 * kTileBytes;
-    uint32_t pos = 0, ph[2] = {0, 0};  // ring entries taken; P tiles per stream
+    uint32_t pos = 0, ph[2][2] = {};  // ring entries taken; weights taken per stream and half
     auto wait_entry = [&](uint32_t e) { return warp_wait(&mi->full[e % ring], (e / ring) & 1, mi); };
+    // descriptors differ by constants: one addition each, in uniform registers
+    const uint32_t leader = elect_one();
+    const uint64_t q_desc = smem_desc(q_addr, 16, 1024), k_desc = smem_desc(r_addr, 16, 1024),
+                   v_desc = smem_desc(r_addr, kHalfTile, 1024);
     auto qk = [&](int stream, int qslot, uint32_t e) {
         tcgen05_fence_after();
-        if (lane == 0) {
-            const uint32_t a = q_addr + qslot * kTileBytes, b = r_addr + (e % ring) * kTileBytes;
+        const uint64_t a = q_desc + qslot * (kTileBytes >> 4), b = k_desc + (e % ring) * (kTileBytes >> 4);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t off = (i >> 2) * kHalfTile + (i & 3) * 32;
-                mma_f16_ss(tmem + stream * 128, smem_desc(a + off, 16, 1024), smem_desc(b + off, 16, 1024), id_qk, i > 0);
-            }
-            mma_commit(&mi->sfull[stream]);
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t off = ((i >> 2) * kHalfTile + (i & 3) * 32) >> 4;
+            mma_f16_ss(tmem + stream * 128, a + off, b + off, id_qk, i > 0, leader);
         }
-        __syncwarp();
+        mma_commit(&mi->sfull[stream], leader);
     };
-    auto pv = [&](int stream, uint32_t e, bool first) {
+    // the next weights of this stream times V: half a tile's where 128 columns
+    // are worked out in two steps, else the tile's
+    auto pv = [&](int stream, uint32_t e, bool first, bool halves) {
+        const uint64_t b = v_desc + (e % ring) * (kTileBytes >> 4);
+        const uint32_t o = tmem + 256 + stream * 128, w = tmem + stream * 128;
+        if (halves) {
+            if (!warp_wait(&mi->pready[stream][0], ph[stream][0]++ & 1, mi)) return false;
+            tcgen05_fence_after();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma_f16_ts(o, w + i * 8, b + i * (2048 >> 4), id_pv, !first || i > 0, leader);
+            mma_commit(&mi->odone[stream][0], leader);
+        }
+        if (!warp_wait(&mi->pready[stream][1], ph[stream][1]++ & 1, mi)) return false;
         tcgen05_fence_after();
-        if (lane == 0) {
-            const uint32_t b = r_addr + (e % ring) * kTileBytes;
+        if (!halves) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                mma_f16_ts(tmem + 256 + stream * 128, tmem + stream * 128 + i * 8, smem_desc(b + i * 2048, kHalfTile, 1024),
-                           id_pv, !first || i > 0);
-            mma_commit(&mi->odone[stream]);
+            for (int i = 0; i < 4; ++i) mma_f16_ts(o, w + i * 8, b + i * (2048 >> 4), id_pv, !first || i > 0, leader);
         }
-        __syncwarp();
+#pragma unroll
+        for (int i = 4; i < 8; ++i) mma_f16_ts(o, w + i * 8, b + i * (2048 >> 4), id_pv, 1, leader);
+        mma_commit(&mi->odone[stream][1], leader);
+        return true;
     };
-    auto release = [&](uint32_t e) {
-        if (lane == 0) mma_commit(&mi->empty[e % ring]);
-        __syncwarp();
-    };
+    auto release = [&](uint32_t e) { mma_commit(&mi->empty[e % ring], leader); };
     // fp16 V rows that no row of the unit sees may hold anything (the end of a
     // page, tokens that left the window): 0 * NaN would reach the sums
     auto clean = [&](const Segment& g, int tile, uint32_t e) {
         if (FMT != kF16) return;  // the conversion writes zeros there
         const int j0 = tile * kTile;
-        if ((j0 >= g.vlo && j0 + kTile - 1 <= g.vhi) || (j0 >= g.fk && j0 + kTile <= g.pfx)) return;
-        unsigned char* v = smem + 2 * kTileBytes + (e % ring) * kTileBytes;
-        for (int i = lane >> 3; i < 2 * kTile; i += 4) {
-            const int r = i >> 1;
-            if (!g.seen(j0 + r))
-                *reinterpret_cast<uint4*>(v + (i & 1) * kHalfTile + r * 128 + (lane & 7) * 16) = uint4{0, 0, 0, 0};
+        const int lo = g.vlo - j0, hi = g.vhi - j0, fk = g.fk - j0, pfx = g.pfx - j0;
+        if ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) return;
+        unsigned char* v = smem + 2 * kTileBytes + (e % ring) * kTileBytes + (lane & 7) * 16;
+#pragma unroll 4
+        for (int r = lane >> 3; r < kTile; r += 4) {
+            if (!((r >= lo && r <= hi) || (r >= fk && r < pfx))) {
+                *reinterpret_cast<uint4*>(v + r * 128) = uint4{0, 0, 0, 0};
+                *reinterpret_cast<uint4*>(v + kHalfTile + r * 128) = uint4{0, 0, 0, 0};
+            }
         }
         fence_async_smem();
         __syncwarp();
@@ -586,16 +732,17 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
-        const int n = g.t1 - g.t0;
+        const int n = __shfl_sync(kFull, g.t1 - g.t0, 0);  // known to be uniform
         if (n > 0) {
             if (!warp_wait(&mi->qfull, qk_seg++ & 1, mi)) return;
-            if (g.rep == 0) {
+            const int rep = __shfl_sync(kFull, g.rep, 0);
+            if (rep == 0) {
                 if (!wait_entry(pos)) return;
                 qk(0, 0, pos);
                 qk(1, 1, pos);
                 release(pos);
                 ++pos;
-                if (n == 1 && lane == 0) mma_commit(&mi->qempty);
+                if (n == 1) mma_commit(&mi->qempty, leader);
                 for (int i = 0; i < n; ++i) {
                     const uint32_t ve = pos, ke = pos + 1;
                     const bool more = i + 1 < n;
@@ -603,8 +750,7 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
                     clean(g, g.tile(g.t0 + i), ve);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        if (!warp_wait(&mi->pready[s], ph[s]++ & 1, mi)) return;
-                        pv(s, ve, i == 0);
+                        if (!pv(s, ve, i == 0, true)) return;
                         if (more) {
                             if (s == 0 && !wait_entry(ke)) return;
                             qk(s, s, ke);
@@ -613,7 +759,7 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
                     release(ve);
                     if (more) {
                         release(ke);
-                        if (i + 2 == n && lane == 0) mma_commit(&mi->qempty);
+                        if (i + 2 == n) mma_commit(&mi->qempty, leader);
                     }
                     pos += more ? 2 : 1;
                 }
@@ -624,13 +770,12 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
                     release(pos);
                     ++pos;
                 }
-                if (n <= 2 && lane == 0) mma_commit(&mi->qempty);
+                if (n <= 2) mma_commit(&mi->qempty, leader);
                 for (int i = 0; i < n; ++i) {
                     const int s = i & 1;
                     if (!wait_entry(pos)) return;
                     clean(g, g.tile(g.t0 + i), pos);
-                    if (!warp_wait(&mi->pready[s], ph[s]++ & 1, mi)) return;
-                    pv(s, pos, i < 2);
+                    if (!pv(s, pos, i < 2, rep == 1)) return;
                     release(pos);
                     ++pos;
                     if (i + 2 < n) {
@@ -638,7 +783,7 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
                         qk(s, 0, pos);
                         release(pos);
                         ++pos;
-                        if (i + 3 == n && lane == 0) mma_commit(&mi->qempty);
+                        if (i + 3 == n) mma_commit(&mi->qempty, leader);
                     }
                 }
             }
@@ -660,7 +805,6 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
     const int subs = kTile / p.box_rows;                       // boxes of a tile
     const int sub = FMT == kF16 ? lane >> 1 : lane;            // this lane's box
     uint32_t pos = 0, q_seg = 0;  // tiles and query loads so far
-    uint32_t narrow = 0;          // 1 + the last narrow segment
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) break;
@@ -669,12 +813,8 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
         const int n = g.t1 - g.t0;
         bool ok = true;
         if (n > 0) {
-            // queries: the last segment's score tiles are done with the first
-            // slot; its epilogue with the scratch space in the second
+            // queries: the last segment's score tiles are done with them
             if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
-            if (g.rep == 0 && narrow && k - (narrow - 1) < kSegs &&
-                !warp_wait(&mi->segempty[(narrow - 1) % kSegs], ((narrow - 1) / kSegs) & 1, mi))
-                break;
             ++q_seg;
             const int copies = g.rep ? g.rep : 2, block = g.rep ? kTile / g.rep : kTile;
             const int toks = block / p.group;
@@ -744,15 +884,14 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
             }
         }
         if (!ok) break;
-        if (g.rep) narrow = k + 1;
         warp_arrive(&mi->segempty[slot]);
     }
     // Leave no copy in flight: after an abort nobody else waits for them.
     if (*reinterpret_cast<volatile int*>(&mi->abort)) {
         for (uint32_t e = pos > ring ? pos - ring : 0; e < pos; ++e)
-            for (uint32_t i = 0; i < kPolls && !poll(&full[e % ring], (e / ring) & 1); ++i) {}
+            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&full[e % ring], (e / ring) & 1); ++i) {}
         if (q_seg > 0)
-            for (uint32_t i = 0; i < kPolls && !poll(&mi->qfull, (q_seg - 1) & 1); ++i) {}
+            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->qfull, (q_seg - 1) & 1); ++i) {}
     }
 }
 
@@ -816,8 +955,10 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem) {
 
 // ---- schedule --------------------------------------------------------------------
 
-// Cost of a unit in tiles (an empty one still writes its rows).
-__device__ __forceinline__ int unit_cost(const Segment& s) { return max(s.nt, 1); }
+// Cost of a unit in tiles: its own (an empty one still writes its rows) behind
+// what starting and finishing one takes.
+constexpr int kUnitCost = 2;
+__device__ __forceinline__ int unit_cost(const Segment& s) { return max(s.nt, 1) + kUnitCost; }
 
 // CTAs that the tiles are split over: none of them goes without, so the CTAs
 // from a split unit's first to its last all hold a part of it.
@@ -885,33 +1026,39 @@ __device__ void schedule_role(const Params& p, Misc* mi) {
     bool split = false;
     Segment s;
     if (left > 0) make_unit(p, id, s);
-    for (uint32_t k = 0;; ++k) {
+    for (uint32_t k = 0;;) {
         const int slot = k % kSegs;
-        if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
         if (left <= 0) {
+            if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
             if (lane == 0) mi->seg[slot].valid = 0;
             warp_arrive(&mi->segfull[slot]);
             break;
         }
-        const int cost = unit_cost(s);
+        const int cost = unit_cost(s), tiles = cost - kUnitCost;
         const int n = static_cast<int>(min(left, static_cast<long long>(cost - off)));
-        s.valid = 1;
-        s.head = head;
-        s.t0 = s.nt ? off : 0;
-        s.t1 = s.nt ? off + n : 0;
-        const bool whole = off == 0 && n == cost;
-        s.dest = !whole ? kSlot : p.shared ? kRowBuf : kDirect;
-        if (lane == 0) {
-            mi->seg[slot] = s;
-            if (off == 0) {
-                const long long end = at + cost - 1;  // its last tile's owner finishes the unit
-                const int last = whole ? -1 : static_cast<int>(((end + 1) * sharing_ctas(p, total) - 1) / total);
-                if (p.shared) p.units[static_cast<size_t>(id) * p.n_kv + head] = {static_cast<int>(blockIdx.x), last};
-                if (!whole) p.split[blockIdx.x] = {s.tok0, s.ntok, head, last};
+        const int t0 = max(off - kUnitCost, 0), t1 = max(off + n - kUnitCost, 0);
+        if (t1 > t0) {
+            const bool whole = t0 == 0 && t1 == tiles;
+            s.valid = 1;
+            s.head = head;
+            s.t0 = s.nt ? t0 : 0;
+            s.t1 = s.nt ? t1 : 0;
+            s.dest = !whole ? kSlot : p.shared ? kRowBuf : kDirect;
+            if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
+            if (lane == 0) {
+                mi->seg[slot] = s;
+                if (t0 == 0) {
+                    const long long end = at - off + cost - 1;  // its last tile's owner finishes the unit
+                    const int last =
+                        whole ? -1 : static_cast<int>(((end + 1) * sharing_ctas(p, total) - 1) / total);
+                    if (p.shared) p.units[static_cast<size_t>(id) * p.n_kv + head] = {static_cast<int>(blockIdx.x), last};
+                    if (!whole) p.split[blockIdx.x] = {s.tok0, s.ntok, head, last};
+                }
             }
+            split |= t0 == 0 && !whole;
+            warp_arrive(&mi->segfull[slot]);
+            ++k;
         }
-        split |= off == 0 && !whole;
-        warp_arrive(&mi->segfull[slot]);
         at += n;
         left -= n;
         off = 0;
@@ -945,8 +1092,10 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
         mbar_init(&mi->qempty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&mi->sfull[i], 1);
-            mbar_init(&mi->pready[i], 4);
-            mbar_init(&mi->odone[i], 1);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&mi->pready[i][h], 4);
+                mbar_init(&mi->odone[i][h], 1);
+            }
         }
         for (int i = 0; i < kSegs; ++i) {
             mbar_init(&mi->segfull[i], 1);
@@ -970,7 +1119,7 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
 
     if (warp < 8) {
         regs_inc<Lay::softmax_regs>();
-        softmax_role<MOD>(p, mi, smem, tmem);
+        softmax_role<FMT, MOD>(p, mi, smem, tmem);
     } else if (warp < 12) {
         regs_dec<Lay::other_regs>();
         if (warp == 8) {
@@ -978,9 +1127,8 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
         } else if (warp == 9) {
             mma_role<FMT>(p, mi, smem, tmem);
             if (*reinterpret_cast<volatile int*>(&mi->abort)) {  // wait out what is still running
-                if ((threadIdx.x & 31) == 0) mma_commit(&mi->drain);
-                __syncwarp();
-                for (uint32_t i = 0; i < kPolls && !poll(&mi->drain, 0); ++i) {}
+                mma_commit(&mi->drain, elect_one());
+                for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->drain, 0); ++i) {}
             }
         } else if (warp == 10) {
             schedule_role(p, mi);
