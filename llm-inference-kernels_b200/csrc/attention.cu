@@ -32,8 +32,8 @@
 //
 // fp16 caches go from the pool to swizzled shared memory by tensor-map copies,
 // one box per run of positions inside a page. INT8 caches arrive as codes and
-// scales; four more warps write fp16(code * scale), the rounding of the
-// dequantizing entry points, into the same swizzled tiles.
+// scales; four more warps write the codes as fp16 integers into the same
+// swizzled tiles, and the softmax applies the scales in fp32.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -53,9 +53,10 @@ namespace {
 constexpr int kTile = 128;                       // key positions per tile
 constexpr int kTileBytes = kTile * kHeadDim * 2; // one fp16 K or V tile
 constexpr int kHalfTile = kTileBytes / 2;        // its 64-channel half
-constexpr int kRing8 = 3, kRing16 = 4;           // fp16 tiles in flight
-constexpr int kRaw = 3;                          // INT8 tiles in flight
-constexpr int kRawBytes = kTile * kHeadDim + 256;
+constexpr int kRing8 = 1, kRing16 = 2;           // fp16 tiles of K, and of V, in flight
+constexpr int kRaw = 4;                          // INT8 tiles in flight
+constexpr int kRawBytes = kTile * kHeadDim;      // codes; their scales: 256 bytes
+constexpr int kScales = 4;                       // INT8: tiles whose scales are kept
 constexpr int kSegs = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum is raised only past this many powers of two, so most
@@ -80,9 +81,9 @@ struct Params {
     const int* first_keys;
     const float* slopes;
     int window;
-    float scale, cap;
+    float kf, cap;  // scores times kf: powers of two, or tanh's argument where they are capped
     int n_tokens, n_heads, n_kv, group;
-    int num_blocks, block_size, box_rows, total_rows;
+    int num_blocks, block_size, box_rows, box_shift, total_rows;
     const __half* k_scale;
     const __half* v_scale;
     __half* out;
@@ -110,15 +111,20 @@ struct Segment {
     int vlo, vhi;               // positions any row sees: [fk, pfx) and [vlo, vhi]
     int t0, t1;                 // this CTA's share of the nt tiles
     int dest;
-    __device__ int tile(int i) const { return i < na ? a0 + i : b0 + i - na; }
-    __device__ bool seen(int j) const { return (j >= vlo && j <= vhi) || (j >= fk && j < pfx); }
+};
+
+// A segment's list of key tiles, in registers.
+struct TileList {
+    int a0, na, b0;
+    __device__ __forceinline__ explicit TileList(const Segment& g) : a0(g.a0), na(g.na), b0(g.b0 - g.na) {}
+    __device__ __forceinline__ int operator()(int i) const { return i + (i < na ? a0 : b0); }
 };
 
 struct Misc {
-    uint64_t full[5], empty[5], rfull[kRaw], rempty[kRaw];
+    uint64_t full[2][kRing16], empty[2][kRing16], rfull[kRaw], rempty[kRaw], vscale[kScales];
     uint64_t qfull, qempty, sfull[2], pready[2][2], odone[2][2], segfull[kSegs], segempty[kSegs], xbar, drain;
     Segment seg[kSegs];
-    long long scan[17];
+    long long scan[20];
     long long start, count, total;
     int start_id, start_head, start_off;
     uint32_t bad[kRaw];
@@ -127,23 +133,32 @@ struct Misc {
 };
 static_assert(sizeof(Misc) <= 2048, "the barrier block must fit behind the tiles");
 
+struct Scales {  // INT8 caches, see convert_role
+    float k[kScales][kTile], v[kScales][kTile];
+    int v_exp[kScales];
+};
+
 template <int FMT>
 struct Layout {
     static constexpr int ring = FMT == kF16 ? kRing16 : kRing8;
-    static constexpr int raw = 2 * kTileBytes + ring * kTileBytes;
+    static constexpr int tiles = 2 * kTileBytes;  // K's, then V's
+    static constexpr int raw = tiles + 2 * ring * kTileBytes;
     // results on their way out, see softmax_role
-    static constexpr int stage = raw + (FMT == kF16 ? 0 : kRaw * kRawBytes);
+    static constexpr int raw_scale = raw + kRaw * kRawBytes;
+    static constexpr int stage = raw + (FMT == kF16 ? 0 : kRaw * (kRawBytes + 256));
     static constexpr int stage_bytes = FMT == kF16 ? 32768 : 16384;
-    static constexpr int misc = stage + stage_bytes;
+    static constexpr int scales = stage + stage_bytes;
+    static constexpr int misc = scales + (FMT == kF16 ? 0 : 4352);
+    static_assert(sizeof(Scales) <= 4352, "scales");
     static constexpr int bytes = misc + 2048;
-    static constexpr int threads = FMT == kF16 ? 384 : 512;
+    static constexpr int threads = FMT == kF16 ? 384 : 640;
     // registers per thread: launched with `base`, then moved between the
     // warpgroups; the shares add up to threads * base
-    static constexpr int base = FMT == kF16 ? 168 : 128;
-    static constexpr int softmax_regs = FMT == kF16 ? 208 : 184;
-    static constexpr int other_regs = FMT == kF16 ? 88 : 48;
-    static constexpr int convert_regs = 96;
-    static_assert(2 * softmax_regs + other_regs + (FMT == kF16 ? 0 : convert_regs) <= threads / 128 * base,
+    static constexpr int base = FMT == kF16 ? 168 : 96;
+    static constexpr int softmax_regs = FMT == kF16 ? 208 : 136;
+    static constexpr int other_regs = FMT == kF16 ? 88 : 80;
+    static constexpr int convert_regs = 64;
+    static_assert(2 * softmax_regs + other_regs + (FMT == kF16 ? 0 : 2 * convert_regs) <= threads / 128 * base,
                   "register shares exceed what the block is launched with");
 };
 
@@ -258,14 +273,20 @@ __device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
 // tanh on [-0.8, 0.8] as an odd polynomial of degree 9, minimax in the absolute
 // error (3.5e-7): Remez exchange on tanh(t) / t over t^2, weighted by t.
 constexpr float kTanhNear = 0.8f;
-__device__ __forceinline__ float2 tanh_near(float2 t) {
-    const float2 y = mul2(t, t);
-    float2 r = fma2({0.01146465539932251f, 0.01146465539932251f}, y, {-0.04826131463050842f, -0.04826131463050842f});
-    r = fma2(r, y, {0.13186219334602356f, 0.13186219334602356f});
-    r = fma2(r, y, {-0.3331742584705353f, -0.3331742584705353f});
-    r = fma2(r, y, {0.9999951124191284f, 0.9999951124191284f});
-    return mul2(r, t);
-}
+struct TanhNear {  // up tanh(in s) for |in s| <= 0.8, the factors folded into the coefficients
+    float2 c[5];
+    __device__ __forceinline__ TanhNear(float in, float up) {
+        const float k[5] = {0.9999951124191284f, -0.3331742584705353f, 0.13186219334602356f, -0.04826131463050842f,
+                            0.01146465539932251f};
+        float f = up * in;
+#pragma unroll
+        for (int i = 0; i < 5; ++i, f *= in * in) c[i] = {k[i] * f, k[i] * f};
+    }
+    __device__ __forceinline__ float2 operator()(float2 s) const {
+        const float2 y = mul2(s, s);
+        return mul2(fma2(fma2(fma2(fma2(c[4], y, c[3]), y, c[2]), y, c[1]), y, c[0]), s);
+    }
+};
 
 // 2^x on the multiply-add pipe for x = 64 u - 56, u in [0, 1]: x splits into an
 // integer, added to the exponent, and a rest in [-1/2, 1/2], whose power is a
@@ -293,6 +314,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float d;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// A load from shared memory that stays where it is written (lifted out of the
+// loop below, a step's scales alone would fill the registers).
+__device__ __forceinline__ float4 load_scales(const float4* p) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_addr(p)));
+    return v;
+}
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo .. hi of a word
     const uint32_t from = lo <= 0 ? ~0u : lo > 31 ? 0u : ~0u << lo;
     const uint32_t to = hi >= 31 ? ~0u : hi < 0 ? 0u : (2u << hi) - 1u;
@@ -300,48 +333,56 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo .
 }
 
 // One step: the softmax of W score columns at s_addr, keys from j0, into W fp16
-// weights at p_addr. `m` is in score units, `sc` turns those into powers of
-// two. The weights are worked out with the maximum so far while the step's own
-// is still being found; only where that turns out to be too low (the first
-// step of a unit, rarely later) the maximum is raised and they are worked out
-// again. On its own the search would hold up every step by a quarter.
-template <int W, bool MOD>
+// weights at p_addr. `m` is the row's reference, in powers of two. The weights
+// are worked out with the reference so far; only where a score turns out to lie
+// more than 2^8 above it (in the first step of a unit, rarely later) the
+// maximum is searched for, the reference raised to it and the weights worked
+// out again. Searched for ahead of the weights it held up every step by a
+// quarter. Weights stay below 2^8, which fp16 holds.
+//
+// Scores come scaled by `kf` (and K's scales, INT8) to powers of two; with MOD,
+// capping and bias follow. INT8: ks holds kf times K's scales, vs V's scales
+// divided by 2^v_exp, the largest so far; the sums are in units of 2^ev. The
+// matrix instructions see the exact codes.
+template <int W, bool I8, bool MOD>
 __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Row& row, uint32_t s_addr, uint32_t p_addr,
                                              uint32_t o_addr, int j0, bool have_sums, uint64_t* odone,
-                                             uint32_t odone_parity, float sc, float& m, float& l) {
+                                             uint32_t odone_parity, const float4* ks, const float4* vs, int v_exp,
+                                             float& m, float& l, int& ev) {
     float s[W];
 #pragma unroll
     for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
     tmem_wait_ld();
+    const float kf = p.kf;
+    if (MOD && (I8 || p.cap == 0.f)) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const float4 k = I8 ? load_scales(ks + i / 4) : float4{kf, kf, kf, kf};
+            const float2 a = mul2({s[i], s[i + 1]}, {k.x, k.y}), b = mul2({s[i + 2], s[i + 3]}, {k.z, k.w});
+            s[i] = a.x;
+            s[i + 1] = a.y;
+            s[i + 2] = b.x;
+            s[i + 3] = b.y;
+        }
+    }
     const int j1 = j0 + W - 1;
     if (MOD) {
         if (p.cap > 0.f) {
-            const float in = p.scale / p.cap, up = p.cap * kLog2e;
-            const float2 in2 = {in, in}, up2 = {up, up};
-            float least = s[0], most = s[0];
+            const float in = I8 ? 1.f : kf, up = p.cap * kLog2e;
+            float far[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 1; i < W; ++i) {
-                least = fminf(least, s[i]);
-                most = fmaxf(most, s[i]);
-            }
-            if (__all_sync(kFull, fmaxf(most, -least) * in <= kTanhNear)) {
+            for (int i = 0; i < W; i += 2) far[i / 2 & 3] = max3_abs(far[i / 2 & 3], s[i], s[i + 1]);
+            if (__all_sync(kFull, fmaxf(max3(far[0], far[1], far[2]), far[3]) * in <= kTanhNear)) {
+                const TanhNear near(in, up);
 #pragma unroll
                 for (int i = 0; i < W; i += 2) {
-                    const float2 t = mul2(tanh_near(mul2({s[i], s[i + 1]}, in2)), up2);
+                    const float2 t = near({s[i], s[i + 1]});
                     s[i] = t.x;
                     s[i + 1] = t.y;
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < W; ++i) s[i] = up * tanh_exp(s[i] * in);
-            }
-        } else {
-            const float up = p.scale * kLog2e;
-#pragma unroll
-            for (int i = 0; i < W; i += 2) {
-                const float2 t = mul2({s[i], s[i + 1]}, {up, up});
-                s[i] = t.x;
-                s[i + 1] = t.y;
             }
         }
         if (p.slopes) {
@@ -372,42 +413,72 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
             for (int c = 0; c < 32; ++c) s[i + c] = (see >> c) & 1u ? s[i + c] : -INFINITY;
         }
     }
-    const float2 sc2 = {sc, sc};
-    const float sc_u = sc * (1.f / 64.f);
 #pragma unroll 1
-    for (;;) {
-        const float ms = m == -INFINITY ? 0.f : -m * sc, ms_u = (ms + 56.f) * (1.f / 64.f);
+    for (bool again = false;; again = true) {
+        const float ms = m == -INFINITY ? 0.f : -m, ms_u = (ms + 56.f) * (1.f / 64.f);
         const float2 ms2 = {ms, ms};
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint32_t w[W / 2];
+        float over[2] = {-INFINITY, -INFINITY}, full = 0.f;
+        uint32_t w[16];
+        float4 k4{}, v4{};
 #pragma unroll
         for (int c = 0; c < W / 2; ++c) {
             const float a = s[2 * c], b = s[2 * c + 1];
+            float2 k = {kf, kf}, v = {1.f, 1.f};
+            if (I8) {
+                if (c % 2 == 0) {
+                    if (!MOD) k4 = load_scales(ks + c / 2);
+                    v4 = load_scales(vs + c / 2);
+                }
+                k = c & 1 ? float2{k4.z, k4.w} : float2{k4.x, k4.y};
+                v = c & 1 ? float2{v4.z, v4.w} : float2{v4.x, v4.y};
+            }
             float2 x;
             if (c % 8 == 1 || c % 8 == 4 || c % 8 == 6) {  // 3 of 8 pairs: measured beside 2 and 4
-                x = exp2_cubic({fma_sat(a, sc_u, ms_u), fma_sat(b, sc_u, ms_u)});
+                float2 u;
+                if (I8 && !MOD) {
+                    x = fma2({a, b}, k, ms2);
+                    u = {fma_sat(x.x, 1.f / 64.f, 56.f / 64.f), fma_sat(x.y, 1.f / 64.f, 56.f / 64.f)};
+                } else {
+                    const float f = (MOD ? 1.f : kf) * (1.f / 64.f);
+                    u = {fma_sat(a, f, ms_u), fma_sat(b, f, ms_u)};
+                }
+                full = max3(full, u.x, u.y);
+                x = exp2_cubic(u);
             } else {
-                x = fma2({a, b}, sc2, ms2);
+                x = MOD ? add2({a, b}, ms2) : fma2({a, b}, k, ms2);
+                over[c & 1] = max3(over[c & 1], x.x, x.y);
                 x.x = fast_exp2(x.x);
                 x.y = fast_exp2(x.y);
             }
-            most[c & 3] = max3(most[c & 3], a, b);
             sum[c & 1] = add2(sum[c & 1], x);
-            w[c] = pack_f16(x.x, x.y);
+            if (I8) x = mul2(x, v);
+            w[c % 16] = pack_f16(x.x, x.y);
+            if (c % 16 == 15) tmem_st16(p_addr + c - 15, w);
         }
-        const float top = fmaxf(max3(most[0], most[1], most[2]), most[3]);
-        if (!__any_sync(kFull, (top - m) * sc > kRaise)) {
-#pragma unroll
-            for (int i = 0; i < W / 2; i += 16) tmem_st16(p_addr + i, w + i);
+        const bool low = fmaxf(over[0], over[1]) > kRaise || full >= 1.f || m == -INFINITY;
+        if (again || !__any_sync(kFull, low || (I8 && v_exp > ev))) {
             const float2 all = add2(sum[0], sum[1]);
             l += all.x + all.y;
             return true;
         }
+        tmem_wait_st();
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const float4 k = MOD ? float4{1.f, 1.f, 1.f, 1.f} : I8 ? load_scales(ks + i / 4) : float4{kf, kf, kf, kf};
+            top = max3(top, s[i] * k.x, s[i + 1] * k.y);
+            top = max3(top, s[i + 2] * k.z, s[i + 3] * k.w);
+        }
         const float up = fmaxf(m, top);
-        const float f = m == -INFINITY ? 0.f : fast_exp2((m - up) * sc);
+        const float f = m == -INFINITY ? 0.f : fast_exp2(m - up);
         m = up;
         l *= f;
+        float fo = f;
+        if (I8) {
+            fo *= fast_exp2(static_cast<float>(ev - v_exp));
+            ev = v_exp;
+        }
         if (have_sums) {
             if (odone && !warp_wait(odone, odone_parity, mi)) return false;
             tcgen05_fence_after();
@@ -417,7 +488,7 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
                 tmem_ld32(o_addr + c, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= f;
+                for (int i = 0; i < 32; ++i) o[i] *= fo;
                 tmem_st32(o_addr + c, o);
             }
         }
@@ -430,25 +501,33 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
 // only after the products of the tile before, so the sums can be scaled at once
 // in a tile's first step and after the first half's product in its second.
 // `tiles` and `halves` count the tiles, and those in two steps, so far.
-template <int NC, bool MOD>
-__device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Segment& g, const Row& row, int stream,
-                                            uint32_t s_addr, uint32_t o_addr, float sc, uint32_t& tiles, uint32_t& halves,
-                                            float& m, float& l) {
+// `before`: tiles of earlier segments.
+template <int NC, bool I8, bool MOD>
+__device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Scales* scales, const Segment& g,
+                                            const Row& row, int stream, uint32_t before, uint32_t s_addr,
+                                            uint32_t o_addr, uint32_t& tiles, uint32_t& halves, float& m,
+                                            float& l, int& ev) {
     constexpr int W = NC == 128 ? 64 : NC;
     const int warp = (threadIdx.x >> 5) & 3;
     const int c0 = NC == 128 ? 0 : NC == 64 ? (warp >> 1) * 64 : warp * 32;
     const int step = g.rep ? 2 : 1;
-    const int i0 = g.t0 + (g.rep ? stream : 0);
+    const int t0 = g.t0, t1 = g.t1, i0 = t0 + (g.rep ? stream : 0);
+    const TileList tile(g);
 #pragma unroll 1
-    for (int i = i0; i < g.t1; i += step) {
+    for (int i = i0; i < t1; i += step) {
         if (!warp_wait(&mi->sfull[stream], tiles & 1, mi)) return false;
         ++tiles;
         tcgen05_fence_after();
-        const int j0 = g.tile(i) * kTile + c0;
+        const int j0 = tile(i) * kTile + c0;
+        const uint32_t at = before + i - t0, st = at % kScales;
+        if (I8 && !warp_wait(&mi->vscale[st], (at / kScales) & 1, mi)) return false;
+        const int v_exp = I8 ? scales->v_exp[st] : 0;
 #pragma unroll 1
         for (int c = 0; c < NC; c += W) {
-            if (!softmax_step<W, MOD>(p, mi, row, s_addr + c0 + c, s_addr + (c0 + c) / 2, o_addr, j0 + c, i > i0 || c > 0,
-                                      c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1, sc, m, l))
+            if (!softmax_step<W, I8, MOD>(p, mi, row, s_addr + c0 + c, s_addr + (c0 + c) / 2, o_addr, j0 + c,
+                                          i > i0 || c > 0, c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1,
+                                          reinterpret_cast<const float4*>(scales->k[st] + c0 + c),
+                                          reinterpret_cast<const float4*>(scales->v[st] + c0 + c), v_exp, m, l, ev))
                 return false;
             if (NC < kTile) {  // the other copies' columns weigh nothing in this one
                 const uint32_t z[16] = {};
@@ -513,8 +592,8 @@ __device__ __forceinline__ void store_wide(unsigned char* stage, unsigned char* 
                 u = {pack_f16(o[8 * i] * f, o[8 * i + 1] * f), pack_f16(o[8 * i + 2] * f, o[8 * i + 3] * f),
                      pack_f16(o[8 * i + 4] * f, o[8 * i + 5] * f), pack_f16(o[8 * i + 6] * f, o[8 * i + 7] * f)};
             } else {
-                u = {__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]), __float_as_uint(o[4 * i + 2]),
-                     __float_as_uint(o[4 * i + 3])};
+                u = {__float_as_uint(o[4 * i] * f), __float_as_uint(o[4 * i + 1] * f),
+                     __float_as_uint(o[4 * i + 2] * f), __float_as_uint(o[4 * i + 3] * f)};
             }
             *reinterpret_cast<uint4*>(mine + lane * bytes + ((i ^ (lane & (lanes - 1))) << 4)) = u;
         }
@@ -538,10 +617,11 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
     const int stream = threadIdx.x >> 7, r_in = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>(r_in & 96) << 16;
     const uint32_t s_addr = tmem + lane_base + stream * 128, o_addr = s_addr + 256;
-    const float sc = MOD ? 1.f : p.scale * kLog2e;
     const int per = kTile / p.group;
     unsigned char* const stage = smem + Layout<FMT>::stage;
-    uint32_t tiles = 0, halves = 0, xphase = 0;
+    const Scales* scales = reinterpret_cast<const Scales*>(smem + Layout<FMT>::scales);
+    constexpr bool I8 = FMT != kF16;
+    uint32_t tiles = 0, halves = 0, before = 0, xphase = 0;
     bool wide_before = false;
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
@@ -566,30 +646,33 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
             if (MOD && p.slopes) row.slope = p.slopes[hr] * kLog2e;
         }
         float m = -INFINITY, l = 0.f;
+        int ev = -200;
         const int mine = g.rep ? (g.t1 - g.t0 - stream + 1) / 2 : g.t1 - g.t0;  // tiles of this stream
         bool ok;
         if (g.rep == 4)
-            ok = softmax_run<32, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, halves, m, l);
+            ok = softmax_run<32, I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev);
         else if (g.rep == 2)
-            ok = softmax_run<64, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, halves, m, l);
+            ok = softmax_run<64, I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev);
         else
-            ok = softmax_run<128, MOD>(p, mi, g, row, stream, s_addr, o_addr, sc, tiles, halves, m, l);
+            ok = softmax_run<128, I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev);
         if (!ok) return;
+        before += g.t1 - g.t0;
+        const float unit_v = I8 && mine > 0 ? fast_exp2(static_cast<float>(ev)) : 1.f;
         if (mine > 0) {
             if (!warp_wait(&mi->odone[stream][1], (tiles - 1) & 1, mi)) return;
             tcgen05_fence_after();
         }
         if (m == -INFINITY) l = 0.f;
-        const float m2 = l > 0.f ? m * sc : -INFINITY;
+        const float m2 = l > 0.f ? m : -INFINITY;
         if (g.rep == 0) {
             const uint32_t row_at = live ? dest_row(p, g, tok, hr, tl * p.group + hr - g.head * p.group) : ~0u;
             if (live) store_ml(p, g, row_at, m2, l);
             if (g.dest == kDirect)
                 store_wide<FMT, true>(stage, reinterpret_cast<unsigned char*>(p.out), o_addr, mine > 0, row_at,
-                                      l > 0.f ? 1.f / l : 0.f);
+                                      l > 0.f ? unit_v / l : 0.f);
             else
                 store_wide<FMT, false>(stage, reinterpret_cast<unsigned char*>(g.dest == kSlot ? p.part : p.rowbuf),
-                                       o_addr, mine > 0, row_at, 1.f);
+                                       o_addr, mine > 0, row_at, unit_v);
         } else {
             // join the copies and streams: each scales its sums to the row's
             // common maximum, then 256 threads add the states in order
@@ -602,7 +685,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
             if (!softmax_sync(mi, xphase)) return;
             float top = -INFINITY;
             for (int t = 0; t < states; ++t) top = fmaxf(top, ml[t * block + rr].x);
-            const float f = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top);
+            const float f = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top) * unit_v;
             int dc = 128;  // channels per pass: what fits the scratch space (states * rows <= 256)
             while (states * rows * dc * 4 > Layout<FMT>::stage_bytes - 2048) dc >>= 1;
             const int quads = dc / 4, spread = min(quads, 8) - 1;
@@ -668,13 +751,13 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
     constexpr int ring = Layout<FMT>::ring;
     constexpr uint32_t id_qk = mma_idesc_f16(128, 128, false), id_pv = mma_idesc_f16(128, 128, true);
     const int lane = threadIdx.x & 31;
-    const uint32_t q_addr = smem_addr(smem), r_addr = q_addr + 2 * kTileBytes;
-    uint32_t pos = 0, ph[2][2] = {};  // ring entries taken; weights taken per stream and half
-    auto wait_entry = [&](uint32_t e) { return warp_wait(&mi->full[e % ring], (e / ring) & 1, mi); };
+    const uint32_t q_addr = smem_addr(smem), k_addr = q_addr + Layout<FMT>::tiles, v_addr = k_addr + ring * kTileBytes;
+    uint32_t n_k = 0, n_v = 0, ph[2][2] = {};  // tiles of K and V; weights taken per stream and half
+    auto wait_tile = [&](int v, uint32_t e) { return warp_wait(&mi->full[v][e % ring], (e / ring) & 1, mi); };
     // descriptors differ by constants: one addition each, in uniform registers
     const uint32_t leader = elect_one();
-    const uint64_t q_desc = smem_desc(q_addr, 16, 1024), k_desc = smem_desc(r_addr, 16, 1024),
-                   v_desc = smem_desc(r_addr, kHalfTile, 1024);
+    const uint64_t q_desc = smem_desc(q_addr, 16, 1024), k_desc = smem_desc(k_addr, 16, 1024),
+                   v_desc = smem_desc(v_addr, kHalfTile, 1024);
     auto qk = [&](int stream, int qslot, uint32_t e) {
         tcgen05_fence_after();
         const uint64_t a = q_desc + qslot * (kTileBytes >> 4), b = k_desc + (e % ring) * (kTileBytes >> 4);
@@ -708,15 +791,15 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
         mma_commit(&mi->odone[stream][1], leader);
         return true;
     };
-    auto release = [&](uint32_t e) { mma_commit(&mi->empty[e % ring], leader); };
+    auto release = [&](int v, uint32_t e) { mma_commit(&mi->empty[v][e % ring], leader); };
     // fp16 V rows that no row of the unit sees may hold anything (the end of a
     // page, tokens that left the window): 0 * NaN would reach the sums
-    auto clean = [&](const Segment& g, int tile, uint32_t e) {
+    auto clean = [&](int4 seen, int tile, uint32_t e) {
         if (FMT != kF16) return;  // the conversion writes zeros there
         const int j0 = tile * kTile;
-        const int lo = g.vlo - j0, hi = g.vhi - j0, fk = g.fk - j0, pfx = g.pfx - j0;
+        const int lo = seen.x - j0, hi = seen.y - j0, fk = seen.z - j0, pfx = seen.w - j0;
         if ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) return;
-        unsigned char* v = smem + 2 * kTileBytes + (e % ring) * kTileBytes + (lane & 7) * 16;
+        unsigned char* v = smem + Layout<FMT>::tiles + (ring + e % ring) * kTileBytes + (lane & 7) * 16;
 #pragma unroll 4
         for (int r = lane >> 3; r < kTile; r += 4) {
             if (!((r >= lo && r <= hi) || (r >= fk && r < pfx))) {
@@ -732,57 +815,51 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
-        const int n = __shfl_sync(kFull, g.t1 - g.t0, 0);  // known to be uniform
+        const int t0 = g.t0, n = __shfl_sync(kFull, g.t1 - t0, 0);  // known to be uniform
+        const TileList tile(g);
+        const int4 seen = {g.vlo, g.vhi, g.fk, g.pfx};
         if (n > 0) {
             if (!warp_wait(&mi->qfull, qk_seg++ & 1, mi)) return;
             const int rep = __shfl_sync(kFull, g.rep, 0);
             if (rep == 0) {
-                if (!wait_entry(pos)) return;
-                qk(0, 0, pos);
-                qk(1, 1, pos);
-                release(pos);
-                ++pos;
+                if (!wait_tile(0, n_k)) return;
+                qk(0, 0, n_k);
+                qk(1, 1, n_k);
+                release(0, n_k++);
                 if (n == 1) mma_commit(&mi->qempty, leader);
                 for (int i = 0; i < n; ++i) {
-                    const uint32_t ve = pos, ke = pos + 1;
                     const bool more = i + 1 < n;
-                    if (!wait_entry(ve)) return;
-                    clean(g, g.tile(g.t0 + i), ve);
+                    if (!wait_tile(1, n_v)) return;
+                    clean(seen, tile(t0 + i), n_v);
 #pragma unroll
                     for (int s = 0; s < 2; ++s) {
-                        if (!pv(s, ve, i == 0, true)) return;
+                        if (!pv(s, n_v, i == 0, true)) return;
                         if (more) {
-                            if (s == 0 && !wait_entry(ke)) return;
-                            qk(s, s, ke);
+                            if (s == 0 && !wait_tile(0, n_k)) return;
+                            qk(s, s, n_k);
                         }
                     }
-                    release(ve);
-                    if (more) {
-                        release(ke);
-                        if (i + 2 == n) mma_commit(&mi->qempty, leader);
-                    }
-                    pos += more ? 2 : 1;
+                    release(1, n_v++);
+                    if (more) release(0, n_k++);
+                    if (i + 2 == n) mma_commit(&mi->qempty, leader);
                 }
             } else {
                 for (int s = 0; s < min(n, 2); ++s) {
-                    if (!wait_entry(pos)) return;
-                    qk(s, 0, pos);
-                    release(pos);
-                    ++pos;
+                    if (!wait_tile(0, n_k)) return;
+                    qk(s, 0, n_k);
+                    release(0, n_k++);
                 }
                 if (n <= 2) mma_commit(&mi->qempty, leader);
                 for (int i = 0; i < n; ++i) {
                     const int s = i & 1;
-                    if (!wait_entry(pos)) return;
-                    clean(g, g.tile(g.t0 + i), pos);
-                    if (!pv(s, pos, i < 2, rep == 1)) return;
-                    release(pos);
-                    ++pos;
+                    if (!wait_tile(1, n_v)) return;
+                    clean(seen, tile(t0 + i), n_v);
+                    if (!pv(s, n_v, i < 2, rep == 1)) return;
+                    release(1, n_v++);
                     if (i + 2 < n) {
-                        if (!wait_entry(pos)) return;
-                        qk(s, 0, pos);
-                        release(pos);
-                        ++pos;
+                        if (!wait_tile(0, n_k)) return;
+                        qk(s, 0, n_k);
+                        release(0, n_k++);
                         if (i + 3 == n) mma_commit(&mi->qempty, leader);
                     }
                 }
@@ -794,93 +871,126 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
 
 // ---- copies --------------------------------------------------------------------
 
-// Ring order, shared with the consumers: K of the first L tiles (wide units 1,
-// narrow units 2), then V_i, K_{i + L} for every tile i.
+// Order of the copies: K of the first L tiles (wide units 1, narrow units 2),
+// then V_i, K_{i + L} for every tile i. K and V have rings of their own, so
+// that each barrier's phases have one waiter that sees every one of them:
+// a parity says nothing to a waiter that may be two phases behind.
 template <int FMT>
 __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const Maps& maps) {
+    // fp16: a ring of K tiles and one of V tiles; INT8: one ring of code tiles
     constexpr int ring = FMT == kF16 ? Layout<FMT>::ring : kRaw;
-    uint64_t* const full = FMT == kF16 ? mi->full : mi->rfull;
-    uint64_t* const empty = FMT == kF16 ? mi->empty : mi->rempty;
     const int lane = threadIdx.x & 31;
-    const int subs = kTile / p.box_rows;                       // boxes of a tile
-    const int sub = FMT == kF16 ? lane >> 1 : lane;            // this lane's box
-    uint32_t pos = 0, q_seg = 0;  // tiles and query loads so far
+    const int subs = kTile >> p.box_shift;  // boxes of a tile: 1 to 8
+    // One instruction issues a V tile's boxes (lower half warp) and a K tile's
+    // (upper half): issued one by one they take the warp 200 clocks each.
+    const bool is_k = lane >= 16;
+    const int sub = FMT == kF16 ? lane >> 1 & 7 : lane & 7;
+    const int part = FMT == kF16 ? lane & 1 : lane >> 3 & 1;  // half of the channels; codes or scales
+    uint32_t n_k = 0, n_v = 0, q_seg = 0;                      // tiles and query loads so far
+    auto full_of = [&](bool v, uint32_t e) { return FMT == kF16 ? &mi->full[v][e % ring] : &mi->rfull[e % ring]; };
+    auto claim = [&](bool v, uint32_t& e) {  // the next ring entry, once it is free
+        e = FMT != kF16 ? n_k + n_v : v ? n_v : n_k;
+        const uint32_t st = e % ring;
+        ++(v ? n_v : n_k);
+        return e < ring || warp_wait(FMT == kF16 ? &mi->empty[v][st] : &mi->rempty[st], (e / ring - 1) & 1, mi);
+    };
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) break;
         const Segment& g = mi->seg[slot];
         if (!g.valid) break;
-        const int n = g.t1 - g.t0;
+        const int t0 = g.t0, n = g.t1 - t0, rep = g.rep;
         bool ok = true;
         if (n > 0) {
+            const TileList tile(g);
+            const int vlo = g.vlo, vhi = g.vhi, fk = g.fk, pfx = g.pfx, head = g.head, tok0 = g.tok0;
+            const KeySet& ks = p.set[g.set];
+            const int* const table = ks.tables + static_cast<size_t>(g.seq) * ks.width;
+            // Pages of 32 boxes (of 32 / subs tiles), one per lane: the page
+            // number, -1 if it is none, -2 where nothing is seen.
+            auto look = [&](int batch) {
+                const int q = batch * 32 + lane, i = q / subs;
+                if (i >= n) return -2;
+                const int j = tile(t0 + i) * kTile + ((q & (subs - 1)) << p.box_shift), e = j + p.box_rows - 1;
+                if (!((e >= vlo && j <= vhi) || (e >= fk && j < pfx))) return -2;
+                return max(__ldg(table + j / p.block_size), -1);
+            };
+            // its row in the caches; the row past the last reads as zeros
+            auto place = [&](int page, int batch) {
+                if (page == -2) return p.total_rows;
+                if (page < 0 || page >= p.num_blocks) {
+                    atomicCAS(&g_attention_error, 0, static_cast<int>(kDevBadBlock));
+                    return p.total_rows;
+                }
+                const int q = batch * 32 + lane;
+                const int j = tile(t0 + q / subs) * kTile + ((q & (subs - 1)) << p.box_shift);
+                return (page * p.n_kv + head) * p.block_size + j % p.block_size;
+            };
+            int batch = 0;
+            const int look0 = look(0), look1 = look(1);
+            int ahead = look(2);
             // queries: the last segment's score tiles are done with them
             if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
             ++q_seg;
-            const int copies = g.rep ? g.rep : 2, block = g.rep ? kTile / g.rep : kTile;
+            const int copies = rep ? rep : 2, block = rep ? kTile / rep : kTile;
             const int toks = block / p.group;
-            const CUtensorMap* qm = &maps.q[g.rep == 4 ? 2 : g.rep == 2 ? 1 : 0];
+            const CUtensorMap* qm = &maps.q[rep == 4 ? 2 : rep == 2 ? 1 : 0];
             if (lane == 0) mbar_arrive_expect_tx(&mi->qfull, static_cast<uint32_t>(copies * toks * p.group * 256));
             __syncwarp();
             if (lane < 2 * copies) {
                 const int c = lane >> 1, half = lane & 1;
-                unsigned char* dst = smem + (g.rep ? c * block * 128 : c * kTileBytes) + half * kHalfTile;
-                tma_load_3d(dst, qm, half * 64, g.head * p.group, g.tok0 + (g.rep ? 0 : c * toks), &mi->qfull);
+                unsigned char* dst = smem + (rep ? c * block * 128 : c * kTileBytes) + half * kHalfTile;
+                tma_load_3d(dst, qm, half * 64, head * p.group, tok0 + (rep ? 0 : c * toks), &mi->qfull);
             }
-            // page of this lane's box in tile i of the list; -2: nothing there is seen
-            auto page = [&](int i) {
-                if (i >= g.t1 || sub >= subs) return -2;
-                const int j = g.tile(i) * kTile + sub * p.box_rows, e = j + p.box_rows - 1;
-                if (!((e >= g.vlo && j <= g.vhi) || (e >= g.fk && j < g.pfx))) return -2;
-                const KeySet& ks = p.set[g.set];
-                return __ldg(ks.tables + static_cast<size_t>(g.seq) * ks.width + j / p.block_size);
-            };
-            auto load = [&](bool v, int i, int pg) {
-                const int st = pos % ring;
-                if (pos >= ring && !warp_wait(&empty[st], (pos / ring - 1) & 1, mi)) return false;
-                ++pos;
-                const bool bad = pg != -2 && (pg < 0 || pg >= p.num_blocks);
-                if (bad) atomicCAS(&g_attention_error, 0, static_cast<int>(kDevBadBlock));
-                const bool there = pg >= 0 && !bad;
-                const int j = g.tile(i) * kTile + sub * p.box_rows;
-                // a row past the end reads as zeros
-                const int row = there ? (pg * p.n_kv + g.head) * p.block_size + j % p.block_size : p.total_rows;
-                const CUtensorMap* map = v ? &maps.v : &maps.k;
+            int rows = place(look0, 0), rows_next = place(look1, 1);
+            // V of tile iv and K of tile ik (of the list; < 0: none)
+            auto load = [&](int iv, int ik) {
+                uint32_t ev = 0, ek = 0;
+                if (iv >= 0 && !claim(true, ev)) return false;
+                if (ik >= 0 && !claim(false, ek)) return false;
+                const int q = (is_k ? max(ik, 0) : max(iv, 0)) * subs + sub;
+                const int r0 = __shfl_sync(kFull, rows, q & 31), r1 = __shfl_sync(kFull, rows_next, q & 31);
+                const int row = (q >> 5) == batch ? r0 : r1;
+                const bool mine = sub < subs && (is_k ? ik >= 0 : iv >= 0);
+                const uint32_t e = is_k ? ek : ev;
+                uint64_t* const full = full_of(!is_k, e);
+                const uint32_t st = e % ring;
+                const CUtensorMap* map = is_k ? &maps.k : &maps.v;
                 if (FMT == kF16) {
-                    if (lane == 0) mbar_arrive_expect_tx(&full[st], kTileBytes);
+                    if ((lane == 0 && iv >= 0) || (lane == 16 && ik >= 0)) mbar_arrive_expect_tx(full, kTileBytes);
                     __syncwarp();
-                    if (sub < subs)
-                        tma_load_2d(smem + 2 * kTileBytes + st * kTileBytes + (lane & 1) * kHalfTile +
-                                        sub * p.box_rows * 128,
-                                    map, (lane & 1) * 64, row, &full[st]);
+                    if (mine)
+                        tma_load_2d(smem + Layout<FMT>::tiles + ((is_k ? 0 : ring) + st) * kTileBytes + part * kHalfTile +
+                                        (sub << p.box_shift) * 128,
+                                    map, part * 64, row, full);
                 } else {
-                    const unsigned here = __ballot_sync(kFull, there && sub < subs);
-                    if (lane == 0) {
-                        mi->bad[st] = ~here;
-                        mbar_arrive_expect_tx(&full[st], kTile * kHeadDim + __popc(here) * p.box_rows * 2);
+                    const bool there = mine && row != p.total_rows;
+                    const unsigned here = __ballot_sync(kFull, there && part == 0) >> (lane & 16) & 0xffu;
+                    if ((lane == 0 && iv >= 0) || (lane == 16 && ik >= 0)) {
+                        mi->bad[st] = ~here & ((1u << subs) - 1);
+                        mbar_arrive_expect_tx(full, kRawBytes + (__popc(here) << p.box_shift) * 2);
                     }
                     __syncwarp();
-                    if (sub < subs) {
-                        unsigned char* dst = smem + Layout<FMT>::raw + st * kRawBytes;
-                        tma_load_2d(dst + sub * p.box_rows * kHeadDim, map, 0, row, &full[st]);
-                        if (there)
-                            bulk_g2s_plain(dst + kTile * kHeadDim + sub * p.box_rows * 2, (v ? p.v_scale : p.k_scale) + row,
-                                           p.box_rows * 2, &full[st]);
-                    }
+                    if (mine && part == 0)
+                        tma_load_2d(smem + Layout<FMT>::raw + st * kRawBytes + (sub << p.box_shift) * kHeadDim, map, 0, row,
+                                    full);
+                    if (there && part == 1)
+                        bulk_g2s_plain(smem + Layout<FMT>::raw_scale + st * 256 + (sub << p.box_shift) * 2,
+                                       (is_k ? p.k_scale : p.v_scale) + row, p.box_rows * 2, full);
                 }
                 __syncwarp();
                 return true;
             };
-            const int L = g.rep ? 2 : 1;
-            int e0 = page(g.t0), e1 = page(g.t0 + 1), e2 = page(g.t0 + 2);
-            ok = load(false, g.t0, e0);
-            if (ok && L == 2 && n > 1) ok = load(false, g.t0 + 1, e1);
-            for (int i = g.t0; ok && i < g.t1; ++i) {
-                const int e3 = page(i + 3);
-                ok = load(true, i, e0);
-                if (ok && i + L < g.t1) ok = load(false, i + L, L == 2 ? e2 : e1);
-                e0 = e1;
-                e1 = e2;
-                e2 = e3;
+            const int L = rep ? 2 : 1;
+            ok = load(-1, 0) && (L == 1 || n == 1 || load(-1, 1));
+            for (int i = 0; ok && i < n; ++i) {
+                if ((i * subs) >> 5 != batch) {
+                    ++batch;
+                    rows = rows_next;
+                    rows_next = place(ahead, batch + 1);
+                    ahead = look(batch + 2);
+                }
+                ok = load(i, i + L < n ? i + L : -1);
             }
         }
         if (!ok) break;
@@ -888,8 +998,16 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
     }
     // Leave no copy in flight: after an abort nobody else waits for them.
     if (*reinterpret_cast<volatile int*>(&mi->abort)) {
-        for (uint32_t e = pos > ring ? pos - ring : 0; e < pos; ++e)
-            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&full[e % ring], (e / ring) & 1); ++i) {}
+        auto settle = [&](bool v, uint32_t n) {
+            for (uint32_t e = n > ring ? n - ring : 0; e < n; ++e)
+                for (uint32_t i = 0; i < kPolls && !mbar_try_wait(full_of(v, e), (e / ring) & 1); ++i) {}
+        };
+        if (FMT == kF16) {
+            settle(false, n_k);
+            settle(true, n_v);
+        } else {
+            settle(false, n_k + n_v);
+        }
         if (q_seg > 0)
             for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->qfull, (q_seg - 1) & 1); ++i) {}
     }
@@ -897,57 +1015,106 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
 
 // ---- INT8 conversion -------------------------------------------------------------
 
+// Codes to fp16 integers (exact) in the swizzled tile, scales to fp32; one
+// warpgroup for K, one for V (a single one took 4200 clocks for a tile of both,
+// three times what its bytes take from memory). V's
+// scales go out before V's codes wait for room, since the softmax of the tile
+// needs them; they are divided by the power of two above the segment's largest
+// so far, so that weight * scale fits fp16. Rows that no row of the unit sees,
+// and rows of pages that are not there, become zeros with scale zero.
+template <bool V>
 __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem) {
     constexpr int ring = Layout<kI8>::ring;
+    Scales* const scales = reinterpret_cast<Scales*>(smem + Layout<kI8>::scales);
     const int t = threadIdx.x & 127;
-    const int c = t & 7, r0 = t >> 3;  // 16 channels of rows r0, r0 + 16, ...
-    uint32_t pos = 0;
-    auto convert = [&](const Segment& g, int tile) {
-        const int st = pos % kRaw, d = pos % ring;
-        if (!warp_wait(&mi->rfull[st], (pos / kRaw) & 1, mi)) return false;
-        if (pos >= ring && !warp_wait(&mi->empty[d], (pos / ring - 1) & 1, mi)) return false;
-        const unsigned char* src = smem + Layout<kI8>::raw + st * kRawBytes;
-        const __half* scale = reinterpret_cast<const __half*>(src + kTile * kHeadDim);
-        unsigned char* dst = smem + 2 * kTileBytes + d * kTileBytes + (c >> 2) * kHalfTile;
-        const uint32_t bad = mi->bad[st];
-        const int j0 = tile * kTile;
+    // 16 channels (chunk c) of eight rows. A quarter warp holds chunks of one
+    // half of rows q and q ^ 5: both the swizzled codes it reads and the
+    // swizzled tile it writes then spread over all banks.
+    const int lane = t & 31;
+    const int c = (lane & 3) + (lane >> 1 & 4), turn = lane & 4 ? 5 : 0, x = (c & 3) * 2;
+    const int r0 = (t >> 5) * 32 + (lane >> 4);
+    auto row_of = [&](int i) { return (r0 + (i >> 1) * 8 + (i & 1) * 2) ^ turn; };
+    uint32_t pos = 0, done = 0;  // code tiles; of this warpgroup's kind
+    int top = 0;  // V's exponent
+    // `seen(r)`: whether row r counts
+    auto convert_tile = [&](const unsigned char* src, int st, auto seen) {
+        const __half* scale = reinterpret_cast<const __half*>(smem + Layout<kI8>::raw_scale + st * 256);
+        const uint32_t n = done++;
+        const int at = n % kScales, d = n % ring;
+        if (!V) {
+            // never zero: a hidden key's score is -inf times this
+            scales->k[at][t] = seen(t) ? fmaxf(__half2float(scale[t]) * p.kf, 1e-30f) : 1.f;
+        } else {
+            const int r4 = (t & 31) * 4;
+            const uint2 raw = *reinterpret_cast<const uint2*>(scale + r4);
+            const float2 a = __half22float2(as_h2(raw.x)), b = __half22float2(as_h2(raw.y));
+            const float most = fmaxf(fmaxf(seen(r4) ? a.x : 0.f, seen(r4 + 1) ? a.y : 0.f),
+                                     fmaxf(seen(r4 + 2) ? b.x : 0.f, seen(r4 + 3) ? b.y : 0.f));
+            const uint32_t bits = __reduce_max_sync(kFull, __float_as_uint(most));
+            top = max(top, static_cast<int>(bits >> 23) - 126);
+            scales->v[at][t] = seen(t) ? __half2float(scale[t]) * __int_as_float((127 - top) << 23) : 0.f;
+            scales->v_exp[at] = top;
+            warp_arrive(&mi->vscale[at]);
+        }
+        uint4 in[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int r = r0 + 16 * i;
-            const uint4 w = *reinterpret_cast<const uint4*>(src + r * kHeadDim + c * 16);
-            const half2 s = __half2half2(scale[r]);
-            const bool keep = g.seen(j0 + r) && !((bad >> (r / p.box_rows)) & 1);
-            uint32_t o[8];
-            const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+            const int r = row_of(i);
+            in[i] = *reinterpret_cast<const uint4*>(src + r * kHeadDim + ((c ^ (r & 7)) << 4));
+        }
+        warp_arrive(&mi->rempty[st]);
+        if (n >= ring && !warp_wait(&mi->empty[V][d], (n / ring - 1) & 1, mi)) return false;
+        unsigned char* dst = smem + Layout<kI8>::tiles + ((V ? ring : 0) + d) * kTileBytes + (c >> 2) * kHalfTile;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                half2 a, b;
-                i8x4_to_h2(in[q], a, b);
-                o[2 * q] = keep ? as_u32(__hmul2(a, s)) : 0u;
-                o[2 * q + 1] = keep ? as_u32(__hmul2(b, s)) : 0u;
-            }
+        for (int i = 0; i < 8; ++i) {
+            const int r = row_of(i);
+            const uint4 w = seen(r) ? in[i] : uint4{0, 0, 0, 0};
+            half2 o[4];
             unsigned char* line = dst + r * 128;
-            const int x = (c & 3) * 2;
-            *reinterpret_cast<uint4*>(line + ((x ^ (r & 7)) << 4)) = uint4{o[0], o[1], o[2], o[3]};
-            *reinterpret_cast<uint4*>(line + (((x + 1) ^ (r & 7)) << 4)) = uint4{o[4], o[5], o[6], o[7]};
+            i8x4_to_h2(w.x, o[0], o[1]);
+            i8x4_to_h2(w.y, o[2], o[3]);
+            *reinterpret_cast<uint4*>(line + ((x ^ (r & 7)) << 4)) =
+                uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
+            i8x4_to_h2(w.z, o[0], o[1]);
+            i8x4_to_h2(w.w, o[2], o[3]);
+            *reinterpret_cast<uint4*>(line + (((x + 1) ^ (r & 7)) << 4)) =
+                uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
         }
         fence_async_smem();
-        warp_arrive(&mi->rempty[st]);
-        warp_arrive(&mi->full[d]);
-        ++pos;
+        warp_arrive(&mi->full[V][d]);
         return true;
+    };
+    auto convert = [&](int4 range, int tile) {
+        const int st = pos % kRaw;
+        const int j0 = tile * kTile;
+        const int lo = range.x - j0, hi = range.y - j0, fk = range.z - j0, pfx = range.w - j0;
+        if (!warp_wait(&mi->rfull[st], (pos / kRaw) & 1, mi)) return false;
+        const unsigned char* src = smem + Layout<kI8>::raw + st * kRawBytes;
+        const uint32_t bad = mi->bad[st];
+        const bool all = ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) && bad == 0;
+        if (__all_sync(kFull, all)) return convert_tile(src, st, [](int) { return true; });
+        return convert_tile(src, st, [&](int r) {
+            return ((r >= lo && r <= hi) || (r >= fk && r < pfx)) && !((bad >> (r >> p.box_shift)) & 1);
+        });
     };
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
-        const int n = g.t1 - g.t0, L = g.rep ? 2 : 1;
-        for (int i = 0; i < min(n, L); ++i)
-            if (!convert(g, g.tile(g.t0 + i))) return;
+        const int t0 = g.t0, n = g.t1 - t0, L = g.rep ? 2 : 1;
+        const TileList tile(g);
+        const int4 range = {g.vlo, g.vhi, g.fk, g.pfx};
+        top = -60;
+        for (int i = 0; i < min(n, L); ++i, ++pos)
+            if (!V && !convert(range, tile(t0 + i))) return;
         for (int i = 0; i < n; ++i) {
-            if (!convert(g, g.tile(g.t0 + i))) return;
-            if (i + L < n && !convert(g, g.tile(g.t0 + i + L))) return;
+            if (V && !convert(range, tile(t0 + i))) return;
+            ++pos;
+            if (i + L < n) {
+                if (!V && !convert(range, tile(t0 + i + L))) return;
+                ++pos;
+            }
         }
         warp_arrive(&mi->segempty[slot]);
     }
@@ -1079,10 +1246,12 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     Misc* mi = reinterpret_cast<Misc*>(smem + Lay::misc);
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
-        const int readers = FMT == kF16 ? 10 : 14;  // warps that read a segment
-        for (int i = 0; i < Lay::ring; ++i) {
-            mbar_init(&mi->full[i], FMT == kF16 ? 1 : 4);
-            mbar_init(&mi->empty[i], 1);
+        const int readers = FMT == kF16 ? 10 : 18;  // warps that read a segment
+        for (int v = 0; v < 2; ++v) {
+            for (int i = 0; i < Lay::ring; ++i) {
+                mbar_init(&mi->full[v][i], FMT == kF16 ? 1 : 4);
+                mbar_init(&mi->empty[v][i], 1);
+            }
         }
         for (int i = 0; i < kRaw; ++i) {
             mbar_init(&mi->rfull[i], 1);
@@ -1101,6 +1270,7 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
             mbar_init(&mi->segfull[i], 1);
             mbar_init(&mi->segempty[i], readers);
         }
+        for (int i = 0; i < kScales; ++i) mbar_init(&mi->vscale[i], 4);
         mbar_init(&mi->xbar, 8);
         mbar_init(&mi->drain, 1);
         mi->abort = 0;
@@ -1136,7 +1306,10 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     } else {
         if constexpr (FMT != kF16) {
             regs_dec<Lay::convert_regs>();
-            convert_role(p, mi, smem);
+            if (warp < 16)
+                convert_role<false>(p, mi, smem);
+            else
+                convert_role<true>(p, mi, smem);
         }
     }
     __syncwarp();
@@ -1164,7 +1337,10 @@ struct Join {
         l = l * a + e.y * b;
         v = {v.x * a + o.x * b, v.y * a + o.y * b, v.z * a + o.z * b, v.w * a + o.w * b};
     }
+    // A CTA that gave up (a wait ran out) may have left its entries unwritten:
+    // what is out of range is left out, and the error word has told.
     __device__ void add_slots(const Params& p, int first, int last, int unit_row, int lane) {
+        if (first < 0 || last >= p.grid || unit_row >= p.slot_rows) return;
         for (int c = first; c <= last; ++c)
             add(p.part_ml, p.part, static_cast<size_t>(2 * c + (c == first)) * p.slot_rows + unit_row, lane);
     }
@@ -1182,7 +1358,8 @@ __global__ void __launch_bounds__(256) join_split_kernel(const __grid_constant__
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 u = p.split[blockIdx.x];
-    if (u.w >= 0) {
+    if (u.w >= 0 && u.x >= 0 && u.y >= 0 && u.x + u.y <= p.n_tokens && u.y <= 2 * (kTile / p.group) && u.z >= 0 &&
+        u.z < p.n_kv) {
         const int rows = u.y * p.group;
         for (int r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
             Join j;
@@ -1396,7 +1573,7 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
         p.window = static_cast<int>(a.window);
     }
     p.slopes = a.alibi_slopes;
-    p.scale = a.softmax_scale;
+    p.kf = a.softcap > 0.f ? a.softmax_scale / a.softcap : a.softmax_scale * kLog2e;
     p.cap = a.softcap;
     p.n_tokens = static_cast<int>(a.n_tokens);
     p.n_heads = static_cast<int>(a.n_heads);
@@ -1405,6 +1582,7 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.num_blocks = static_cast<int>(a.num_blocks);
     p.block_size = static_cast<int>(a.block_size);
     p.box_rows = std::min(kTile, p.block_size & -p.block_size);  // boxes never cross a page
+    for (p.box_shift = 0; 1 << p.box_shift < p.box_rows; ++p.box_shift) {}
     p.total_rows = static_cast<int>(a.num_blocks * a.n_kv_heads * a.block_size);
     p.k_scale = static_cast<const __half*>(a.k_scale);
     p.v_scale = static_cast<const __half*>(a.v_scale);
@@ -1438,7 +1616,7 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(kHeadDim) * (f16 ? 2 : 1)};
     const cuuint32_t box[2] = {f16 ? 64u : 128u, static_cast<cuuint32_t>(p.box_rows)};
     const CUtensorMapDataType dt = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    if (!encode(&maps.k, dt, 2, a.k, dims, strides, box, f16, err) || !encode(&maps.v, dt, 2, a.v, dims, strides, box, f16, err))
+    if (!encode(&maps.k, dt, 2, a.k, dims, strides, box, true, err) || !encode(&maps.v, dt, 2, a.v, dims, strides, box, true, err))
         return LIK_ERR_CUDA;
     const bool mod = p.cap > 0.f || p.slopes;
     if (f16) return mod ? launch<kF16, true>(maps, p, stream, err) : launch<kF16, false>(maps, p, stream, err);

@@ -4,15 +4,17 @@ against a plain 64-bit implementation.
 
 The bound of a row, with A = sum p |v| / sum p, B = the largest sum |q_i k_i|
 times the softmax scale, n its keys:
-  * the weights are rounded to fp16 once (half a step, 2^-11): 2^-11 A, and
-    below 2^-14 by 2^-25 at most, at a largest weight of 1 or more: n 2^-25 max|v|;
+  * the weights (times V's scale, in an INT8 cache) are rounded to fp16 once (half
+    a step, 2^-11): 2^-11 A, and below 2^-14 by 2^-25 at most, at a largest weight of
+    1 or more: n 2^-25 max|v|;
+  * a part of them comes from a cubic for 2^x that is 7.5e-5 off at most: 8e-5 A in
+    the sum of weights times values, as much in the sum of weights;
   * the result is rounded to fp16: 2^-11 |out|;
   * a score is an fp32 sum of 128 exact products in any order (128 2^-24 B),
     scaled, capped and biased by a few fp32 operations (8 2^-23 |score| and the
     2^-20 the hardware exponentials leave in tanh, times the cap): a score off
-    by d moves weights and their sum by e^d - 1 each;
-  * INT8 rows are read as fp16(code * scale): 2^-11 B more in the score,
-    2^-11 A more in the values.
+    by d moves weights and their sum by e^d - 1 each. INT8 codes are exact in the
+    products, their scales one fp32 operation (among the 8).
 """
 import math
 
@@ -79,7 +81,7 @@ class Pool:
         return dict(k_scale=self.scale["k"], v_scale=self.scale["v"])
 
 
-def reference(q, k, v, seen, dist, kv, cap=0.0, slopes=None):
+def reference(q, k, v, seen, dist, cap=0.0, slopes=None):
     """q [n, H, 128], k and v [Hkv, m, 128], seen [n, m], dist [n, m]: output and bound, 64 bits."""
     n, H, _ = q.shape
     G = H // k.shape[0]
@@ -101,10 +103,7 @@ def reference(q, k, v, seen, dist, kv, cap=0.0, slopes=None):
         near = near + torch.where(e > 1e-9, slopes.double()[:, None, None] * dist.double(), torch.zeros_like(s)).amax(
             -1, keepdim=True)
     d = 128 * 2.0 ** -24 * B + 8 * 2.0 ** -23 * near + cap * 2.0 ** -20
-    if kv != "fp16":
-        d = d + H11 * B
-    rel = H11 * (2 if kv != "fp16" else 1)
-    tol = A * (rel + 2 * torch.expm1(d)) + H11 * out.abs() + kk.shape[1] * 2.0 ** -25 * vv.abs().amax() + 1e-7
+    tol = A * (H11 + 2 * 8e-5 + 2 * torch.expm1(d)) + H11 * out.abs() + kk.shape[1] * 2.0 ** -25 * vv.abs().amax() + 1e-7
     return out.transpose(0, 1), tol.transpose(0, 1)
 
 
@@ -153,7 +152,7 @@ def run_case(L, kv, H, Hkv, nq, ctx, bs, causal=True, cap=0.0, window=0, alibi=F
             assert (got[lo:lo + m] == 0).all()
             continue
         ref, tol = reference(q[lo:lo + m], pool.rows("k", table[b], c), pool.rows("v", table[b], c), seen, (p - j).abs(),
-                             kv, cap, slopes)
+                             cap, slopes)
         check(got[lo:lo + m], ref, tol)
         empty = ~seen.any(-1)
         assert (got[lo:lo + m][empty] == 0).all()
@@ -256,7 +255,7 @@ def test_growing_scores_raise_the_maximum(L, kv):
     got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, torch.tensor([600], dtype=torch.int32, device="cuda"),
                             cu, SCALE, causal=False, **pool.args())
     seen = torch.ones(3, 600, dtype=torch.bool, device="cuda")
-    ref, tol = reference(q, pool.rows("k", table[0], 600), pool.rows("v", table[0], 600), seen, seen.long(), kv)
+    ref, tol = reference(q, pool.rows("k", table[0], 600), pool.rows("v", table[0], 600), seen, seen.long())
     check(got, ref, tol)
 
 
@@ -324,7 +323,7 @@ def test_offsets_past_32_bits(L):
     got = L.paged_attention(q, cache["k"], cache["v"], table, ctx, cu, SCALE)
     k, v = (cache[x][table[0].long()].double().transpose(0, 1).reshape(hk, -1, 128)[:, :120] for x in "kv")
     p, j = torch.arange(117, 120, device="cuda")[:, None], torch.arange(120, device="cuda")[None]
-    check(got, *reference(q, k, v, j <= p, p - j, "fp16"))
+    check(got, *reference(q, k, v, j <= p, p - j))
 
 
 @pytest.mark.parametrize("kv", KV)
@@ -345,9 +344,9 @@ def test_bad_table_entries_are_reported_and_read_as_zeros(L, kv):
         seen = torch.ones(1, 200, dtype=torch.bool, device="cuda")
         k, v = pool.rows("k", table[0], 200), pool.rows("v", table[0], 200)
         k[:, 80:96], v[:, 80:96] = 0, 0
-        check(got[:1], *reference(q[:1], k, v, seen, seen.long(), kv))
+        check(got[:1], *reference(q[:1], k, v, seen, seen.long()))
         check(got[1:], *reference(q[1:], pool.rows("k", table[1], 150), pool.rows("v", table[1], 150), seen[:, :150],
-                                  seen[:, :150].long(), kv))
+                                  seen[:, :150].long()))
 
 
 def test_offsets_that_do_not_ascend_stay_in_bounds(L):
@@ -387,7 +386,7 @@ def shared_case(L, kv, H, Hkv, sizes, prefix, own, bs, cap=0.0, alibi=False, spr
             continue
         seen = torch.ones(1, m, dtype=torch.bool, device="cuda")
         dist = (m - 1 - torch.arange(m, device="cuda"))[None]
-        check(got[b:b + 1], *reference(q[b:b + 1], rows["k"], rows["v"], seen, dist, kv, cap, slopes))
+        check(got[b:b + 1], *reference(q[b:b + 1], rows["k"], rows["v"], seen, dist, cap, slopes))
 
 
 @pytest.mark.parametrize("kv", KV)
@@ -472,7 +471,7 @@ def test_append_prompt_and_decode_together(L):
             assert torch.equal(v, torch.cat(values[i]))
             p, j = torch.arange(done[i] - c[i], done[i], device="cuda")[:, None], at[None]
             check(got[lo:hi], *reference(q[lo:hi], k.double().transpose(0, 1), v.double().transpose(0, 1), j <= p,
-                                         p - j, "fp16"))
+                                         p - j))
     assert done == lens
     # the decode operator that was there reads the same cache
     dec = L.paged_decode_attention(q, cache["k"], cache["v"], pages, ctx, SCALE, max(lens))
