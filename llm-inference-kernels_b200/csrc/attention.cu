@@ -20,15 +20,16 @@
 // run under the other's exponentials:
 //   wide units (more than 128 rows): stream s holds rows [s], both read every
 //     key tile;
-//   narrow units: both streams hold the same rows and take alternate key
-//     tiles. Units of at most 64 (32) rows are repeated 2 (4) times along the
-//     128 rows of the matrix instruction, and each copy takes the softmax of
-//     its own 64 (32) columns of a tile; a single token's softmax then occupies
-//     all eight warps instead of one. The copies' states are joined at the
-//     unit's end.
-// Tensor memory: S0 | S1 | O0 | O1, 128 columns each; the fp16 weights P
-// overwrite the scores they come from. P V reads P from tensor memory and V as
-// stored ([position, channel], the transposed-operand form).
+//   paired units (up to 128 rows): both streams hold the same rows and take
+//     alternate key tiles, their states are joined at the unit's end;
+//   thin units (up to 32 rows, single tokens among them): paired, and with the
+//     operands exchanged, scores [position][row] = K q^T and sums
+//     [channel][row] = V^T w^T, so that few rows mean a small matrix product
+//     instead of a padded one and a tile's softmax is one position per thread.
+// Tensor memory: S0 | S1 | O0 | O1, 128 columns each. The fp16 weights overwrite
+// the scores they come from and P V reads them there, with V as stored
+// ([position, channel], the transposed-operand form); thin units keep them in
+// shared memory.
 //
 // fp16 caches go from the pool to swizzled shared memory by tensor-map copies,
 // one box per run of positions inside a page. INT8 caches arrive as codes and
@@ -58,13 +59,31 @@ constexpr int kRaw = 4;                          // INT8 tiles in flight
 constexpr int kRawBytes = kTile * kHeadDim;      // codes; their scales: 256 bytes
 constexpr int kScales = 4;                       // INT8: tiles whose scales are kept
 constexpr int kSegs = 4;
+constexpr int kThinRows = 16;
+constexpr uint32_t kTmem = 0;                    // first column of tensor memory
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum is raised only past this many powers of two, so most
 // tiles leave the accumulator alone; weights stay below 2^8 in fp16.
 constexpr float kRaise = 8.0f;
 constexpr uint32_t kPolls = 1u << 18;            // a poll sleeps for a few microseconds at most
 
+enum Mode : int { kWide = 0, kPaired = 1, kThin = 2 };
 enum Dest : int { kDirect = 0, kSlot = 1, kRowBuf = 2 };
+
+// Division of 0 <= x < 2^31 by a launch constant (the round-up method of
+// Granlund and Montgomery): a multiplication instead of some thirty
+// instructions, at places where the code's size counts.
+struct Div {
+    uint32_t d, m, s;
+    __device__ __forceinline__ int operator()(int x) const {
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(x), m) + static_cast<uint32_t>(x)) >> s);
+    }
+};
+Div make_div(uint32_t d) {
+    uint32_t s = 0;
+    while ((uint64_t{1} << s) < d) ++s;
+    return {d, static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << s) - d)) / d + 1), s};
+}
 
 struct KeySet {
     const int* cu;      // [n_seq + 1] token offsets; null: token i is sequence i
@@ -83,6 +102,8 @@ struct Params {
     int window;
     float kf, cap;  // scores times kf: powers of two, or tanh's argument where they are capped
     int n_tokens, n_heads, n_kv, group;
+    int per, thin_per;  // tokens of 128 rows (a paired unit, half a wide one) and of a thin unit
+    Div by_group, by_unit, by_block;
     int num_blocks, block_size, box_rows, box_shift, total_rows;
     const __half* k_scale;
     const __half* v_scale;
@@ -99,13 +120,13 @@ struct Params {
 };
 
 struct Maps {
-    CUtensorMap q[3];  // boxes of 128, 64 and 32 rows' whole tokens
+    CUtensorMap q[2];  // boxes of the whole tokens of 128 and of 16 rows
     CUtensorMap k, v;
 };
 
 struct Segment {
     int valid, set, seq, head;
-    int tok0, ntok, rep;        // rep 0: wide
+    int tok0, ntok, mode;
     int ctx, pos0, pfx, fk;     // fk: smallest first key
     int a0, na, b0, nt;         // key tiles: na from a0, the rest from b0
     int vlo, vhi;               // positions any row sees: [fk, pfx) and [vlo, vhi]
@@ -122,12 +143,13 @@ struct TileList {
 
 struct Misc {
     uint64_t full[2][kRing16], empty[2][kRing16], rfull[kRaw], rempty[kRaw], vscale[kScales];
-    uint64_t qfull, qempty, sfull[2], pready[2][2], odone[2][2], segfull[kSegs], segempty[kSegs], xbar, drain;
-    Segment seg[kSegs];
+    uint64_t qfull, qempty, sfull[2], pready[2][2], odone[2][2], tbar[2], segfull[kSegs], segempty[kSegs], xbar, drain;
+    Segment seg[kSegs], first;
     long long scan[20];
     long long start, count, total;
     int start_id, start_head, start_off;
     uint32_t bad[kRaw];
+    int low[2][2][4];  // thin units: a warp's reference is too low
     int abort;
     uint32_t tmem;
 };
@@ -137,6 +159,18 @@ struct Scales {  // INT8 caches, see convert_role
     float k[kScales][kTile], v[kScales][kTile];
     int v_exp[kScales];
 };
+
+// Thin units, in the second query tile's place.
+struct ThinRow {
+    int lo, hi, fk;
+    float pos, slope;
+};
+struct ThinSpace {
+    unsigned char w[2][kThinRows * 256];  // per stream: weights [2][row][64 positions], swizzled
+    float top[2][4][kThinRows], sum[2][4][kThinRows], ref[2][kThinRows], down[2][kThinRows];
+    ThinRow row[kThinRows];
+};
+static_assert(sizeof(ThinSpace) <= kTileBytes, "thin space");
 
 template <int FMT>
 struct Layout {
@@ -155,8 +189,8 @@ struct Layout {
     // registers per thread: launched with `base`, then moved between the
     // warpgroups; the shares add up to threads * base
     static constexpr int base = FMT == kF16 ? 168 : 96;
-    static constexpr int softmax_regs = FMT == kF16 ? 208 : 136;
-    static constexpr int other_regs = FMT == kF16 ? 88 : 80;
+    static constexpr int softmax_regs = FMT == kF16 ? 192 : 136;
+    static constexpr int other_regs = FMT == kF16 ? 120 : 80;
     static constexpr int convert_regs = 64;
     static_assert(2 * softmax_regs + other_regs + (FMT == kF16 ? 0 : 2 * convert_regs) <= threads / 128 * base,
                   "register shares exceed what the block is launched with");
@@ -173,23 +207,15 @@ __device__ __forceinline__ void regs_dec() {
 
 // ---- bounded waits -----------------------------------------------------------
 
-__device__ __forceinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* abort_flag) {
-#pragma unroll 1
-    for (uint32_t i = 0; i < kPolls; ++i) {
-        if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
-        if (*reinterpret_cast<volatile int*>(abort_flag)) break;
-    }
-    if ((threadIdx.x & 31) == 0) {
-        *reinterpret_cast<volatile int*>(abort_flag) = 1;
-        atomicCAS(&g_attention_error, 0, static_cast<int>(kDevWaitTimeout));
-    }
-    return false;
-}
 // Whole warp; every lane has observed the phase on return. False: give up
-// (this wait or another one of the CTA ran out).
+// (this wait or another one of the CTA ran out; the kernel's end reports it).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Misc* m) {
-    if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
-    return wait_slow(bar, parity, &m->abort);
+#pragma unroll 1
+    for (uint32_t i = 0;; ++i) {
+        if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
+        if (i == kPolls) *reinterpret_cast<volatile int*>(&m->abort) = 1;
+        if (*reinterpret_cast<volatile int*>(&m->abort)) return false;
+    }
 }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     __syncwarp();
@@ -205,12 +231,12 @@ __device__ __forceinline__ int cu_at(const KeySet& k, int b, int n_tokens) {
 
 // The key set and the sequence whose unit numbers include `id`; a sequence
 // whose tokens start at c owns the numbers from c / unit + (its index).
-__device__ __forceinline__ int seq_of(const KeySet& k, int id, int unit, int n_tokens) {
+__device__ __forceinline__ int seq_of(const KeySet& k, int id, Div by_unit, int n_tokens) {
     if (!k.cu) return id;
     int lo = 0, hi = k.n_seq - 1;  // largest b with cu[b] / unit + b <= id
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (cu_at(k, mid, n_tokens) / unit + mid <= id) lo = mid; else hi = mid - 1;
+        if (by_unit(cu_at(k, mid, n_tokens)) + mid <= id) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
@@ -221,19 +247,16 @@ __device__ bool make_unit(const Params& p, int id, Segment& s) {
     const KeySet& k = p.set[s.set];
     if (s.set) id -= p.set[0].n_ids;
     if (k.n_seq <= 0) return false;
-    const int per = kTile / p.group, unit = 2 * per;
-    const int b = seq_of(k, id, unit, p.n_tokens);
+    const int unit = 2 * p.per;
+    const int b = seq_of(k, id, p.by_unit, p.n_tokens);
     const int c0 = cu_at(k, b, p.n_tokens);
     const int n = k.cu ? cu_at(k, b + 1, p.n_tokens) - c0 : 1;
-    const int at = k.cu ? (id - (c0 / unit + b)) * unit : 0;
+    const int at = k.cu ? (id - (p.by_unit(c0) + b)) * unit : 0;
     if (at < 0 || at >= n) return false;
     s.seq = b;
     s.tok0 = c0 + at;
     s.ntok = min(unit, n - at);
-    s.rep = s.ntok * p.group <= 32 / p.group * p.group   ? 4
-            : s.ntok * p.group <= 64 / p.group * p.group ? 2
-            : s.ntok <= per                              ? 1
-                                                         : 0;
+    s.mode = s.ntok <= p.thin_per ? kThin : s.ntok <= p.per ? kPaired : kWide;
     s.ctx = static_cast<int>(min(static_cast<long long>(max(k.ctx[b], 0)),
                                  static_cast<long long>(k.width) * p.block_size));
     s.pos0 = s.ctx - n + at;
@@ -495,51 +518,42 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
     }
 }
 
-// All of a stream's tiles of a segment. NC: the columns of a tile this copy of
-// the rows works on; 128 go in two steps, the first one's weights being
-// multiplied with V while the second is worked out. A tile's scores are there
-// only after the products of the tile before, so the sums can be scaled at once
-// in a tile's first step and after the first half's product in its second.
-// `tiles` and `halves` count the tiles, and those in two steps, so far.
-// `before`: tiles of earlier segments.
-template <int NC, bool I8, bool MOD>
+// All of a stream's tiles of a wide or paired segment, each in two steps of 64
+// columns, the first one's weights being multiplied with V while the second is
+// worked out. A tile's scores are there only after the products of the tile
+// before, so the sums can be scaled at once in a tile's first step and after the
+// first half's product in its second. `tiles` and `halves` count the tiles so
+// far (of all segments, of these ones), `before` those of earlier segments.
+template <bool I8, bool MOD>
 __device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Scales* scales, const Segment& g,
                                             const Row& row, int stream, uint32_t before, uint32_t s_addr,
-                                            uint32_t o_addr, uint32_t& tiles, uint32_t& halves, float& m,
-                                            float& l, int& ev) {
-    constexpr int W = NC == 128 ? 64 : NC;
-    const int warp = (threadIdx.x >> 5) & 3;
-    const int c0 = NC == 128 ? 0 : NC == 64 ? (warp >> 1) * 64 : warp * 32;
-    const int step = g.rep ? 2 : 1;
-    const int t0 = g.t0, t1 = g.t1, i0 = t0 + (g.rep ? stream : 0);
+                                            uint32_t o_addr, uint32_t& tiles, uint32_t& halves, float& m, float& l,
+                                            int& ev) {
+    constexpr int W = 64;
+    const int step = g.mode == kWide ? 1 : 2;
+    const int t0 = g.t0, t1 = g.t1, i0 = t0 + (g.mode == kWide ? 0 : stream);
     const TileList tile(g);
 #pragma unroll 1
     for (int i = i0; i < t1; i += step) {
         if (!warp_wait(&mi->sfull[stream], tiles & 1, mi)) return false;
         ++tiles;
         tcgen05_fence_after();
-        const int j0 = tile(i) * kTile + c0;
+        const int j0 = tile(i) * kTile;
         const uint32_t at = before + i - t0, st = at % kScales;
         if (I8 && !warp_wait(&mi->vscale[st], (at / kScales) & 1, mi)) return false;
         const int v_exp = I8 ? scales->v_exp[st] : 0;
 #pragma unroll 1
-        for (int c = 0; c < NC; c += W) {
-            if (!softmax_step<W, I8, MOD>(p, mi, row, s_addr + c0 + c, s_addr + (c0 + c) / 2, o_addr, j0 + c,
-                                          i > i0 || c > 0, c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1,
-                                          reinterpret_cast<const float4*>(scales->k[st] + c0 + c),
-                                          reinterpret_cast<const float4*>(scales->v[st] + c0 + c), v_exp, m, l, ev))
+        for (int c = 0; c < kTile; c += W) {
+            if (!softmax_step<W, I8, MOD>(p, mi, row, s_addr + c, s_addr + c / 2, o_addr, j0 + c, i > i0 || c > 0,
+                                          c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1,
+                                          reinterpret_cast<const float4*>(scales->k[st] + c),
+                                          reinterpret_cast<const float4*>(scales->v[st] + c), v_exp, m, l, ev))
                 return false;
-            if (NC < kTile) {  // the other copies' columns weigh nothing in this one
-                const uint32_t z[16] = {};
-#pragma unroll
-                for (int k = 0; k < kTile; k += 32)
-                    if (k < c0 || k >= c0 + NC) tmem_st16(s_addr + k / 2, z);
-            }
             tmem_wait_st();
             tcgen05_fence_before();
-            warp_arrive(&mi->pready[stream][NC < kTile || c > 0]);
+            warp_arrive(&mi->pready[stream][c > 0]);
         }
-        if (NC == kTile) ++halves;
+        ++halves;
     }
     return true;
 }
@@ -610,30 +624,257 @@ __device__ __forceinline__ void store_wide(unsigned char* stage, unsigned char* 
     }
 }
 
+// Barrier of a stream's four softmax warps.
+__device__ __forceinline__ bool stream_sync(Misc* mi, int stream, uint32_t& phase) {
+    warp_arrive(&mi->tbar[stream]);
+    return warp_wait(&mi->tbar[stream], phase++ & 1, mi);
+}
+
+// A thin segment. Scores come transposed, [position][row], so a thread holds one
+// position's scores of all rows; a row's reference is the same in all 128
+// threads of the stream, and each keeps its own part of the sum of weights. A
+// vote per tile finds out whether any reference has to be raised. What is
+// needed for few tiles (masks, the raising) or rows goes four rows at a time
+// through tensor memory, in loops: unrolled it made the kernel twice as large
+// and slower than its instruction fetches.
+template <int FMT, bool MOD>
+__device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, const Segment& g, int stream, uint32_t before,
+                             uint32_t s_addr, uint32_t o_addr, uint32_t& tiles, uint32_t& tphase, uint32_t& votes,
+                             uint32_t& xphase) {
+    constexpr bool I8 = FMT != kF16;
+    constexpr int NT = kThinRows;
+    const int r_in = threadIdx.x & 127, lane = threadIdx.x & 31, warp = r_in >> 5;
+    ThinSpace* const sp = reinterpret_cast<ThinSpace*>(smem + kTileBytes);
+    const Scales* scales = reinterpret_cast<const Scales*>(smem + Layout<FMT>::scales);
+    const KeySet& ks = p.set[g.set];
+    const int rows = g.ntok * p.group, pfx = g.pfx;
+    if (r_in < NT) {  // both streams write the same
+        const int tl = p.by_group(r_in), tok = g.tok0 + tl;
+        ThinRow q = {0, -1, 0, 0.f, 0.f};
+        if (r_in < rows) {
+            const int pos = ks.extra ? max(ks.extra[tok], 0) + g.ctx - 1 : g.pos0 + tl;
+            q.fk = p.first_keys ? max(p.first_keys[tok], 0) : 0;
+            q.lo = max(p.window > 0 ? max(pos - p.window + 1, 0) : 0, q.fk);
+            q.hi = ks.causal ? min(pos, g.ctx - 1) : g.ctx - 1;
+            q.pos = static_cast<float>(pos);
+            if (MOD && p.slopes) q.slope = p.slopes[g.head * p.group + r_in - tl * p.group] * kLog2e;
+        }
+        sp->row[r_in] = q;
+        sp->ref[stream][r_in] = -INFINITY;
+    }
+    if (!stream_sync(mi, stream, tphase)) return false;
+    int lo_max = 0, hi_min = 0x7fffffff, fk_max = 0;
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+        lo_max = max(lo_max, sp->row[r].lo);
+        hi_min = min(hi_min, sp->row[r].hi);
+        fk_max = max(fk_max, sp->row[r].fk);
+    }
+    float* const ref = sp->ref[stream];
+    float l[NT];
+#pragma unroll
+    for (int r = 0; r < NT; ++r) l[r] = 0.f;
+    int ev = -200;
+    const int t0 = g.t0, t1 = g.t1;
+    const TileList tile(g);
+    unsigned char* const w_at = sp->w[stream] + (r_in >> 6) * (kThinRows * 128) + (r_in & 7) * 2;
+    const int chunk = (r_in & 63) >> 3;
+    bool any = false;
+#pragma unroll 1
+    for (int i = t0 + stream; i < t1; i += 2, any = true) {
+        const int j0 = tile(i) * kTile, j = j0 + r_in;
+        if (!warp_wait(&mi->sfull[stream], tiles & 1, mi)) return false;
+        ++tiles;
+        tcgen05_fence_after();
+        const uint32_t at = before + i - t0, st = at % kScales;
+        if (I8 && !warp_wait(&mi->vscale[st], (at / kScales) & 1, mi)) return false;
+        const int v_exp = I8 ? scales->v_exp[st] : 0;
+        const float vx = I8 ? scales->v[st][r_in] : 1.f;
+        float kx = I8 ? scales->k[st][r_in] : p.kf;
+        const bool whole = (j0 >= lo_max && j0 + kTile - 1 <= hi_min) || (j0 >= fk_max && j0 + kTile <= pfx);
+        if (MOD || !whole) {  // scores in powers of two, -inf where hidden, written back
+#pragma unroll 1
+            for (int r0 = 0; r0 < rows; r0 += 4) {
+                float x[4];
+                tmem_ld4(s_addr + r0, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const ThinRow& q = sp->row[r0 + c];
+                    x[c] *= kx;
+                    if (MOD && p.cap > 0.f) x[c] = p.cap * kLog2e * tanh_exp(x[c]);
+                    if (MOD && p.slopes) x[c] = fmaf(-q.slope, fabsf(static_cast<float>(j) - q.pos), x[c]);
+                    if (!((j >= q.lo && j <= q.hi) || (j >= q.fk && j < pfx))) x[c] = -INFINITY;
+                }
+                tmem_st4(s_addr + r0, x);
+            }
+            tmem_wait_st();
+            kx = 1.f;
+        }
+#pragma unroll 1
+        for (int pass = 0;; ++pass) {
+            float x[NT];
+            tmem_ld16(s_addr, x);
+            tmem_wait_ld();
+            bool low = I8 && v_exp > ev;
+#pragma unroll
+            for (int r = 0; r < NT; ++r) {
+                if (r < rows) {
+                    const float m = ref[r];
+                    x[r] *= kx;
+                    low = low || x[r] - m > kRaise;
+                    x[r] = fast_exp2(x[r] - (m == -INFINITY ? 0.f : m));
+                    *reinterpret_cast<__half*>(w_at + r * 128 + ((chunk ^ (r & 7)) << 4)) = __float2half_rn(x[r] * vx);
+                }
+            }
+            low = __any_sync(kFull, low);
+            int* const flag = mi->low[stream][votes++ & 1];
+            if (lane == 0) *reinterpret_cast<volatile int*>(flag + warp) = low;
+            fence_async_smem();  // the weights, for the matrix instructions
+            if (!stream_sync(mi, stream, tphase)) return false;
+            const volatile int* f = flag;
+            if (pass > 0 || !(f[0] | f[1] | f[2] | f[3])) {
+#pragma unroll
+                for (int r = 0; r < NT; ++r) l[r] += r < rows ? x[r] : 0.f;
+                break;
+            }
+            // raise the references to the tile's maxima
+#pragma unroll 1
+            for (int r0 = 0; r0 < rows; r0 += 4) {
+                tmem_ld4(s_addr + r0, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float t = x[c] * kx;
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, d));
+                    if (lane == 0) sp->top[stream][warp][r0 + c] = t;
+                }
+            }
+            if (!stream_sync(mi, stream, tphase)) return false;
+            if (r_in < rows) {
+                const float old = ref[r_in];
+                const float up = fmaxf(max3(old, sp->top[stream][0][r_in], sp->top[stream][1][r_in]),
+                                       fmaxf(sp->top[stream][2][r_in], sp->top[stream][3][r_in]));
+                sp->down[stream][r_in] = old == -INFINITY ? 0.f : fast_exp2(old - up);
+                ref[r_in] = up;
+            }
+            if (!stream_sync(mi, stream, tphase)) return false;
+#pragma unroll
+            for (int r = 0; r < NT; ++r)
+                if (r < rows) l[r] *= sp->down[stream][r];
+            float fo = 1.f;
+            if (I8) {
+                fo = fast_exp2(static_cast<float>(ev - v_exp));
+                ev = v_exp;
+            }
+            if (any) {  // this stream's products so far are done: the scores came after them
+#pragma unroll 1
+                for (int r0 = 0; r0 < rows; r0 += 4) {
+                    tmem_ld4(o_addr + r0, x);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) x[c] *= r0 + c < rows ? sp->down[stream][r0 + c] * fo : 0.f;
+                    tmem_st4(o_addr + r0, x);
+                }
+                tmem_wait_st();
+            }
+        }
+        tcgen05_fence_before();
+        warp_arrive(&mi->pready[stream][1]);
+    }
+    if (any) {
+        if (!warp_wait(&mi->odone[stream][1], (tiles - 1) & 1, mi)) return false;
+        tcgen05_fence_after();
+    }
+    // join the two streams; a thread holds one channel of all rows now
+    const float unit_v = I8 && any ? fast_exp2(static_cast<float>(ev)) : 1.f;
+#pragma unroll
+    for (int r = 0; r < NT; ++r) {
+        if (r < rows) {
+            float t = l[r];
+#pragma unroll
+            for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(kFull, t, d);
+            if (lane == 0) sp->sum[stream][warp][r] = t;
+        }
+    }
+    if (!softmax_sync(mi, xphase)) return false;
+    float* const other = reinterpret_cast<float*>(smem + Layout<FMT>::stage);  // [row][channel]
+#pragma unroll 1
+    for (int turn = 1; turn >= 0; --turn) {  // stream 1 hands over, stream 0 adds and stores
+#pragma unroll 1
+        for (int r0 = 0; stream == turn && r0 < rows; r0 += 4) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (any) {
+                tmem_ld4(o_addr + r0, x);
+                tmem_wait_ld();
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = r0 + c;
+                if (r >= rows) break;
+                const float m0 = sp->ref[0][r], m1 = sp->ref[1][r], top = fmaxf(m0, m1);
+                const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
+                const float f = (stream ? a1 : a0) * unit_v;
+                const float v = f > 0.f ? x[c] * f : 0.f;
+                if (turn) {
+                    other[r * kHeadDim + r_in] = v;
+                    continue;
+                }
+                const float* s0 = sp->sum[0][0] + r;
+                const float* s1 = sp->sum[1][0] + r;
+                const float sum = a0 * ((s0[0] + s0[NT]) + (s0[2 * NT] + s0[3 * NT])) +
+                                  a1 * ((s1[0] + s1[NT]) + (s1[2 * NT] + s1[3 * NT]));
+                const float all = v + other[r * kHeadDim + r_in];
+                const int tl = p.by_group(r);
+                const uint32_t to = dest_row(p, g, g.tok0 + tl, g.head * p.group + r - tl * p.group, r);
+                if (r_in == 0) store_ml(p, g, to, top, sum);
+                const size_t e = static_cast<size_t>(to) * kHeadDim + r_in;
+                if (g.dest == kDirect)
+                    p.out[e] = __float2half_rn(sum > 0.f ? all / sum : 0.f);
+                else
+                    (g.dest == kSlot ? p.part : p.rowbuf)[e] = all;
+            }
+        }
+        if (turn == 0) fence_async_smem();  // queries may be copied over the space that was used here
+        if (!softmax_sync(mi, xphase)) return false;
+    }
+    tcgen05_fence_before();
+    return true;
+}
+
 // Results leave through shared memory, so that a warp writes whole runs of a
 // row instead of 16 bytes of 32 rows (a quarter of the time for a wide unit).
 template <int FMT, bool MOD>
-__device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uint32_t tmem) {
+__device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
     const int stream = threadIdx.x >> 7, r_in = threadIdx.x & 127;
     const uint32_t lane_base = static_cast<uint32_t>(r_in & 96) << 16;
-    const uint32_t s_addr = tmem + lane_base + stream * 128, o_addr = s_addr + 256;
-    const int per = kTile / p.group;
+    const uint32_t s_addr = kTmem + lane_base + stream * 128, o_addr = s_addr + 256;
     unsigned char* const stage = smem + Layout<FMT>::stage;
     const Scales* scales = reinterpret_cast<const Scales*>(smem + Layout<FMT>::scales);
     constexpr bool I8 = FMT != kF16;
-    uint32_t tiles = 0, halves = 0, before = 0, xphase = 0;
+    uint32_t tiles = 0, halves = 0, before = 0, xphase = 0, tphase = 0, votes = 0;
     bool wide_before = false;
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
+        if (g.mode == kThin) {
+            const uint32_t b = before;
+            before += g.t1 - g.t0;
+            const bool ok =
+                thin_segment<FMT, MOD>(p, mi, smem, g, stream, b, s_addr, o_addr, tiles, tphase, votes, xphase);
+            if (!ok) return;
+            wide_before = false;
+            warp_arrive(&mi->segempty[slot]);
+            continue;
+        }
         const KeySet& ks = p.set[g.set];
-        const int block = g.rep ? kTile / g.rep : kTile;  // rows of one copy
-        const int rr = r_in & (block - 1);
-        const int tl0 = rr / p.group, hr = g.head * p.group + rr - tl0 * p.group;
-        const int tl = tl0 + (g.rep ? 0 : stream * per);
-        const bool live = tl < g.ntok && rr < block / p.group * p.group;
+        const bool wide = g.mode == kWide;
+        const int tl0 = p.by_group(r_in), hr = g.head * p.group + r_in - tl0 * p.group;
+        const int tl = tl0 + (wide ? stream * p.per : 0);
+        const bool live = tl < g.ntok && tl0 < p.per;
         const int tok = g.tok0 + tl;
         Row row{0, 0x7fffffff, 0, 0, 0.f, 0.f};  // a row that is not live keeps every column: nothing reads it
         if (live) {
@@ -647,15 +888,8 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
         }
         float m = -INFINITY, l = 0.f;
         int ev = -200;
-        const int mine = g.rep ? (g.t1 - g.t0 - stream + 1) / 2 : g.t1 - g.t0;  // tiles of this stream
-        bool ok;
-        if (g.rep == 4)
-            ok = softmax_run<32, I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev);
-        else if (g.rep == 2)
-            ok = softmax_run<64, I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev);
-        else
-            ok = softmax_run<128, I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev);
-        if (!ok) return;
+        const int mine = wide ? g.t1 - g.t0 : (g.t1 - g.t0 - stream + 1) / 2;  // tiles of this stream
+        if (!softmax_run<I8, MOD>(p, mi, scales, g, row, stream, before, s_addr, o_addr, tiles, halves, m, l, ev)) return;
         before += g.t1 - g.t0;
         const float unit_v = I8 && mine > 0 ? fast_exp2(static_cast<float>(ev)) : 1.f;
         if (mine > 0) {
@@ -664,7 +898,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
         }
         if (m == -INFINITY) l = 0.f;
         const float m2 = l > 0.f ? m : -INFINITY;
-        if (g.rep == 0) {
+        if (wide) {
             const uint32_t row_at = live ? dest_row(p, g, tok, hr, tl * p.group + hr - g.head * p.group) : ~0u;
             if (live) store_ml(p, g, row_at, m2, l);
             if (g.dest == kDirect)
@@ -674,23 +908,25 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
                 store_wide<FMT, false>(stage, reinterpret_cast<unsigned char*>(g.dest == kSlot ? p.part : p.rowbuf),
                                        o_addr, mine > 0, row_at, unit_v);
         } else {
-            // join the copies and streams: each scales its sums to the row's
-            // common maximum, then 256 threads add the states in order
+            // join the streams: each scales its sums to the row's common
+            // reference, then 256 threads add the two in order
             if (wide_before && !softmax_sync(mi, xphase)) return;  // the staging space was the warps' own
             float2* ml = reinterpret_cast<float2*>(stage);
             float4* data = reinterpret_cast<float4*>(stage + 2048);
-            const int states = 2 * g.rep, rows = g.ntok * p.group;
-            const int state = stream * g.rep + r_in / block;
+            constexpr int states = 2, block = kTile;
+            const int rows = g.ntok * p.group, rr = r_in, state = stream;
             ml[threadIdx.x] = live ? float2{m2, l} : float2{-INFINITY, 0.f};
             if (!softmax_sync(mi, xphase)) return;
             float top = -INFINITY;
-            for (int t = 0; t < states; ++t) top = fmaxf(top, ml[t * block + rr].x);
+            top = fmaxf(ml[rr].x, ml[block + rr].x);
             const float f = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top) * unit_v;
             int dc = 128;  // channels per pass: what fits the scratch space (states * rows <= 256)
             while (states * rows * dc * 4 > Layout<FMT>::stage_bytes - 2048) dc >>= 1;
             const int quads = dc / 4, spread = min(quads, 8) - 1;
             float4* const mine_at = data + (state * rows + rr) * quads;
+#pragma unroll 1
             for (int d0 = 0; d0 < kHeadDim; d0 += dc) {
+#pragma unroll 1
                 for (int c = 0; c < dc; c += 32) {
                     float o[32];
 #pragma unroll
@@ -713,6 +949,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
                     }
                 }
                 if (!softmax_sync(mi, xphase)) return;
+#pragma unroll 1
                 for (int it = threadIdx.x; it < rows * quads; it += 256) {
                     const int r = it / quads, c4 = it - r * quads;
                     float mx = -INFINITY, sum = 0.f;
@@ -724,7 +961,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
                         const float4 a = data[(t * rows + r) * quads + (c4 ^ (r & spread))];
                         v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
                     }
-                    const int tk = r / p.group;
+                    const int tk = p.by_group(r);
                     const uint32_t at = dest_row(p, g, g.tok0 + tk, g.head * p.group + r - tk * p.group, r);
                     if (d0 == 0 && c4 == 0) store_ml(p, g, at, mx, sum);
                     const size_t e = static_cast<size_t>(at) * kHeadDim + d0 + 4 * c4;
@@ -738,7 +975,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
                 if (!softmax_sync(mi, xphase)) return;
             }
         }
-        wide_before = g.rep == 0;
+        wide_before = wide;
         tcgen05_fence_before();
         warp_arrive(&mi->segempty[slot]);
     }
@@ -747,7 +984,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem, uin
 // ---- matrix instructions -------------------------------------------------------
 
 template <int FMT>
-__device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_t tmem) {
+__device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem) {
     constexpr int ring = Layout<FMT>::ring;
     constexpr uint32_t id_qk = mma_idesc_f16(128, 128, false), id_pv = mma_idesc_f16(128, 128, true);
     const int lane = threadIdx.x & 31;
@@ -758,36 +995,44 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
     const uint32_t leader = elect_one();
     const uint64_t q_desc = smem_desc(q_addr, 16, 1024), k_desc = smem_desc(k_addr, 16, 1024),
                    v_desc = smem_desc(v_addr, kHalfTile, 1024);
-    auto qk = [&](int stream, int qslot, uint32_t e) {
+    // scores [row][position] = q K^T; thin units: [position][row] = K q^T
+    auto scores = [&](int stream, int qslot, uint32_t e, bool thin, uint32_t idesc) {
         tcgen05_fence_after();
-        const uint64_t a = q_desc + qslot * (kTileBytes >> 4), b = k_desc + (e % ring) * (kTileBytes >> 4);
+        const uint64_t q = q_desc + qslot * (kTileBytes >> 4), k = k_desc + (e % ring) * (kTileBytes >> 4);
+        const uint64_t a = thin ? k : q, b = thin ? q : k;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t off = ((i >> 2) * kHalfTile + (i & 3) * 32) >> 4;
-            mma_f16_ss(tmem + stream * 128, a + off, b + off, id_qk, i > 0, leader);
+            mma_f16_ss(kTmem + stream * 128, a + off, b + off, idesc, i > 0, leader);
         }
         mma_commit(&mi->sfull[stream], leader);
     };
-    // the next weights of this stream times V: half a tile's where 128 columns
-    // are worked out in two steps, else the tile's
-    auto pv = [&](int stream, uint32_t e, bool first, bool halves) {
+    // the next weights of this stream times V, half a tile's at a time
+    auto pv = [&](int stream, uint32_t e, bool first) {
         const uint64_t b = v_desc + (e % ring) * (kTileBytes >> 4);
-        const uint32_t o = tmem + 256 + stream * 128, w = tmem + stream * 128;
-        if (halves) {
-            if (!warp_wait(&mi->pready[stream][0], ph[stream][0]++ & 1, mi)) return false;
+        const uint32_t o = kTmem + 256 + stream * 128, w = kTmem + stream * 128;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+            if (!warp_wait(&mi->pready[stream][h], ph[stream][h]++ & 1, mi)) return false;
             tcgen05_fence_after();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_f16_ts(o, w + i * 8, b + i * (2048 >> 4), id_pv, !first || i > 0, leader);
-            mma_commit(&mi->odone[stream][0], leader);
+            for (int i = 0; i < 4; ++i)
+                mma_f16_ts(o, w + (4 * h + i) * 8, b + (4 * h + i) * (2048 >> 4), id_pv, !first || h > 0 || i > 0, leader);
+            mma_commit(&mi->odone[stream][h], leader);
         }
+        return true;
+    };
+    // thin units: sums [channel][row] += V^T w^T
+    const uint64_t w_desc = smem_desc(q_addr + kTileBytes, 16, 1024);
+    auto pv_thin = [&](int stream, uint32_t e, bool first, uint32_t idesc) {
+        const uint64_t a = v_desc + (e % ring) * (kTileBytes >> 4), b = w_desc + stream * (kThinRows * 256 >> 4);
         if (!warp_wait(&mi->pready[stream][1], ph[stream][1]++ & 1, mi)) return false;
         tcgen05_fence_after();
-        if (!halves) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma_f16_ts(o, w + i * 8, b + i * (2048 >> 4), id_pv, !first || i > 0, leader);
-        }
-#pragma unroll
-        for (int i = 4; i < 8; ++i) mma_f16_ts(o, w + i * 8, b + i * (2048 >> 4), id_pv, 1, leader);
+        for (int i = 0; i < 8; ++i)
+            mma_f16_ss(kTmem + 256 + stream * 128, a + i * (2048 >> 4),
+                       b + (((i >> 2) * (kThinRows * 128) + (i & 3) * 32) >> 4),
+                       idesc, !first || i > 0, leader);
         mma_commit(&mi->odone[stream][1], leader);
         return true;
     };
@@ -815,54 +1060,37 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
-        const int t0 = g.t0, n = __shfl_sync(kFull, g.t1 - t0, 0);  // known to be uniform
+        // loads that the compiler then knows to be uniform
+        const int t0 = __shfl_sync(kFull, g.t0, 0), n = __shfl_sync(kFull, g.t1, 0) - t0;
         const TileList tile(g);
         const int4 seen = {g.vlo, g.vhi, g.fk, g.pfx};
         if (n > 0) {
             if (!warp_wait(&mi->qfull, qk_seg++ & 1, mi)) return;
-            const int rep = __shfl_sync(kFull, g.rep, 0);
-            if (rep == 0) {
-                if (!wait_tile(0, n_k)) return;
-                qk(0, 0, n_k);
-                qk(1, 1, n_k);
-                release(0, n_k++);
-                if (n == 1) mma_commit(&mi->qempty, leader);
-                for (int i = 0; i < n; ++i) {
-                    const bool more = i + 1 < n;
+            // K of tile i + L and V of tile i, in the order they are copied
+            const int mode = __shfl_sync(kFull, g.mode, 0), L = mode == kWide ? 1 : 2;
+            const bool thin = mode == kThin;
+            const uint32_t id_s = thin ? mma_idesc_f16(128, kThinRows, false) : id_qk;
+#pragma unroll 1
+            for (int i = -L; i < n; ++i) {
+                const bool more = i + L < n;
+                if (i >= 0) {
                     if (!wait_tile(1, n_v)) return;
                     clean(seen, tile(t0 + i), n_v);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        if (!pv(s, n_v, i == 0, true)) return;
-                        if (more) {
-                            if (s == 0 && !wait_tile(0, n_k)) return;
-                            qk(s, s, n_k);
-                        }
-                    }
-                    release(1, n_v++);
-                    if (more) release(0, n_k++);
-                    if (i + 2 == n) mma_commit(&mi->qempty, leader);
                 }
-            } else {
-                for (int s = 0; s < min(n, 2); ++s) {
-                    if (!wait_tile(0, n_k)) return;
-                    qk(s, 0, n_k);
-                    release(0, n_k++);
-                }
-                if (n <= 2) mma_commit(&mi->qempty, leader);
-                for (int i = 0; i < n; ++i) {
-                    const int s = i & 1;
-                    if (!wait_tile(1, n_v)) return;
-                    clean(seen, tile(t0 + i), n_v);
-                    if (!pv(s, n_v, i < 2, rep == 1)) return;
-                    release(1, n_v++);
-                    if (i + 2 < n) {
-                        if (!wait_tile(0, n_k)) return;
-                        qk(s, 0, n_k);
-                        release(0, n_k++);
-                        if (i + 3 == n) mma_commit(&mi->qempty, leader);
+#pragma unroll 1
+                for (int turn = 0; turn < 3 - L; ++turn) {
+                    const int s = mode == kWide ? turn : i & 1;
+                    if (i >= 0 && !(thin ? pv_thin(s, n_v, i < L, mma_idesc_f16(128, kThinRows, false) | (1u << 15))
+                                         : pv(s, n_v, i < L)))
+                        return;
+                    if (more) {
+                        if (turn == 0 && !wait_tile(0, n_k)) return;
+                        scores(s, turn, n_k, thin, id_s);
                     }
                 }
+                if (i >= 0) release(1, n_v++);
+                if (more) release(0, n_k++);
+                if (i + L + 1 == n) mma_commit(&mi->qempty, leader);
             }
         }
         warp_arrive(&mi->segempty[slot]);
@@ -871,7 +1099,7 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem, uint32_
 
 // ---- copies --------------------------------------------------------------------
 
-// Order of the copies: K of the first L tiles (wide units 1, narrow units 2),
+// Order of the copies: K of the first L tiles (wide units 1, others 2),
 // then V_i, K_{i + L} for every tile i. K and V have rings of their own, so
 // that each barrier's phases have one waiter that sees every one of them:
 // a parity says nothing to a waiter that may be two phases behind.
@@ -887,6 +1115,7 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
     const int sub = FMT == kF16 ? lane >> 1 & 7 : lane & 7;
     const int part = FMT == kF16 ? lane & 1 : lane >> 3 & 1;  // half of the channels; codes or scales
     uint32_t n_k = 0, n_v = 0, q_seg = 0;                      // tiles and query loads so far
+    uint32_t thin = 0;                                         // 1 + the last thin segment
     auto full_of = [&](bool v, uint32_t e) { return FMT == kF16 ? &mi->full[v][e % ring] : &mi->rfull[e % ring]; };
     auto claim = [&](bool v, uint32_t& e) {  // the next ring entry, once it is free
         e = FMT != kF16 ? n_k + n_v : v ? n_v : n_k;
@@ -899,7 +1128,7 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) break;
         const Segment& g = mi->seg[slot];
         if (!g.valid) break;
-        const int t0 = g.t0, n = g.t1 - t0, rep = g.rep;
+        const int t0 = g.t0, n = g.t1 - t0, mode = g.mode;
         bool ok = true;
         if (n > 0) {
             const TileList tile(g);
@@ -908,12 +1137,13 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
             const int* const table = ks.tables + static_cast<size_t>(g.seq) * ks.width;
             // Pages of 32 boxes (of 32 / subs tiles), one per lane: the page
             // number, -1 if it is none, -2 where nothing is seen.
+            const int sub_shift = 7 - p.box_shift;  // subs = 1 << sub_shift
             auto look = [&](int batch) {
-                const int q = batch * 32 + lane, i = q / subs;
+                const int q = batch * 32 + lane, i = q >> sub_shift;
                 if (i >= n) return -2;
                 const int j = tile(t0 + i) * kTile + ((q & (subs - 1)) << p.box_shift), e = j + p.box_rows - 1;
                 if (!((e >= vlo && j <= vhi) || (e >= fk && j < pfx))) return -2;
-                return max(__ldg(table + j / p.block_size), -1);
+                return max(__ldg(table + p.by_block(j)), -1);
             };
             // its row in the caches; the row past the last reads as zeros
             auto place = [&](int page, int batch) {
@@ -923,31 +1153,35 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
                     return p.total_rows;
                 }
                 const int q = batch * 32 + lane;
-                const int j = tile(t0 + q / subs) * kTile + ((q & (subs - 1)) << p.box_shift);
-                return (page * p.n_kv + head) * p.block_size + j % p.block_size;
+                const int j = tile(t0 + (q >> sub_shift)) * kTile + ((q & (subs - 1)) << p.box_shift);
+                return (page * p.n_kv + head) * p.block_size + j - p.by_block(j) * p.block_size;
             };
-            int batch = 0;
-            const int look0 = look(0), look1 = look(1);
-            int ahead = look(2);
+            int batch = -2, ahead = look(0), rows = 0, rows_next = 0;
             // queries: the last segment's score tiles are done with them
             if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
             ++q_seg;
-            const int copies = rep ? rep : 2, block = rep ? kTile / rep : kTile;
-            const int toks = block / p.group;
-            const CUtensorMap* qm = &maps.q[rep == 4 ? 2 : rep == 2 ? 1 : 0];
+            if (mode == kWide && thin && k - (thin - 1) < kSegs &&
+                !warp_wait(&mi->segempty[(thin - 1) % kSegs], ((thin - 1) / kSegs) & 1, mi))
+                break;  // a thin segment still uses the second tile's place
+            const int copies = mode == kWide ? 2 : 1, toks = mode == kThin ? p.thin_per : p.per;
+            const CUtensorMap* qm = &maps.q[mode == kThin];
             if (lane == 0) mbar_arrive_expect_tx(&mi->qfull, static_cast<uint32_t>(copies * toks * p.group * 256));
             __syncwarp();
             if (lane < 2 * copies) {
                 const int c = lane >> 1, half = lane & 1;
-                unsigned char* dst = smem + (rep ? c * block * 128 : c * kTileBytes) + half * kHalfTile;
-                tma_load_3d(dst, qm, half * 64, head * p.group, tok0 + (rep ? 0 : c * toks), &mi->qfull);
+                tma_load_3d(smem + c * kTileBytes + half * kHalfTile, qm, half * 64, head * p.group, tok0 + c * toks,
+                            &mi->qfull);
             }
-            int rows = place(look0, 0), rows_next = place(look1, 1);
             // V of tile iv and K of tile ik (of the list; < 0: none)
             auto load = [&](int iv, int ik) {
                 uint32_t ev = 0, ek = 0;
-                if (iv >= 0 && !claim(true, ev)) return false;
-                if (ik >= 0 && !claim(false, ek)) return false;
+#pragma unroll 1
+                for (int v = 1; v >= 0; --v) {
+                    uint32_t e;
+                    if ((v ? iv : ik) < 0) continue;
+                    if (!claim(v, e)) return false;
+                    (v ? ev : ek) = e;
+                }
                 const int q = (is_k ? max(ik, 0) : max(iv, 0)) * subs + sub;
                 const int r0 = __shfl_sync(kFull, rows, q & 31), r1 = __shfl_sync(kFull, rows_next, q & 31);
                 const int row = (q >> 5) == batch ? r0 : r1;
@@ -981,10 +1215,11 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
                 __syncwarp();
                 return true;
             };
-            const int L = rep ? 2 : 1;
-            ok = load(-1, 0) && (L == 1 || n == 1 || load(-1, 1));
-            for (int i = 0; ok && i < n; ++i) {
-                if ((i * subs) >> 5 != batch) {
+            const int L = mode == kWide ? 1 : 2;
+#pragma unroll 1
+            for (int i = -L; ok && i < n; ++i) {
+#pragma unroll 1
+                while (max(i, 0) << sub_shift >> 5 > batch) {  // twice at first: this batch and the next
                     ++batch;
                     rows = rows_next;
                     rows_next = place(ahead, batch + 1);
@@ -994,6 +1229,7 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
             }
         }
         if (!ok) break;
+        if (mode == kThin) thin = k + 1;
         warp_arrive(&mi->segempty[slot]);
     }
     // Leave no copy in flight: after an abort nobody else waits for them.
@@ -1022,8 +1258,7 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
 // needs them; they are divided by the power of two above the segment's largest
 // so far, so that weight * scale fits fp16. Rows that no row of the unit sees,
 // and rows of pages that are not there, become zeros with scale zero.
-template <bool V>
-__device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem) {
+__device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, bool is_v) {
     constexpr int ring = Layout<kI8>::ring;
     Scales* const scales = reinterpret_cast<Scales*>(smem + Layout<kI8>::scales);
     const int t = threadIdx.x & 127;
@@ -1035,86 +1270,86 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem) {
     const int r0 = (t >> 5) * 32 + (lane >> 4);
     auto row_of = [&](int i) { return (r0 + (i >> 1) * 8 + (i & 1) * 2) ^ turn; };
     uint32_t pos = 0, done = 0;  // code tiles; of this warpgroup's kind
-    int top = 0;  // V's exponent
-    // `seen(r)`: whether row r counts
-    auto convert_tile = [&](const unsigned char* src, int st, auto seen) {
-        const __half* scale = reinterpret_cast<const __half*>(smem + Layout<kI8>::raw_scale + st * 256);
-        const uint32_t n = done++;
-        const int at = n % kScales, d = n % ring;
-        if (!V) {
-            // never zero: a hidden key's score is -inf times this
-            scales->k[at][t] = seen(t) ? fmaxf(__half2float(scale[t]) * p.kf, 1e-30f) : 1.f;
-        } else {
-            const int r4 = (t & 31) * 4;
-            const uint2 raw = *reinterpret_cast<const uint2*>(scale + r4);
-            const float2 a = __half22float2(as_h2(raw.x)), b = __half22float2(as_h2(raw.y));
-            const float most = fmaxf(fmaxf(seen(r4) ? a.x : 0.f, seen(r4 + 1) ? a.y : 0.f),
-                                     fmaxf(seen(r4 + 2) ? b.x : 0.f, seen(r4 + 3) ? b.y : 0.f));
-            const uint32_t bits = __reduce_max_sync(kFull, __float_as_uint(most));
-            top = max(top, static_cast<int>(bits >> 23) - 126);
-            scales->v[at][t] = seen(t) ? __half2float(scale[t]) * __int_as_float((127 - top) << 23) : 0.f;
-            scales->v_exp[at] = top;
-            warp_arrive(&mi->vscale[at]);
-        }
-        uint4 in[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = row_of(i);
-            in[i] = *reinterpret_cast<const uint4*>(src + r * kHeadDim + ((c ^ (r & 7)) << 4));
-        }
-        warp_arrive(&mi->rempty[st]);
-        if (n >= ring && !warp_wait(&mi->empty[V][d], (n / ring - 1) & 1, mi)) return false;
-        unsigned char* dst = smem + Layout<kI8>::tiles + ((V ? ring : 0) + d) * kTileBytes + (c >> 2) * kHalfTile;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = row_of(i);
-            const uint4 w = seen(r) ? in[i] : uint4{0, 0, 0, 0};
-            half2 o[4];
-            unsigned char* line = dst + r * 128;
-            i8x4_to_h2(w.x, o[0], o[1]);
-            i8x4_to_h2(w.y, o[2], o[3]);
-            *reinterpret_cast<uint4*>(line + ((x ^ (r & 7)) << 4)) =
-                uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
-            i8x4_to_h2(w.z, o[0], o[1]);
-            i8x4_to_h2(w.w, o[2], o[3]);
-            *reinterpret_cast<uint4*>(line + (((x + 1) ^ (r & 7)) << 4)) =
-                uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
-        }
-        fence_async_smem();
-        warp_arrive(&mi->full[V][d]);
-        return true;
-    };
-    auto convert = [&](int4 range, int tile) {
-        const int st = pos % kRaw;
-        const int j0 = tile * kTile;
-        const int lo = range.x - j0, hi = range.y - j0, fk = range.z - j0, pfx = range.w - j0;
-        if (!warp_wait(&mi->rfull[st], (pos / kRaw) & 1, mi)) return false;
-        const unsigned char* src = smem + Layout<kI8>::raw + st * kRawBytes;
-        const uint32_t bad = mi->bad[st];
-        const bool all = ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) && bad == 0;
-        if (__all_sync(kFull, all)) return convert_tile(src, st, [](int) { return true; });
-        return convert_tile(src, st, [&](int r) {
-            return ((r >= lo && r <= hi) || (r >= fk && r < pfx)) && !((bad >> (r >> p.box_shift)) & 1);
-        });
-    };
+    int top = 0;                 // V's exponent
+#pragma unroll 1
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
-        const int t0 = g.t0, n = g.t1 - t0, L = g.rep ? 2 : 1;
+        const int t0 = g.t0, n = g.t1 - t0, L = g.mode == kWide ? 1 : 2;
         const TileList tile(g);
         const int4 range = {g.vlo, g.vhi, g.fk, g.pfx};
         top = -60;
-        for (int i = 0; i < min(n, L); ++i, ++pos)
-            if (!V && !convert(range, tile(t0 + i))) return;
-        for (int i = 0; i < n; ++i) {
-            if (V && !convert(range, tile(t0 + i))) return;
-            ++pos;
-            if (i + L < n) {
-                if (!V && !convert(range, tile(t0 + i + L))) return;
-                ++pos;
+#pragma unroll 1
+        for (int i = -L; i < n; ++i) {
+            // V of tile i comes first, then K of tile i + L
+            const int mine = is_v ? i : i + L;
+            const bool here = mine >= 0 && mine < n;
+            const uint32_t e = pos + (!is_v && i >= 0);
+            pos += (i >= 0) + (i + L < n);
+            if (!here) continue;
+            const int st = e % kRaw, j0 = tile(t0 + mine) * kTile;
+            if (!warp_wait(&mi->rfull[st], (e / kRaw) & 1, mi)) return;
+            const unsigned char* src = smem + Layout<kI8>::raw + st * kRawBytes;
+            const __half* scale = reinterpret_cast<const __half*>(smem + Layout<kI8>::raw_scale + st * 256);
+            const uint32_t bad = mi->bad[st];
+            const int lo = range.x - j0, hi = range.y - j0, fk = range.z - j0, pfx = range.w - j0;
+            const bool all = __all_sync(kFull, ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) && bad == 0);
+            auto seen = [&](int r) {
+                return ((r >= lo && r <= hi) || (r >= fk && r < pfx)) && !((bad >> (r >> p.box_shift)) & 1);
+            };
+            const uint32_t m = done++;
+            const int at = m % kScales, d = m % ring;
+            const bool mine_seen = all || seen(t);
+            const float sc = mine_seen ? __half2float(scale[t]) : 0.f;
+            if (!is_v) {
+                // never zero: a hidden key's score is -inf times this
+                scales->k[at][t] = mine_seen ? fmaxf(sc * p.kf, 1e-30f) : 1.f;
+            } else {
+                const int r4 = lane * 4;
+                const uint2 raw = *reinterpret_cast<const uint2*>(scale + r4);
+                const float2 a = __half22float2(as_h2(raw.x)), b = __half22float2(as_h2(raw.y));
+                float most = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
+                if (!all)
+                    most = fmaxf(fmaxf(seen(r4) ? a.x : 0.f, seen(r4 + 1) ? a.y : 0.f),
+                                 fmaxf(seen(r4 + 2) ? b.x : 0.f, seen(r4 + 3) ? b.y : 0.f));
+                const uint32_t bits = __reduce_max_sync(kFull, __float_as_uint(most));
+                top = max(top, static_cast<int>(bits >> 23) - 126);
+                scales->v[at][t] = sc * __int_as_float((127 - top) << 23);
+                scales->v_exp[at] = top;
+                warp_arrive(&mi->vscale[at]);
             }
+            uint4 in[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int r = row_of(q);
+                in[q] = *reinterpret_cast<const uint4*>(src + r * kHeadDim + ((c ^ (r & 7)) << 4));
+            }
+            if (!all) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (!seen(row_of(q))) in[q] = {0, 0, 0, 0};
+            }
+            warp_arrive(&mi->rempty[st]);
+            if (m >= ring && !warp_wait(&mi->empty[is_v][d], (m / ring - 1) & 1, mi)) return;
+            unsigned char* dst = smem + Layout<kI8>::tiles + ((is_v ? ring : 0) + d) * kTileBytes + (c >> 2) * kHalfTile;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int r = row_of(q);
+                half2 o[4];
+                unsigned char* line = dst + r * 128;
+                i8x4_to_h2(in[q].x, o[0], o[1]);
+                i8x4_to_h2(in[q].y, o[2], o[3]);
+                *reinterpret_cast<uint4*>(line + ((x ^ (r & 7)) << 4)) =
+                    uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
+                i8x4_to_h2(in[q].z, o[0], o[1]);
+                i8x4_to_h2(in[q].w, o[2], o[3]);
+                *reinterpret_cast<uint4*>(line + (((x + 1) ^ (r & 7)) << 4)) =
+                    uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
+            }
+            fence_async_smem();
+            warp_arrive(&mi->full[is_v][d]);
         }
         warp_arrive(&mi->segempty[slot]);
     }
@@ -1127,11 +1362,22 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem) {
 constexpr int kUnitCost = 2;
 __device__ __forceinline__ int unit_cost(const Segment& s) { return max(s.nt, 1) + kUnitCost; }
 
-// CTAs that the tiles are split over: none of them goes without, so the CTAs
-// from a split unit's first to its last all hold a part of it.
-__device__ __forceinline__ long long sharing_ctas(const Params& p, long long total) {
-    return min(static_cast<long long>(p.grid), total);
-}
+// The tiles are split over `ctas` CTAs, the first `more` of which take one more
+// than the others. None goes without, so the CTAs from a split unit's first to
+// its last all hold a part of it.
+struct Split {
+    long long each, more, ctas;
+    __device__ Split(const Params& p, long long total)
+        : ctas(min(static_cast<long long>(p.grid), max(total, 1LL))) {
+        each = total / ctas;
+        more = total - each * ctas;
+    }
+    __device__ long long start(long long cta) const { return cta * each + min(cta, more); }
+    __device__ int owner(long long x) const {
+        const long long edge = more * (each + 1);
+        return static_cast<int>(x < edge ? x / (each + 1) : more + (x - edge) / each);
+    }
+};
 
 // This CTA's share [start, start + count) of all units' tiles, and the unit it
 // begins in: a block-wide prefix sum over the unit numbers.
@@ -1141,89 +1387,90 @@ __device__ void plan(const Params& p, Misc* mi) {
     const int chunk = (n_ids + THREADS - 1) / THREADS;
     const int id0 = threadIdx.x * chunk, id1 = min(id0 + chunk, n_ids);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long mine = 0;
+    long long sum = 0, a = 0, at = 0;
     Segment s;
-    for (int id = id0; id < id1; ++id)
-        if (make_unit(p, id, s)) mine += unit_cost(s);
-    long long incl = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(kFull, incl, d);
-        if (lane >= d) incl += o;
-    }
-    if (lane == 31) mi->scan[warp] = incl;
-    __syncthreads();
-    long long before = 0, total = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) before += mi->scan[w];
-        total += mi->scan[w];
-    }
-    total *= p.n_kv;
-    const long long ctas = sharing_ctas(p, total);
-    const long long a = blockIdx.x < ctas ? total * blockIdx.x / ctas : 0;
-    const long long e = blockIdx.x < ctas ? total * (blockIdx.x + 1) / ctas : 0;
-    const long long lo = (before + incl - mine) * p.n_kv, hi = (before + incl) * p.n_kv;
-    if (threadIdx.x == 0) {
-        mi->start = a;
-        mi->count = e - a;
-        mi->total = total;
-    }
-    if (e > a && lo <= a && a < hi) {
-        long long at = lo;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {  // add up; then, in the thread that has it, find the CTA's first unit
+#pragma unroll 1
         for (int id = id0; id < id1; ++id) {
             if (!make_unit(p, id, s)) continue;
             const int c = unit_cost(s);
-            if (a < at + static_cast<long long>(c) * p.n_kv) {
+            if (pass == 0) {
+                sum += c;
+            } else if (a - at < static_cast<long long>(c) * p.n_kv) {
+                const uint32_t rest = static_cast<uint32_t>(a - at);
                 mi->start_id = id;
-                mi->start_head = static_cast<int>((a - at) / c);
-                mi->start_off = static_cast<int>((a - at) % c);
+                mi->start_head = rest / c;
+                mi->start_off = rest % c;
+                mi->first = s;
                 break;
+            } else {
+                at += static_cast<long long>(c) * p.n_kv;
             }
-            at += static_cast<long long>(c) * p.n_kv;
         }
+        if (pass == 1) break;
+        long long incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(kFull, incl, d);
+            if (lane >= d) incl += o;
+        }
+        if (lane == 31) mi->scan[warp] = incl;
+        __syncthreads();
+        long long total = 0;
+#pragma unroll 1
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) at += mi->scan[w];
+            total += mi->scan[w];
+        }
+        total *= p.n_kv;
+        const Split split(p, total);
+        a = split.start(blockIdx.x);
+        const long long e = blockIdx.x < split.ctas ? split.start(blockIdx.x + 1) : a;
+        if (threadIdx.x == 0) {
+            mi->start = a;
+            mi->count = e - a;
+            mi->total = total;
+        }
+        at = (at + incl - sum) * p.n_kv;
+        if (!(e > a && at <= a && a < at + sum * p.n_kv)) break;
     }
 }
 
 __device__ void schedule_role(const Params& p, Misc* mi) {
     const int lane = threadIdx.x & 31;
     long long left = mi->count, at = mi->start;
-    const long long total = mi->total;
+    const Split parts(p, mi->total);
     const int n_ids = p.set[0].n_ids + (p.n_sets > 1 ? p.set[1].n_ids : 0);
     int id = mi->start_id, head = mi->start_head, off = mi->start_off;
     bool split = false;
-    Segment s;
-    if (left > 0) make_unit(p, id, s);
+    Segment s = mi->first;
+#pragma unroll 1
     for (uint32_t k = 0;;) {
         const int slot = k % kSegs;
-        if (left <= 0) {
-            if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
-            if (lane == 0) mi->seg[slot].valid = 0;
-            warp_arrive(&mi->segfull[slot]);
-            break;
-        }
         const int cost = unit_cost(s), tiles = cost - kUnitCost;
         const int n = static_cast<int>(min(left, static_cast<long long>(cost - off)));
         const int t0 = max(off - kUnitCost, 0), t1 = max(off + n - kUnitCost, 0);
-        if (t1 > t0) {
+        const bool last = left <= 0;
+        if (last || t1 > t0) {
             const bool whole = t0 == 0 && t1 == tiles;
-            s.valid = 1;
-            s.head = head;
-            s.t0 = s.nt ? t0 : 0;
-            s.t1 = s.nt ? t1 : 0;
-            s.dest = !whole ? kSlot : p.shared ? kRowBuf : kDirect;
             if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
             if (lane == 0) {
+                s.valid = !last;
+                s.head = head;
+                s.t0 = s.nt ? t0 : 0;
+                s.t1 = s.nt ? t1 : 0;
+                s.dest = !whole ? kSlot : p.shared ? kRowBuf : kDirect;
                 mi->seg[slot] = s;
-                if (t0 == 0) {
-                    const long long end = at - off + cost - 1;  // its last tile's owner finishes the unit
-                    const int last =
-                        whole ? -1 : static_cast<int>(((end + 1) * sharing_ctas(p, total) - 1) / total);
-                    if (p.shared) p.units[static_cast<size_t>(id) * p.n_kv + head] = {static_cast<int>(blockIdx.x), last};
-                    if (!whole) p.split[blockIdx.x] = {s.tok0, s.ntok, head, last};
+                if (!last && t0 == 0) {  // a split unit is finished by the owner of its last tile
+                    const int to = whole ? -1 : parts.owner(at - off + cost - 1);
+                    if (p.shared) p.units[static_cast<size_t>(id) * p.n_kv + head] = {static_cast<int>(blockIdx.x), to};
+                    if (!whole) p.split[blockIdx.x] = {s.tok0, s.ntok, head, to};
                 }
             }
-            split |= t0 == 0 && !whole;
             warp_arrive(&mi->segfull[slot]);
+            if (last) break;
+            split |= t0 == 0 && !whole;
             ++k;
         }
         at += n;
@@ -1271,6 +1518,7 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
             mbar_init(&mi->segempty[i], readers);
         }
         for (int i = 0; i < kScales; ++i) mbar_init(&mi->vscale[i], 4);
+        for (int i = 0; i < 2; ++i) mbar_init(&mi->tbar[i], 4);
         mbar_init(&mi->xbar, 8);
         mbar_init(&mi->drain, 1);
         mi->abort = 0;
@@ -1285,17 +1533,20 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    const uint32_t tmem = mi->tmem;
+    // All columns were asked for, so they start at 0: a constant, which keeps
+    // the matrix instructions' operands in uniform registers. (Checked: any
+    // other answer ends the block as an expired wait does.)
+    if (mi->tmem != kTmem) *reinterpret_cast<volatile int*>(&mi->abort) = 1;
 
     if (warp < 8) {
         regs_inc<Lay::softmax_regs>();
-        softmax_role<FMT, MOD>(p, mi, smem, tmem);
+        softmax_role<FMT, MOD>(p, mi, smem);
     } else if (warp < 12) {
         regs_dec<Lay::other_regs>();
         if (warp == 8) {
             copy_role<FMT>(p, mi, smem, maps);
         } else if (warp == 9) {
-            mma_role<FMT>(p, mi, smem, tmem);
+            mma_role<FMT>(p, mi, smem);
             if (*reinterpret_cast<volatile int*>(&mi->abort)) {  // wait out what is still running
                 mma_commit(&mi->drain, elect_one());
                 for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->drain, 0); ++i) {}
@@ -1306,10 +1557,7 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     } else {
         if constexpr (FMT != kF16) {
             regs_dec<Lay::convert_regs>();
-            if (warp < 16)
-                convert_role<false>(p, mi, smem);
-            else
-                convert_role<true>(p, mi, smem);
+            convert_role(p, mi, smem, warp >= 16);
         }
     }
     __syncwarp();
@@ -1317,7 +1565,8 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     __syncthreads();
     if (warp == 9) {
         tcgen05_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(mi->tmem, 512);
+        if (mi->abort) atomicCAS(&g_attention_error, 0, static_cast<int>(kDevWaitTimeout));
     }
 }
 
@@ -1579,6 +1828,11 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.n_heads = static_cast<int>(a.n_heads);
     p.n_kv = static_cast<int>(a.n_kv_heads);
     p.group = p.n_heads / p.n_kv;
+    p.per = w.per;
+    p.thin_per = kThinRows / p.group;
+    p.by_group = make_div(p.group);
+    p.by_unit = make_div(w.unit);
+    p.by_block = make_div(static_cast<uint32_t>(a.block_size));
     p.num_blocks = static_cast<int>(a.num_blocks);
     p.block_size = static_cast<int>(a.block_size);
     p.box_rows = std::min(kTile, p.block_size & -p.block_size);  // boxes never cross a page
@@ -1600,8 +1854,8 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.units = reinterpret_cast<int2*>(ws + w.units);
 
     Maps maps;
-    for (int i = 0; i < 3; ++i) {
-        const int toks = (kTile >> i) / p.group;
+    for (int i = 0; i < 2; ++i) {
+        const int toks = i ? p.thin_per : p.per;
         if (toks == 0) {
             maps.q[i] = maps.q[0];
             continue;
