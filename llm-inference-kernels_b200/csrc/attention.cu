@@ -104,6 +104,7 @@ struct Params {
     int n_tokens, n_heads, n_kv, group;
     int per, thin_per;  // tokens of 128 rows (a paired unit, half a wide one) and of a thin unit
     Div by_group, by_unit, by_block;
+    int lead, weight[3];
     int num_blocks, block_size, box_rows, box_shift, total_rows;
     const __half* k_scale;
     const __half* v_scale;
@@ -146,6 +147,7 @@ struct Misc {
     uint64_t qfull, qempty, sfull[2], pready[2][2], odone[2][2], tbar[2], segfull[kSegs], segempty[kSegs], xbar, drain;
     Segment seg[kSegs], first;
     long long scan[20];
+    int heavy[20], heaviest;
     long long start, count, total;
     int start_id, start_head, start_off;
     uint32_t bad[kRaw];
@@ -167,7 +169,9 @@ struct ThinRow {
 };
 struct ThinSpace {
     unsigned char w[2][kThinRows * 256];  // per stream: weights [2][row][64 positions], swizzled
-    float top[2][4][kThinRows], sum[2][4][kThinRows], ref[2][kThinRows], down[2][kThinRows];
+    float l[2][kThinRows][kTile];         // each thread's part of a row's sum of weights
+    float top[2][4][kThinRows], sum[2][kThinRows], ref[2][kThinRows], down[2][kThinRows], inv[kThinRows];
+    uint32_t to[kThinRows];
     ThinRow row[kThinRows];
 };
 static_assert(sizeof(ThinSpace) <= kTileBytes, "thin space");
@@ -296,14 +300,13 @@ __device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
 // tanh on [-0.8, 0.8] as an odd polynomial of degree 9, minimax in the absolute
 // error (3.5e-7): Remez exchange on tanh(t) / t over t^2, weighted by t.
 constexpr float kTanhNear = 0.8f;
-struct TanhNear {  // up tanh(in s) for |in s| <= 0.8, the factors folded into the coefficients
+struct TanhNear {  // up tanh(s) for |s| <= 0.8
     float2 c[5];
-    __device__ __forceinline__ TanhNear(float in, float up) {
+    __device__ __forceinline__ TanhNear(float up) {
         const float k[5] = {0.9999951124191284f, -0.3331742584705353f, 0.13186219334602356f, -0.04826131463050842f,
                             0.01146465539932251f};
-        float f = up * in;
 #pragma unroll
-        for (int i = 0; i < 5; ++i, f *= in * in) c[i] = {k[i] * f, k[i] * f};
+        for (int i = 0; i < 5; ++i) c[i] = {k[i] * up, k[i] * up};
     }
     __device__ __forceinline__ float2 operator()(float2 s) const {
         const float2 y = mul2(s, s);
@@ -355,6 +358,29 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo .
     return from & to;
 }
 
+// W scores that are not near zero, capped in place: up tanh(k s), 16 columns at
+// a time (rolled: this code beside the step's own would crowd the instruction
+// cache, and capped scores are mostly near).
+template <int W, bool I8>
+__device__ __forceinline__ void cap_far(float up, float kf, uint32_t s_addr, const float4* ks) {
+#pragma unroll 1
+    for (int i0 = 0; i0 < W; i0 += 16) {
+        float s[16];
+        tmem_ld16(s_addr + i0, s);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 k = I8 ? load_scales(ks + (i0 + i) / 4) : float4{kf, kf, kf, kf};
+            s[i] = up * tanh_exp(s[i] * k.x);
+            s[i + 1] = up * tanh_exp(s[i + 1] * k.y);
+            s[i + 2] = up * tanh_exp(s[i + 2] * k.z);
+            s[i + 3] = up * tanh_exp(s[i + 3] * k.w);
+        }
+        tmem_st16(s_addr + i0, reinterpret_cast<const uint32_t*>(s));
+    }
+    tmem_wait_st();
+}
+
 // One step: the softmax of W score columns at s_addr, keys from j0, into W fp16
 // weights at p_addr. `m` is the row's reference, in powers of two. The weights
 // are worked out with the reference so far; only where a score turns out to lie
@@ -363,40 +389,34 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo .
 // out again. Searched for ahead of the weights it held up every step by a
 // quarter. Weights stay below 2^8, which fp16 holds.
 //
-// Scores come scaled by `kf` (and K's scales, INT8) to powers of two; with MOD,
-// capping and bias follow. INT8: ks holds kf times K's scales, vs V's scales
-// divided by 2^v_exp, the largest so far; the sums are in units of 2^ev. The
-// matrix instructions see the exact codes.
+// INT8: ks holds kf times K's scales, vs V's scales divided by 2^v_exp, the
+// largest so far; the sums are in units of 2^ev. The matrix instructions see the
+// exact codes.
 template <int W, bool I8, bool MOD>
 __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Row& row, uint32_t s_addr, uint32_t p_addr,
-                                             uint32_t o_addr, int j0, bool have_sums, uint64_t* odone,
-                                             uint32_t odone_parity, const float4* ks, const float4* vs, int v_exp,
-                                             float& m, float& l, int& ev) {
+                                             uint32_t o_addr, int j0, bool have_sums, uint64_t* odone, uint32_t odone_parity,
+                                             const float4* ks, const float4* vs, int v_exp, float& m, float& l,
+                                             int& ev) {
     float s[W];
 #pragma unroll
     for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
     tmem_wait_ld();
-    const float kf = p.kf;
-    if (MOD && (I8 || p.cap == 0.f)) {
+    if (MOD) {  // scores to powers of two
+        float far = 0.f;
 #pragma unroll
         for (int i = 0; i < W; i += 4) {
-            const float4 k = I8 ? load_scales(ks + i / 4) : float4{kf, kf, kf, kf};
+            const float4 k = I8 ? load_scales(ks + i / 4) : float4{p.kf, p.kf, p.kf, p.kf};
             const float2 a = mul2({s[i], s[i + 1]}, {k.x, k.y}), b = mul2({s[i + 2], s[i + 3]}, {k.z, k.w});
+            far = max3_abs(max3_abs(far, a.x, a.y), b.x, b.y);
             s[i] = a.x;
             s[i + 1] = a.y;
             s[i + 2] = b.x;
             s[i + 3] = b.y;
         }
-    }
-    const int j1 = j0 + W - 1;
-    if (MOD) {
         if (p.cap > 0.f) {
-            const float in = I8 ? 1.f : kf, up = p.cap * kLog2e;
-            float far[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < W; i += 2) far[i / 2 & 3] = max3_abs(far[i / 2 & 3], s[i], s[i + 1]);
-            if (__all_sync(kFull, fmaxf(max3(far[0], far[1], far[2]), far[3]) * in <= kTanhNear)) {
-                const TanhNear near(in, up);
+            const float up = p.cap * kLog2e;
+            if (__all_sync(kFull, far <= kTanhNear)) {
+                const TanhNear near(up);
 #pragma unroll
                 for (int i = 0; i < W; i += 2) {
                     const float2 t = near({s[i], s[i + 1]});
@@ -404,29 +424,19 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
                     s[i + 1] = t.y;
                 }
             } else {
+                cap_far<W, I8>(up, p.kf, s_addr, ks);
 #pragma unroll
-                for (int i = 0; i < W; ++i) s[i] = up * tanh_exp(s[i] * in);
+                for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
+                tmem_wait_ld();
             }
         }
         if (p.slopes) {
             const float from = static_cast<float>(j0) - row.pos;
-            if (__all_sync(kFull, from + static_cast<float>(W - 1) <= 0.f)) {  // no key behind the query
-                const float2 up = {row.slope, row.slope}, two = {2.f, 2.f};
-                float2 d = {from, from + 1.f};
 #pragma unroll
-                for (int i = 0; i < W; i += 2) {
-                    const float2 t = fma2(up, d, {s[i], s[i + 1]});
-                    s[i] = t.x;
-                    s[i + 1] = t.y;
-                    d = add2(d, two);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < W; ++i) s[i] = fmaf(-row.slope, fabsf(from + static_cast<float>(i)), s[i]);
-            }
+            for (int i = 0; i < W; ++i) s[i] = fmaf(-row.slope, fabsf(from + static_cast<float>(i)), s[i]);
         }
     }
-    const bool whole = (j0 >= row.lo && j1 <= row.hi) || (j0 >= row.fk && j1 < row.pfx);
+    const bool whole = (j0 >= row.lo && j0 + W - 1 <= row.hi) || (j0 >= row.fk && j0 + W <= row.pfx);
     if (__any_sync(kFull, !whole)) {
 #pragma unroll
         for (int i = 0; i < W; i += 32) {
@@ -436,6 +446,7 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
             for (int c = 0; c < 32; ++c) s[i + c] = (see >> c) & 1u ? s[i + c] : -INFINITY;
         }
     }
+    const float kf = MOD ? 1.f : p.kf;
 #pragma unroll 1
     for (bool again = false;; again = true) {
         const float ms = m == -INFINITY ? 0.f : -m, ms_u = (ms + 56.f) * (1.f / 64.f);
@@ -450,7 +461,7 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
             float2 k = {kf, kf}, v = {1.f, 1.f};
             if (I8) {
                 if (c % 2 == 0) {
-                    if (!MOD) k4 = load_scales(ks + c / 2);
+                    k4 = MOD ? float4{1.f, 1.f, 1.f, 1.f} : load_scales(ks + c / 2);
                     v4 = load_scales(vs + c / 2);
                 }
                 k = c & 1 ? float2{k4.z, k4.w} : float2{k4.x, k4.y};
@@ -463,13 +474,12 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
                     x = fma2({a, b}, k, ms2);
                     u = {fma_sat(x.x, 1.f / 64.f, 56.f / 64.f), fma_sat(x.y, 1.f / 64.f, 56.f / 64.f)};
                 } else {
-                    const float f = (MOD ? 1.f : kf) * (1.f / 64.f);
-                    u = {fma_sat(a, f, ms_u), fma_sat(b, f, ms_u)};
+                    u = {fma_sat(a, kf * (1.f / 64.f), ms_u), fma_sat(b, kf * (1.f / 64.f), ms_u)};
                 }
                 full = max3(full, u.x, u.y);
                 x = exp2_cubic(u);
             } else {
-                x = MOD ? add2({a, b}, ms2) : fma2({a, b}, k, ms2);
+                x = fma2({a, b}, k, ms2);
                 over[c & 1] = max3(over[c & 1], x.x, x.y);
                 x.x = fast_exp2(x.x);
                 x.y = fast_exp2(x.y);
@@ -489,7 +499,7 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < W; i += 4) {
-            const float4 k = MOD ? float4{1.f, 1.f, 1.f, 1.f} : I8 ? load_scales(ks + i / 4) : float4{kf, kf, kf, kf};
+            const float4 k = I8 && !MOD ? load_scales(ks + i / 4) : float4{kf, kf, kf, kf};
             top = max3(top, s[i] * k.x, s[i + 1] * k.y);
             top = max3(top, s[i + 2] * k.z, s[i + 3] * k.w);
         }
@@ -506,13 +516,13 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
             if (odone && !warp_wait(odone, odone_parity, mi)) return false;
             tcgen05_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < kHeadDim; c += 32) {
-                float o[32];
-                tmem_ld32(o_addr + c, o);
+            for (int c = 0; c < kHeadDim; c += 16) {
+                float o[16];
+                tmem_ld16(o_addr + c, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] *= fo;
-                tmem_st32(o_addr + c, o);
+                for (int i = 0; i < 16; ++i) o[i] *= fo;
+                tmem_st16(o_addr + c, reinterpret_cast<const uint32_t*>(o));
             }
         }
     }
@@ -544,10 +554,10 @@ __device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Sca
         const int v_exp = I8 ? scales->v_exp[st] : 0;
 #pragma unroll 1
         for (int c = 0; c < kTile; c += W) {
+            const float4* ks = reinterpret_cast<const float4*>(scales->k[st] + c);
             if (!softmax_step<W, I8, MOD>(p, mi, row, s_addr + c, s_addr + c / 2, o_addr, j0 + c, i > i0 || c > 0,
-                                          c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1,
-                                          reinterpret_cast<const float4*>(scales->k[st] + c),
-                                          reinterpret_cast<const float4*>(scales->v[st] + c), v_exp, m, l, ev))
+                                     c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1, ks,
+                                     reinterpret_cast<const float4*>(scales->v[st] + c), v_exp, m, l, ev))
                 return false;
             tmem_wait_st();
             tcgen05_fence_before();
@@ -633,10 +643,9 @@ __device__ __forceinline__ bool stream_sync(Misc* mi, int stream, uint32_t& phas
 // A thin segment. Scores come transposed, [position][row], so a thread holds one
 // position's scores of all rows; a row's reference is the same in all 128
 // threads of the stream, and each keeps its own part of the sum of weights. A
-// vote per tile finds out whether any reference has to be raised. What is
-// needed for few tiles (masks, the raising) or rows goes four rows at a time
-// through tensor memory, in loops: unrolled it made the kernel twice as large
-// and slower than its instruction fetches.
+// vote per tile finds out whether any reference has to be raised first. Four
+// rows at a time, in loops: unrolled over the rows the kernel was twice as large
+// and waited for its instructions.
 template <int FMT, bool MOD>
 __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, const Segment& g, int stream, uint32_t before,
                              uint32_t s_addr, uint32_t o_addr, uint32_t& tiles, uint32_t& tphase, uint32_t& votes,
@@ -671,9 +680,10 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         fk_max = max(fk_max, sp->row[r].fk);
     }
     float* const ref = sp->ref[stream];
-    float l[NT];
-#pragma unroll
-    for (int r = 0; r < NT; ++r) l[r] = 0.f;
+    float* const l = &sp->l[stream][0][r_in];
+    const int rows4 = (rows + 3) & ~3;
+#pragma unroll 1
+    for (int r = 0; r < rows4; ++r) l[r * kTile] = 0.f;
     int ev = -200;
     const int t0 = g.t0, t1 = g.t1;
     const TileList tile(g);
@@ -690,9 +700,37 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         if (I8 && !warp_wait(&mi->vscale[st], (at / kScales) & 1, mi)) return false;
         const int v_exp = I8 ? scales->v_exp[st] : 0;
         const float vx = I8 ? scales->v[st][r_in] : 1.f;
-        float kx = I8 ? scales->k[st][r_in] : p.kf;
+        const float kx = I8 ? scales->k[st][r_in] : p.kf;
         const bool whole = (j0 >= lo_max && j0 + kTile - 1 <= hi_min) || (j0 >= fk_max && j0 + kTile <= pfx);
-        if (MOD || !whole) {  // scores in powers of two, -inf where hidden, written back
+        bool low = I8 && v_exp > ev;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 4) {  // scores in powers of two, -inf where hidden, written back
+            float x[4];
+            tmem_ld4(s_addr + r0, x);
+            const float4 m4 = *reinterpret_cast<const float4*>(ref + r0);
+            const float m[4] = {m4.x, m4.y, m4.z, m4.w};
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                x[c] *= kx;
+                if (MOD && p.cap > 0.f) x[c] = p.cap * kLog2e * tanh_exp(x[c]);
+                if (MOD && p.slopes)
+                    x[c] = fmaf(-sp->row[r0 + c].slope, fabsf(static_cast<float>(j) - sp->row[r0 + c].pos), x[c]);
+                if (!whole || r0 + c >= rows) {
+                    const ThinRow& q = sp->row[r0 + c];
+                    if (!((j >= q.lo && j <= q.hi) || (j >= q.fk && j < pfx && r0 + c < rows))) x[c] = -INFINITY;
+                }
+                low = low || x[c] - m[c] > kRaise;
+            }
+            tmem_st4(s_addr + r0, x);
+        }
+        tmem_wait_st();
+        low = __any_sync(kFull, low);
+        int* const flag = mi->low[stream][votes++ & 1];
+        if (lane == 0) *reinterpret_cast<volatile int*>(flag + warp) = low;
+        if (!stream_sync(mi, stream, tphase)) return false;
+        const volatile int* f = flag;
+        if (f[0] | f[1] | f[2] | f[3]) {  // raise the references to the tile's maxima
 #pragma unroll 1
             for (int r0 = 0; r0 < rows; r0 += 4) {
                 float x[4];
@@ -700,55 +738,9 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
                 tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const ThinRow& q = sp->row[r0 + c];
-                    x[c] *= kx;
-                    if (MOD && p.cap > 0.f) x[c] = p.cap * kLog2e * tanh_exp(x[c]);
-                    if (MOD && p.slopes) x[c] = fmaf(-q.slope, fabsf(static_cast<float>(j) - q.pos), x[c]);
-                    if (!((j >= q.lo && j <= q.hi) || (j >= q.fk && j < pfx))) x[c] = -INFINITY;
-                }
-                tmem_st4(s_addr + r0, x);
-            }
-            tmem_wait_st();
-            kx = 1.f;
-        }
-#pragma unroll 1
-        for (int pass = 0;; ++pass) {
-            float x[NT];
-            tmem_ld16(s_addr, x);
-            tmem_wait_ld();
-            bool low = I8 && v_exp > ev;
 #pragma unroll
-            for (int r = 0; r < NT; ++r) {
-                if (r < rows) {
-                    const float m = ref[r];
-                    x[r] *= kx;
-                    low = low || x[r] - m > kRaise;
-                    x[r] = fast_exp2(x[r] - (m == -INFINITY ? 0.f : m));
-                    *reinterpret_cast<__half*>(w_at + r * 128 + ((chunk ^ (r & 7)) << 4)) = __float2half_rn(x[r] * vx);
-                }
-            }
-            low = __any_sync(kFull, low);
-            int* const flag = mi->low[stream][votes++ & 1];
-            if (lane == 0) *reinterpret_cast<volatile int*>(flag + warp) = low;
-            fence_async_smem();  // the weights, for the matrix instructions
-            if (!stream_sync(mi, stream, tphase)) return false;
-            const volatile int* f = flag;
-            if (pass > 0 || !(f[0] | f[1] | f[2] | f[3])) {
-#pragma unroll
-                for (int r = 0; r < NT; ++r) l[r] += r < rows ? x[r] : 0.f;
-                break;
-            }
-            // raise the references to the tile's maxima
-#pragma unroll 1
-            for (int r0 = 0; r0 < rows; r0 += 4) {
-                tmem_ld4(s_addr + r0, x);
-                tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float t = x[c] * kx;
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, d));
-                    if (lane == 0) sp->top[stream][warp][r0 + c] = t;
+                    for (int d = 16; d; d >>= 1) x[c] = fmaxf(x[c], __shfl_xor_sync(kFull, x[c], d));
+                    if (lane == 0) sp->top[stream][warp][r0 + c] = x[c];
                 }
             }
             if (!stream_sync(mi, stream, tphase)) return false;
@@ -760,9 +752,6 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
                 ref[r_in] = up;
             }
             if (!stream_sync(mi, stream, tphase)) return false;
-#pragma unroll
-            for (int r = 0; r < NT; ++r)
-                if (r < rows) l[r] *= sp->down[stream][r];
             float fo = 1.f;
             if (I8) {
                 fo = fast_exp2(static_cast<float>(ev - v_exp));
@@ -771,15 +760,36 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
             if (any) {  // this stream's products so far are done: the scores came after them
 #pragma unroll 1
                 for (int r0 = 0; r0 < rows; r0 += 4) {
+                    float x[4];
                     tmem_ld4(o_addr + r0, x);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) x[c] *= r0 + c < rows ? sp->down[stream][r0 + c] * fo : 0.f;
+                    for (int c = 0; c < 4; ++c) {
+                        const float d = r0 + c < rows ? sp->down[stream][r0 + c] : 0.f;
+                        l[(r0 + c) * kTile] *= d;
+                        x[c] *= d * fo;
+                    }
                     tmem_st4(o_addr + r0, x);
                 }
                 tmem_wait_st();
             }
         }
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 4) {
+            float x[4];
+            tmem_ld4(s_addr + r0, x);
+            const float4 m4 = *reinterpret_cast<const float4*>(ref + r0);
+            const float m[4] = {m4.x, m4.y, m4.z, m4.w};
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int r = r0 + c;
+                const float e = fast_exp2(x[c] - (m[c] == -INFINITY ? 0.f : m[c]));
+                l[r * kTile] += e;
+                *reinterpret_cast<__half*>(w_at + r * 128 + ((chunk ^ (r & 7)) << 4)) = __float2half_rn(e * vx);
+            }
+        }
+        fence_async_smem();  // the weights, for the matrix instructions
         tcgen05_fence_before();
         warp_arrive(&mi->pready[stream][1]);
     }
@@ -788,18 +798,32 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         tcgen05_fence_after();
     }
     // join the two streams; a thread holds one channel of all rows now
-    const float unit_v = I8 && any ? fast_exp2(static_cast<float>(ev)) : 1.f;
+    if (!stream_sync(mi, stream, tphase)) return false;
+#pragma unroll 1
+    for (int r = warp; r < rows; r += 4) {
+        const float4 q = *reinterpret_cast<const float4*>(&sp->l[stream][r][lane * 4]);
+        float t = (q.x + q.y) + (q.z + q.w);
 #pragma unroll
-    for (int r = 0; r < NT; ++r) {
-        if (r < rows) {
-            float t = l[r];
-#pragma unroll
-            for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(kFull, t, d);
-            if (lane == 0) sp->sum[stream][warp][r] = t;
-        }
+        for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(kFull, t, d);
+        if (lane == 0) sp->sum[stream][r] = t;
     }
     if (!softmax_sync(mi, xphase)) return false;
-    float* const other = reinterpret_cast<float*>(smem + Layout<FMT>::stage);  // [row][channel]
+    if (r_in < rows) {  // each stream's factors, and where the row goes
+        const float m0 = sp->ref[0][r_in], m1 = sp->ref[1][r_in], top = fmaxf(m0, m1);
+        const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
+        sp->down[stream][r_in] = (stream ? a1 : a0) * (I8 && any ? fast_exp2(static_cast<float>(ev)) : 1.f);
+        if (stream == 0) {
+            const float sum = a0 * sp->sum[0][r_in] + a1 * sp->sum[1][r_in];
+            const int tl = p.by_group(r_in);
+            const uint32_t to = dest_row(p, g, g.tok0 + tl, g.head * p.group + r_in - tl * p.group, r_in);
+            store_ml(p, g, to, top, sum);
+            sp->inv[r_in] = sum > 0.f ? 1.f / sum : 0.f;
+            sp->to[r_in] = to;
+        }
+    }
+    if (!stream_sync(mi, stream, tphase)) return false;
+    float* const other = reinterpret_cast<float*>(smem + Layout<FMT>::stage) + r_in;  // [row][channel]
+    const int dest = g.dest;
 #pragma unroll 1
     for (int turn = 1; turn >= 0; --turn) {  // stream 1 hands over, stream 0 adds and stores
 #pragma unroll 1
@@ -813,27 +837,18 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
             for (int c = 0; c < 4; ++c) {
                 const int r = r0 + c;
                 if (r >= rows) break;
-                const float m0 = sp->ref[0][r], m1 = sp->ref[1][r], top = fmaxf(m0, m1);
-                const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
-                const float f = (stream ? a1 : a0) * unit_v;
-                const float v = f > 0.f ? x[c] * f : 0.f;
+                const float f = sp->down[stream][r];
+                float v = f > 0.f ? x[c] * f : 0.f;
                 if (turn) {
-                    other[r * kHeadDim + r_in] = v;
+                    other[r * kHeadDim] = v;
                     continue;
                 }
-                const float* s0 = sp->sum[0][0] + r;
-                const float* s1 = sp->sum[1][0] + r;
-                const float sum = a0 * ((s0[0] + s0[NT]) + (s0[2 * NT] + s0[3 * NT])) +
-                                  a1 * ((s1[0] + s1[NT]) + (s1[2 * NT] + s1[3 * NT]));
-                const float all = v + other[r * kHeadDim + r_in];
-                const int tl = p.by_group(r);
-                const uint32_t to = dest_row(p, g, g.tok0 + tl, g.head * p.group + r - tl * p.group, r);
-                if (r_in == 0) store_ml(p, g, to, top, sum);
-                const size_t e = static_cast<size_t>(to) * kHeadDim + r_in;
-                if (g.dest == kDirect)
-                    p.out[e] = __float2half_rn(sum > 0.f ? all / sum : 0.f);
+                v += other[r * kHeadDim];
+                const size_t e = static_cast<size_t>(sp->to[r]) * kHeadDim + r_in;
+                if (dest == kDirect)
+                    p.out[e] = __float2half_rn(v * sp->inv[r]);
                 else
-                    (g.dest == kSlot ? p.part : p.rowbuf)[e] = all;
+                    (dest == kSlot ? p.part : p.rowbuf)[e] = v;
             }
         }
         if (turn == 0) fence_async_smem();  // queries may be copied over the space that was used here
@@ -1326,11 +1341,6 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
                 const int r = row_of(q);
                 in[q] = *reinterpret_cast<const uint4*>(src + r * kHeadDim + ((c ^ (r & 7)) << 4));
             }
-            if (!all) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (!seen(row_of(q))) in[q] = {0, 0, 0, 0};
-            }
             warp_arrive(&mi->rempty[st]);
             if (m >= ring && !warp_wait(&mi->empty[is_v][d], (m / ring - 1) & 1, mi)) return;
             unsigned char* dst = smem + Layout<kI8>::tiles + ((is_v ? ring : 0) + d) * kTileBytes + (c >> 2) * kHalfTile;
@@ -1348,6 +1358,15 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
                 *reinterpret_cast<uint4*>(line + (((x + 1) ^ (r & 7)) << 4)) =
                     uint4{as_u32(o[0]), as_u32(o[1]), as_u32(o[2]), as_u32(o[3])};
             }
+            if (!all) {
+#pragma unroll 1
+                for (int q = 0; q < 8; ++q) {
+                    const int r = row_of(q);
+                    if (seen(r)) continue;
+                    *reinterpret_cast<uint4*>(dst + r * 128 + ((x ^ (r & 7)) << 4)) = uint4{0, 0, 0, 0};
+                    *reinterpret_cast<uint4*>(dst + r * 128 + (((x + 1) ^ (r & 7)) << 4)) = uint4{0, 0, 0, 0};
+                }
+            }
             fence_async_smem();
             warp_arrive(&mi->full[is_v][d]);
         }
@@ -1357,18 +1376,21 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
 
 // ---- schedule --------------------------------------------------------------------
 
-// Cost of a unit in tiles: its own (an empty one still writes its rows) behind
-// what starting and finishing one takes.
-constexpr int kUnitCost = 2;
-__device__ __forceinline__ int unit_cost(const Segment& s) { return max(s.nt, 1) + kUnitCost; }
+// Cost of a unit: its tiles (an empty one still writes its rows) behind what
+// starting and finishing one takes. A tile weighs p.weight[mode], what it was
+// measured to take; tile t of a unit lies at lead + t * weight and belongs to the
+// CTA that this position belongs to.
+__device__ __forceinline__ int unit_cost(const Params& p, const Segment& s) {
+    return p.lead + max(s.nt, 1) * p.weight[s.mode];
+}
 
-// The tiles are split over `ctas` CTAs, the first `more` of which take one more
-// than the others. None goes without, so the CTAs from a split unit's first to
-// its last all hold a part of it.
+// The units, laid end to end, are split over `ctas` CTAs, the first `more` of
+// which take one more than the others. Each takes at least the heaviest tile's
+// weight, so that from a split unit's first CTA to its last all have a tile of it.
 struct Split {
     long long each, more, ctas;
-    __device__ Split(const Params& p, long long total)
-        : ctas(min(static_cast<long long>(p.grid), max(total, 1LL))) {
+    __device__ Split(const Params& p, long long total, int heaviest)
+        : ctas(max(min(static_cast<long long>(p.grid), total / max(heaviest, 1)), 1LL)) {
         each = total / ctas;
         more = total - each * ctas;
     }
@@ -1388,15 +1410,17 @@ __device__ void plan(const Params& p, Misc* mi) {
     const int id0 = threadIdx.x * chunk, id1 = min(id0 + chunk, n_ids);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long sum = 0, a = 0, at = 0;
+    int heaviest = 0;
     Segment s;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {  // add up; then, in the thread that has it, find the CTA's first unit
 #pragma unroll 1
         for (int id = id0; id < id1; ++id) {
             if (!make_unit(p, id, s)) continue;
-            const int c = unit_cost(s);
+            const int c = unit_cost(p, s);
             if (pass == 0) {
                 sum += c;
+                heaviest = max(heaviest, p.weight[s.mode]);
             } else if (a - at < static_cast<long long>(c) * p.n_kv) {
                 const uint32_t rest = static_cast<uint32_t>(a - at);
                 mi->start_id = id;
@@ -1415,22 +1439,28 @@ __device__ void plan(const Params& p, Misc* mi) {
             const long long o = __shfl_up_sync(kFull, incl, d);
             if (lane >= d) incl += o;
         }
-        if (lane == 31) mi->scan[warp] = incl;
+        heaviest = __reduce_max_sync(kFull, heaviest);
+        if (lane == 31) {
+            mi->scan[warp] = incl;
+            mi->heavy[warp] = heaviest;
+        }
         __syncthreads();
         long long total = 0;
 #pragma unroll 1
         for (int w = 0; w < THREADS / 32; ++w) {
             if (w < warp) at += mi->scan[w];
             total += mi->scan[w];
+            heaviest = max(heaviest, mi->heavy[w]);
         }
         total *= p.n_kv;
-        const Split split(p, total);
+        const Split split(p, total, heaviest);
         a = split.start(blockIdx.x);
         const long long e = blockIdx.x < split.ctas ? split.start(blockIdx.x + 1) : a;
         if (threadIdx.x == 0) {
             mi->start = a;
             mi->count = e - a;
             mi->total = total;
+            mi->heaviest = heaviest;
         }
         at = (at + incl - sum) * p.n_kv;
         if (!(e > a && at <= a && a < at + sum * p.n_kv)) break;
@@ -1440,7 +1470,7 @@ __device__ void plan(const Params& p, Misc* mi) {
 __device__ void schedule_role(const Params& p, Misc* mi) {
     const int lane = threadIdx.x & 31;
     long long left = mi->count, at = mi->start;
-    const Split parts(p, mi->total);
+    const Split parts(p, mi->total, mi->heaviest);
     const int n_ids = p.set[0].n_ids + (p.n_sets > 1 ? p.set[1].n_ids : 0);
     int id = mi->start_id, head = mi->start_head, off = mi->start_off;
     bool split = false;
@@ -1448,9 +1478,11 @@ __device__ void schedule_role(const Params& p, Misc* mi) {
 #pragma unroll 1
     for (uint32_t k = 0;;) {
         const int slot = k % kSegs;
-        const int cost = unit_cost(s), tiles = cost - kUnitCost;
+        const int cost = unit_cost(p, s), weight = p.weight[s.mode], tiles = max(s.nt, 1);
         const int n = static_cast<int>(min(left, static_cast<long long>(cost - off)));
-        const int t0 = max(off - kUnitCost, 0), t1 = max(off + n - kUnitCost, 0);
+        // tiles that begin within [off, off + n)
+        const int t0 = (max(off - p.lead, 0) + weight - 1) / weight;
+        const int t1 = (max(off + n - p.lead, 0) + weight - 1) / weight;
         const bool last = left <= 0;
         if (last || t1 > t0) {
             const bool whole = t0 == 0 && t1 == tiles;
@@ -1463,7 +1495,7 @@ __device__ void schedule_role(const Params& p, Misc* mi) {
                 s.dest = !whole ? kSlot : p.shared ? kRowBuf : kDirect;
                 mi->seg[slot] = s;
                 if (!last && t0 == 0) {  // a split unit is finished by the owner of its last tile
-                    const int to = whole ? -1 : parts.owner(at - off + cost - 1);
+                    const int to = whole ? -1 : parts.owner(at - off + cost - weight);
                     if (p.shared) p.units[static_cast<size_t>(id) * p.n_kv + head] = {static_cast<int>(blockIdx.x), to};
                     if (!whole) p.split[blockIdx.x] = {s.tok0, s.ntok, head, to};
                 }
@@ -1830,6 +1862,14 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.group = p.n_heads / p.n_kv;
     p.per = w.per;
     p.thin_per = kThinRows / p.group;
+    // clocks measured per tile, in units of 600: wide 2400 (fp16) and 4800
+    // (INT8, converted on the way), paired 1800 and 3000, thin 1800 (what its bytes
+    // take from memory) and 2400; 5400 to start and finish a unit
+    const bool int8 = a.fmt != kF16;
+    p.lead = 9;
+    p.weight[kWide] = int8 ? 8 : 4;
+    p.weight[kPaired] = int8 ? 5 : 3;
+    p.weight[kThin] = int8 ? 4 : 4;
     p.by_group = make_div(p.group);
     p.by_unit = make_div(w.unit);
     p.by_block = make_div(static_cast<uint32_t>(a.block_size));
