@@ -278,7 +278,8 @@ size_t lik_attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t 
  *   if softcap > 0: score = softcap * tanh(score / softcap)
  *   if alibi_slopes (fp32 [n_heads]): score -= slope * |p - j|
  *   visible: j < context_lens[b], j >= first_keys[token] (int32 [n_tokens], may
- *     be NULL: the start of the token's document), and either
+ *     be NULL: the start of the token's document; within a sequence it does not
+ *     decrease from token to token), and either
  *     j < prefix_lens[b] (int32 [n_seqs], may be NULL: a prefix that every query
  *     of the sequence sees), or j <= p if causal and j > p - window if window > 0
  *

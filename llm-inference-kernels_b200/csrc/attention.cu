@@ -54,8 +54,8 @@ namespace {
 constexpr int kTile = 128;                       // key positions per tile
 constexpr int kTileBytes = kTile * kHeadDim * 2; // one fp16 K or V tile
 constexpr int kHalfTile = kTileBytes / 2;        // its 64-channel half
-constexpr int kRing8 = 1, kRing16 = 2;           // fp16 tiles of K, and of V, in flight
-constexpr int kRaw = 4;                          // INT8 tiles in flight
+constexpr int kMaxRing = 2;                      // fp16 tiles of K, and of V, in flight
+constexpr int kRaw = 2;                          // INT8 tiles of K, and of V, in flight
 constexpr int kRawBytes = kTile * kHeadDim;      // codes; their scales: 256 bytes
 constexpr int kScales = 4;                       // INT8: tiles whose scales are kept
 constexpr int kSegs = 4;
@@ -143,14 +143,14 @@ struct TileList {
 };
 
 struct Misc {
-    uint64_t full[2][kRing16], empty[2][kRing16], rfull[kRaw], rempty[kRaw], vscale[kScales];
+    uint64_t full[2][kMaxRing], empty[2][kMaxRing], rfull[2][kRaw], rempty[2][kRaw], vscale[kScales];
     uint64_t qfull, qempty, sfull[2], pready[2][2], odone[2][2], tbar[2], segfull[kSegs], segempty[kSegs], xbar, drain;
     Segment seg[kSegs], first;
     long long scan[20];
     int heavy[20], heaviest;
     long long start, count, total;
     int start_id, start_head, start_off;
-    uint32_t bad[kRaw];
+    uint32_t bad[2][kRaw];
     int low[2][2][4];  // thin units: a warp's reference is too low
     int abort;
     uint32_t tmem;
@@ -178,12 +178,13 @@ static_assert(sizeof(ThinSpace) <= kTileBytes, "thin space");
 
 template <int FMT>
 struct Layout {
-    static constexpr int ring = FMT == kF16 ? kRing16 : kRing8;
+    static constexpr int ring = FMT == kF16 ? 2 : 1;
     static constexpr int tiles = 2 * kTileBytes;  // K's, then V's
-    static constexpr int raw = tiles + 2 * ring * kTileBytes;
+    static constexpr int v_tiles = tiles + ring * kTileBytes;
+    static constexpr int raw = v_tiles + ring * kTileBytes;  // K's, then V's; then their scales
     // results on their way out, see softmax_role
-    static constexpr int raw_scale = raw + kRaw * kRawBytes;
-    static constexpr int stage = raw + (FMT == kF16 ? 0 : kRaw * (kRawBytes + 256));
+    static constexpr int raw_scale = raw + 2 * kRaw * kRawBytes;
+    static constexpr int stage = raw + (FMT == kF16 ? 0 : 2 * kRaw * (kRawBytes + 256));
     static constexpr int stage_bytes = FMT == kF16 ? 32768 : 16384;
     static constexpr int scales = stage + stage_bytes;
     static constexpr int misc = scales + (FMT == kF16 ? 0 : 4352);
@@ -265,12 +266,7 @@ __device__ bool make_unit(const Params& p, int id, Segment& s) {
                                  static_cast<long long>(k.width) * p.block_size));
     s.pos0 = s.ctx - n + at;
     s.pfx = p.prefix_lens && s.set == 0 ? min(p.prefix_lens[b], s.ctx) : 0;
-    int fk = 0;
-    if (p.first_keys) {
-        fk = 0x7fffffff;
-        for (int i = 0; i < s.ntok; ++i) fk = min(fk, p.first_keys[s.tok0 + i]);
-        fk = max(fk, 0);
-    }
+    const int fk = p.first_keys ? max(p.first_keys[s.tok0], 0) : 0;  // they do not decrease
     s.fk = fk;
     s.vlo = p.window > 0 ? max(s.pos0 - p.window + 1, fk) : fk;
     s.vhi = k.causal ? min(s.pos0 + s.ntok - 1, s.ctx - 1) : s.ctx - 1;
@@ -601,7 +597,9 @@ __device__ __forceinline__ void store_wide(unsigned char* stage, unsigned char* 
 #pragma unroll
         for (int i = 0; i < cols; ++i) o[i] = 0.f;
         if (any) {
-            if constexpr (cols == 16) {
+            if constexpr (cols == 8) {
+                tmem_ld8(o_addr + c, o);
+            } else if constexpr (cols == 16) {
                 tmem_ld16(o_addr + c, o);
             } else {
 #pragma unroll
@@ -1003,9 +1001,12 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem) {
     constexpr int ring = Layout<FMT>::ring;
     constexpr uint32_t id_qk = mma_idesc_f16(128, 128, false), id_pv = mma_idesc_f16(128, 128, true);
     const int lane = threadIdx.x & 31;
-    const uint32_t q_addr = smem_addr(smem), k_addr = q_addr + Layout<FMT>::tiles, v_addr = k_addr + ring * kTileBytes;
+    const uint32_t q_addr = smem_addr(smem), k_addr = q_addr + Layout<FMT>::tiles,
+                   v_addr = q_addr + Layout<FMT>::v_tiles;
     uint32_t n_k = 0, n_v = 0, ph[2][2] = {};  // tiles of K and V; weights taken per stream and half
-    auto wait_tile = [&](int v, uint32_t e) { return warp_wait(&mi->full[v][e % ring], (e / ring) & 1, mi); };
+    auto wait_tile = [&](int v, uint32_t e) {
+        return warp_wait(&mi->full[v][e % ring], (e / ring) & 1, mi);
+    };
     // descriptors differ by constants: one addition each, in uniform registers
     const uint32_t leader = elect_one();
     const uint64_t q_desc = smem_desc(q_addr, 16, 1024), k_desc = smem_desc(k_addr, 16, 1024),
@@ -1059,7 +1060,7 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem) {
         const int j0 = tile * kTile;
         const int lo = seen.x - j0, hi = seen.y - j0, fk = seen.z - j0, pfx = seen.w - j0;
         if ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) return;
-        unsigned char* v = smem + Layout<FMT>::tiles + (ring + e % ring) * kTileBytes + (lane & 7) * 16;
+        unsigned char* v = smem + Layout<FMT>::v_tiles + (e % ring) * kTileBytes + (lane & 7) * 16;
 #pragma unroll 4
         for (int r = lane >> 3; r < kTile; r += 4) {
             if (!((r >= lo && r <= hi) || (r >= fk && r < pfx))) {
@@ -1118,26 +1119,22 @@ __device__ void mma_role(const Params& p, Misc* mi, unsigned char* smem) {
 // then V_i, K_{i + L} for every tile i. K and V have rings of their own, so
 // that each barrier's phases have one waiter that sees every one of them:
 // a parity says nothing to a waiter that may be two phases behind.
+//
+// One warp copies K (and the queries), one V: a copy takes its warp some 120
+// clocks to issue, and pages of 16 positions mean 16 copies for a tile of each.
 template <int FMT>
-__device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const Maps& maps) {
-    // fp16: a ring of K tiles and one of V tiles; INT8: one ring of code tiles
+__device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const Maps& maps, bool is_v) {
     constexpr int ring = FMT == kF16 ? Layout<FMT>::ring : kRaw;
     const int lane = threadIdx.x & 31;
-    const int subs = kTile >> p.box_shift;  // boxes of a tile: 1 to 8
-    // One instruction issues a V tile's boxes (lower half warp) and a K tile's
-    // (upper half): issued one by one they take the warp 200 clocks each.
-    const bool is_k = lane >= 16;
-    const int sub = FMT == kF16 ? lane >> 1 & 7 : lane & 7;
-    const int part = FMT == kF16 ? lane & 1 : lane >> 3 & 1;  // half of the channels; codes or scales
-    uint32_t n_k = 0, n_v = 0, q_seg = 0;                      // tiles and query loads so far
-    uint32_t thin = 0;                                         // 1 + the last thin segment
-    auto full_of = [&](bool v, uint32_t e) { return FMT == kF16 ? &mi->full[v][e % ring] : &mi->rfull[e % ring]; };
-    auto claim = [&](bool v, uint32_t& e) {  // the next ring entry, once it is free
-        e = FMT != kF16 ? n_k + n_v : v ? n_v : n_k;
-        const uint32_t st = e % ring;
-        ++(v ? n_v : n_k);
-        return e < ring || warp_wait(FMT == kF16 ? &mi->empty[v][st] : &mi->rempty[st], (e / ring - 1) & 1, mi);
-    };
+    const int sub_shift = 7 - p.box_shift, subs = 1 << sub_shift;    // boxes of a tile: 1 to 8
+    const int sub = FMT == kF16 ? lane >> 1 & 7 : lane & 7;          // this lane's box
+    const int part = FMT == kF16 ? lane & 1 : lane >> 3 & 1;         // half of the channels; codes or scales
+    const bool mine = sub < subs && lane < 16;
+    uint32_t pos = 0, q_seg = 0;  // tiles and query loads so far
+    uint32_t thin = 0;            // 1 + the last thin segment
+    uint64_t* const fulls = FMT == kF16 ? mi->full[is_v] : mi->rfull[is_v];
+    uint64_t* const empties = FMT == kF16 ? mi->empty[is_v] : mi->rempty[is_v];
+#pragma unroll 1
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) break;
@@ -1152,7 +1149,6 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
             const int* const table = ks.tables + static_cast<size_t>(g.seq) * ks.width;
             // Pages of 32 boxes (of 32 / subs tiles), one per lane: the page
             // number, -1 if it is none, -2 where nothing is seen.
-            const int sub_shift = 7 - p.box_shift;  // subs = 1 << sub_shift
             auto look = [&](int batch) {
                 const int q = batch * 32 + lane, i = q >> sub_shift;
                 if (i >= n) return -2;
@@ -1171,76 +1167,65 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
                 const int j = tile(t0 + (q >> sub_shift)) * kTile + ((q & (subs - 1)) << p.box_shift);
                 return (page * p.n_kv + head) * p.block_size + j - p.by_block(j) * p.block_size;
             };
-            int batch = -2, ahead = look(0), rows = 0, rows_next = 0;
-            // queries: the last segment's score tiles are done with them
-            if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
-            ++q_seg;
-            if (mode == kWide && thin && k - (thin - 1) < kSegs &&
-                !warp_wait(&mi->segempty[(thin - 1) % kSegs], ((thin - 1) / kSegs) & 1, mi))
-                break;  // a thin segment still uses the second tile's place
-            const int copies = mode == kWide ? 2 : 1, toks = mode == kThin ? p.thin_per : p.per;
-            const CUtensorMap* qm = &maps.q[mode == kThin];
-            if (lane == 0) mbar_arrive_expect_tx(&mi->qfull, static_cast<uint32_t>(copies * toks * p.group * 256));
-            __syncwarp();
-            if (lane < 2 * copies) {
-                const int c = lane >> 1, half = lane & 1;
-                tma_load_3d(smem + c * kTileBytes + half * kHalfTile, qm, half * 64, head * p.group, tok0 + c * toks,
-                            &mi->qfull);
-            }
-            // V of tile iv and K of tile ik (of the list; < 0: none)
-            auto load = [&](int iv, int ik) {
-                uint32_t ev = 0, ek = 0;
-#pragma unroll 1
-                for (int v = 1; v >= 0; --v) {
-                    uint32_t e;
-                    if ((v ? iv : ik) < 0) continue;
-                    if (!claim(v, e)) return false;
-                    (v ? ev : ek) = e;
+            int batch = -1, ahead = look(0), rows = 0;
+            if (!is_v) {
+                // queries: the last segment's score tiles are done with them
+                if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
+                ++q_seg;
+                if (mode == kWide && thin && k - (thin - 1) < kSegs &&
+                    !warp_wait(&mi->segempty[(thin - 1) % kSegs], ((thin - 1) / kSegs) & 1, mi))
+                    break;  // a thin segment still uses the second tile's place
+                const int copies = mode == kWide ? 2 : 1, toks = mode == kThin ? p.thin_per : p.per;
+                if (lane == 0) mbar_arrive_expect_tx(&mi->qfull, static_cast<uint32_t>(copies * toks * p.group * 256));
+                __syncwarp();
+                if (lane < 2 * copies) {
+                    const int c = lane >> 1, half = lane & 1;
+                    tma_load_3d(smem + c * kTileBytes + half * kHalfTile, &maps.q[mode == kThin], half * 64,
+                                head * p.group, tok0 + c * toks, &mi->qfull);
                 }
-                const int q = (is_k ? max(ik, 0) : max(iv, 0)) * subs + sub;
-                const int r0 = __shfl_sync(kFull, rows, q & 31), r1 = __shfl_sync(kFull, rows_next, q & 31);
-                const int row = (q >> 5) == batch ? r0 : r1;
-                const bool mine = sub < subs && (is_k ? ik >= 0 : iv >= 0);
-                const uint32_t e = is_k ? ek : ev;
-                uint64_t* const full = full_of(!is_k, e);
+            }
+            const int L = mode == kWide ? 1 : 2;
+#pragma unroll 1
+            for (int i = -L; i < n; ++i) {
+                const int it = is_v ? i : i + L;  // this warp's tile now
+                if (it < 0 || it >= n) continue;
+                const uint32_t e = pos++;
+                if (it << sub_shift >> 5 != batch) {
+                    ++batch;
+                    rows = place(ahead, batch);
+                    ahead = look(batch + 1);
+                }
                 const uint32_t st = e % ring;
-                const CUtensorMap* map = is_k ? &maps.k : &maps.v;
+                if (e >= ring && !warp_wait(&empties[st], (e / ring - 1) & 1, mi)) {
+                    ok = false;
+                    break;
+                }
+                const int row = __shfl_sync(kFull, rows, ((it << sub_shift) + sub) & 31);
+                uint64_t* const full = &fulls[st];
+                const CUtensorMap* map = is_v ? &maps.v : &maps.k;
                 if (FMT == kF16) {
-                    if ((lane == 0 && iv >= 0) || (lane == 16 && ik >= 0)) mbar_arrive_expect_tx(full, kTileBytes);
+                    if (lane == 0) mbar_arrive_expect_tx(full, kTileBytes);
                     __syncwarp();
                     if (mine)
-                        tma_load_2d(smem + Layout<FMT>::tiles + ((is_k ? 0 : ring) + st) * kTileBytes + part * kHalfTile +
-                                        (sub << p.box_shift) * 128,
+                        tma_load_2d(smem + (is_v ? Layout<FMT>::v_tiles : Layout<FMT>::tiles) + st * kTileBytes +
+                                        part * kHalfTile + (sub << p.box_shift) * 128,
                                     map, part * 64, row, full);
                 } else {
                     const bool there = mine && row != p.total_rows;
-                    const unsigned here = __ballot_sync(kFull, there && part == 0) >> (lane & 16) & 0xffu;
-                    if ((lane == 0 && iv >= 0) || (lane == 16 && ik >= 0)) {
-                        mi->bad[st] = ~here & ((1u << subs) - 1);
+                    const unsigned here = __ballot_sync(kFull, there && part == 0);
+                    if (lane == 0) {
+                        mi->bad[is_v][st] = ~here & ((1u << subs) - 1);
                         mbar_arrive_expect_tx(full, kRawBytes + (__popc(here) << p.box_shift) * 2);
                     }
                     __syncwarp();
                     if (mine && part == 0)
-                        tma_load_2d(smem + Layout<FMT>::raw + st * kRawBytes + (sub << p.box_shift) * kHeadDim, map, 0, row,
+                        tma_load_2d(smem + Layout<FMT>::raw + (is_v * kRaw + st) * kRawBytes + (sub << p.box_shift) * kHeadDim, map, 0, row,
                                     full);
                     if (there && part == 1)
-                        bulk_g2s_plain(smem + Layout<FMT>::raw_scale + st * 256 + (sub << p.box_shift) * 2,
-                                       (is_k ? p.k_scale : p.v_scale) + row, p.box_rows * 2, full);
+                        bulk_g2s_plain(smem + Layout<FMT>::raw_scale + (is_v * kRaw + st) * 256 + (sub << p.box_shift) * 2,
+                                       (is_v ? p.v_scale : p.k_scale) + row, p.box_rows * 2, full);
                 }
                 __syncwarp();
-                return true;
-            };
-            const int L = mode == kWide ? 1 : 2;
-#pragma unroll 1
-            for (int i = -L; ok && i < n; ++i) {
-#pragma unroll 1
-                while (max(i, 0) << sub_shift >> 5 > batch) {  // twice at first: this batch and the next
-                    ++batch;
-                    rows = rows_next;
-                    rows_next = place(ahead, batch + 1);
-                    ahead = look(batch + 2);
-                }
-                ok = load(i, i + L < n ? i + L : -1);
             }
         }
         if (!ok) break;
@@ -1249,16 +1234,8 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
     }
     // Leave no copy in flight: after an abort nobody else waits for them.
     if (*reinterpret_cast<volatile int*>(&mi->abort)) {
-        auto settle = [&](bool v, uint32_t n) {
-            for (uint32_t e = n > ring ? n - ring : 0; e < n; ++e)
-                for (uint32_t i = 0; i < kPolls && !mbar_try_wait(full_of(v, e), (e / ring) & 1); ++i) {}
-        };
-        if (FMT == kF16) {
-            settle(false, n_k);
-            settle(true, n_v);
-        } else {
-            settle(false, n_k + n_v);
-        }
+        for (uint32_t e = pos > ring ? pos - ring : 0; e < pos; ++e)
+            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&fulls[e % ring], (e / ring) & 1); ++i) {}
         if (q_seg > 0)
             for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->qfull, (q_seg - 1) & 1); ++i) {}
     }
@@ -1274,7 +1251,7 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
 // so far, so that weight * scale fits fp16. Rows that no row of the unit sees,
 // and rows of pages that are not there, become zeros with scale zero.
 __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, bool is_v) {
-    constexpr int ring = Layout<kI8>::ring;
+    constexpr uint32_t ring = Layout<kI8>::ring;
     Scales* const scales = reinterpret_cast<Scales*>(smem + Layout<kI8>::scales);
     const int t = threadIdx.x & 127;
     // 16 channels (chunk c) of eight rows. A quarter warp holds chunks of one
@@ -1284,37 +1261,31 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
     const int c = (lane & 3) + (lane >> 1 & 4), turn = lane & 4 ? 5 : 0, x = (c & 3) * 2;
     const int r0 = (t >> 5) * 32 + (lane >> 4);
     auto row_of = [&](int i) { return (r0 + (i >> 1) * 8 + (i & 1) * 2) ^ turn; };
-    uint32_t pos = 0, done = 0;  // code tiles; of this warpgroup's kind
-    int top = 0;                 // V's exponent
+    uint32_t done = 0;  // tiles
+    int top = 0;        // V's exponent
 #pragma unroll 1
     for (uint32_t k = 0;; ++k) {
         const int slot = k % kSegs;
         if (!warp_wait(&mi->segfull[slot], (k / kSegs) & 1, mi)) return;
         const Segment& g = mi->seg[slot];
         if (!g.valid) return;
-        const int t0 = g.t0, n = g.t1 - t0, L = g.mode == kWide ? 1 : 2;
+        const int t0 = g.t0, n = g.t1 - t0;
         const TileList tile(g);
         const int4 range = {g.vlo, g.vhi, g.fk, g.pfx};
         top = -60;
 #pragma unroll 1
-        for (int i = -L; i < n; ++i) {
-            // V of tile i comes first, then K of tile i + L
-            const int mine = is_v ? i : i + L;
-            const bool here = mine >= 0 && mine < n;
-            const uint32_t e = pos + (!is_v && i >= 0);
-            pos += (i >= 0) + (i + L < n);
-            if (!here) continue;
-            const int st = e % kRaw, j0 = tile(t0 + mine) * kTile;
-            if (!warp_wait(&mi->rfull[st], (e / kRaw) & 1, mi)) return;
-            const unsigned char* src = smem + Layout<kI8>::raw + st * kRawBytes;
-            const __half* scale = reinterpret_cast<const __half*>(smem + Layout<kI8>::raw_scale + st * 256);
-            const uint32_t bad = mi->bad[st];
+        for (int i = 0; i < n; ++i) {
+            const uint32_t m = done++;
+            const int st = m % kRaw, j0 = tile(t0 + i) * kTile;
+            if (!warp_wait(&mi->rfull[is_v][st], (m / kRaw) & 1, mi)) return;
+            const unsigned char* src = smem + Layout<kI8>::raw + (is_v * kRaw + st) * kRawBytes;
+            const __half* scale = reinterpret_cast<const __half*>(smem + Layout<kI8>::raw_scale + (is_v * kRaw + st) * 256);
+            const uint32_t bad = mi->bad[is_v][st];
             const int lo = range.x - j0, hi = range.y - j0, fk = range.z - j0, pfx = range.w - j0;
             const bool all = __all_sync(kFull, ((lo <= 0 && hi >= kTile - 1) || (fk <= 0 && pfx >= kTile)) && bad == 0);
             auto seen = [&](int r) {
                 return ((r >= lo && r <= hi) || (r >= fk && r < pfx)) && !((bad >> (r >> p.box_shift)) & 1);
             };
-            const uint32_t m = done++;
             const int at = m % kScales, d = m % ring;
             const bool mine_seen = all || seen(t);
             const float sc = mine_seen ? __half2float(scale[t]) : 0.f;
@@ -1341,9 +1312,9 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
                 const int r = row_of(q);
                 in[q] = *reinterpret_cast<const uint4*>(src + r * kHeadDim + ((c ^ (r & 7)) << 4));
             }
-            warp_arrive(&mi->rempty[st]);
+            warp_arrive(&mi->rempty[is_v][st]);
             if (m >= ring && !warp_wait(&mi->empty[is_v][d], (m / ring - 1) & 1, mi)) return;
-            unsigned char* dst = smem + Layout<kI8>::tiles + ((is_v ? ring : 0) + d) * kTileBytes + (c >> 2) * kHalfTile;
+            unsigned char* dst = smem + (is_v ? Layout<kI8>::v_tiles : Layout<kI8>::tiles) + d * kTileBytes + (c >> 2) * kHalfTile;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 const int r = row_of(q);
@@ -1525,16 +1496,16 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     Misc* mi = reinterpret_cast<Misc*>(smem + Lay::misc);
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
-        const int readers = FMT == kF16 ? 10 : 18;  // warps that read a segment
+        const int readers = FMT == kF16 ? 11 : 19;  // warps that read a segment
         for (int v = 0; v < 2; ++v) {
-            for (int i = 0; i < Lay::ring; ++i) {
+            for (int i = 0; i < kMaxRing; ++i) {
                 mbar_init(&mi->full[v][i], FMT == kF16 ? 1 : 4);
                 mbar_init(&mi->empty[v][i], 1);
             }
         }
-        for (int i = 0; i < kRaw; ++i) {
-            mbar_init(&mi->rfull[i], 1);
-            mbar_init(&mi->rempty[i], 4);
+        for (int i = 0; i < 2 * kRaw; ++i) {
+            mbar_init(&mi->rfull[0][i], 1);
+            mbar_init(&mi->rempty[0][i], 4);
         }
         mbar_init(&mi->qfull, 1);
         mbar_init(&mi->qempty, 1);
@@ -1576,7 +1547,9 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     } else if (warp < 12) {
         regs_dec<Lay::other_regs>();
         if (warp == 8) {
-            copy_role<FMT>(p, mi, smem, maps);
+            copy_role<FMT>(p, mi, smem, maps, false);
+        } else if (warp == 11) {
+            copy_role<FMT>(p, mi, smem, maps, true);
         } else if (warp == 9) {
             mma_role<FMT>(p, mi, smem);
             if (*reinterpret_cast<volatile int*>(&mi->abort)) {  // wait out what is still running

@@ -61,6 +61,12 @@ __device__ __forceinline__ void tmem_ld4(uint32_t addr, float* v) {
                  : "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, float* v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(addr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st4(uint32_t addr, const float* v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                  "f"(v[3])
