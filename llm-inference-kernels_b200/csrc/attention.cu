@@ -170,7 +170,7 @@ struct ThinRow {
 struct ThinSpace {
     unsigned char w[2][kThinRows * 256];  // per stream: weights [2][row][64 positions], swizzled
     float l[2][kThinRows][kTile];         // each thread's part of a row's sum of weights
-    float top[2][4][kThinRows], sum[2][kThinRows], ref[2][kThinRows], down[2][kThinRows], inv[kThinRows];
+    float top[2][4][kThinRows], sum[2][kThinRows], ref[2][kThinRows], down[2][kThinRows], unit[2];
     uint32_t to[kThinRows];
     ThinRow row[kThinRows];
 };
@@ -234,14 +234,15 @@ __device__ __forceinline__ int cu_at(const KeySet& k, int b, int n_tokens) {
     return k.cu ? clampi(k.cu[b], 0, n_tokens) : b;
 }
 
-// The key set and the sequence whose unit numbers include `id`; a sequence
-// whose tokens start at c owns the numbers from c / unit + (its index).
-__device__ __forceinline__ int seq_of(const KeySet& k, int id, Div by_unit, int n_tokens) {
-    if (!k.cu) return id;
-    int lo = 0, hi = k.n_seq - 1;  // largest b with cu[b] / unit + b <= id
+// Unit numbers of a key set: b is the first unit of sequence b; the others of a
+// sequence whose tokens start at c are n_seq + c / unit and following (some
+// numbers are nobody's). The sequence that a number from n_seq on belongs to:
+__device__ __forceinline__ int seq_of(const KeySet& k, int extra, Div by_unit, int n_tokens) {
+    int lo = 0, hi = k.n_seq - 1;  // largest b with cu[b] / unit <= extra
+#pragma unroll 1
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (by_unit(cu_at(k, mid, n_tokens)) + mid <= id) lo = mid; else hi = mid - 1;
+        if (by_unit(cu_at(k, mid, n_tokens)) <= extra) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
@@ -253,11 +254,11 @@ __device__ bool make_unit(const Params& p, int id, Segment& s) {
     if (s.set) id -= p.set[0].n_ids;
     if (k.n_seq <= 0) return false;
     const int unit = 2 * p.per;
-    const int b = seq_of(k, id, p.by_unit, p.n_tokens);
+    const int b = id < k.n_seq ? id : seq_of(k, id - k.n_seq, p.by_unit, p.n_tokens);
     const int c0 = cu_at(k, b, p.n_tokens);
     const int n = k.cu ? cu_at(k, b + 1, p.n_tokens) - c0 : 1;
-    const int at = k.cu ? (id - (p.by_unit(c0) + b)) * unit : 0;
-    if (at < 0 || at >= n) return false;
+    const int at = id < k.n_seq ? 0 : (id - k.n_seq - p.by_unit(c0) + 1) * unit;
+    if (at < 0 || at >= n || (id >= k.n_seq && at == 0)) return false;
     s.seq = b;
     s.tok0 = c0 + at;
     s.ntok = min(unit, n - at);
@@ -296,13 +297,14 @@ __device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
 // tanh on [-0.8, 0.8] as an odd polynomial of degree 9, minimax in the absolute
 // error (3.5e-7): Remez exchange on tanh(t) / t over t^2, weighted by t.
 constexpr float kTanhNear = 0.8f;
-struct TanhNear {  // up tanh(s) for |s| <= 0.8
+struct TanhNear {  // up tanh(in s) for |in s| <= 0.8, the factors folded into the coefficients
     float2 c[5];
-    __device__ __forceinline__ TanhNear(float up) {
+    __device__ __forceinline__ TanhNear(float in, float up) {
         const float k[5] = {0.9999951124191284f, -0.3331742584705353f, 0.13186219334602356f, -0.04826131463050842f,
                             0.01146465539932251f};
+        float f = up * in;
 #pragma unroll
-        for (int i = 0; i < 5; ++i) c[i] = {k[i] * up, k[i] * up};
+        for (int i = 0; i < 5; ++i, f *= in * in) c[i] = {k[i] * f, k[i] * f};
     }
     __device__ __forceinline__ float2 operator()(float2 s) const {
         const float2 y = mul2(s, s);
@@ -398,21 +400,24 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
     for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
     tmem_wait_ld();
     if (MOD) {  // scores to powers of two
-        float far = 0.f;
+        if (I8 || p.cap == 0.f) {
 #pragma unroll
-        for (int i = 0; i < W; i += 4) {
-            const float4 k = I8 ? load_scales(ks + i / 4) : float4{p.kf, p.kf, p.kf, p.kf};
-            const float2 a = mul2({s[i], s[i + 1]}, {k.x, k.y}), b = mul2({s[i + 2], s[i + 3]}, {k.z, k.w});
-            far = max3_abs(max3_abs(far, a.x, a.y), b.x, b.y);
-            s[i] = a.x;
-            s[i + 1] = a.y;
-            s[i + 2] = b.x;
-            s[i + 3] = b.y;
+            for (int i = 0; i < W; i += 4) {
+                const float4 k = I8 ? load_scales(ks + i / 4) : float4{p.kf, p.kf, p.kf, p.kf};
+                const float2 a = mul2({s[i], s[i + 1]}, {k.x, k.y}), b = mul2({s[i + 2], s[i + 3]}, {k.z, k.w});
+                s[i] = a.x;
+                s[i + 1] = a.y;
+                s[i + 2] = b.x;
+                s[i + 3] = b.y;
+            }
         }
         if (p.cap > 0.f) {
-            const float up = p.cap * kLog2e;
-            if (__all_sync(kFull, far <= kTanhNear)) {
-                const TanhNear near(up);
+            const float up = p.cap * kLog2e, in = I8 ? 1.f : p.kf;
+            float far[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < W; i += 2) far[i / 2 & 3] = max3_abs(far[i / 2 & 3], s[i], s[i + 1]);
+            if (__all_sync(kFull, fmaxf(max3(far[0], far[1], far[2]), far[3]) * in <= kTanhNear)) {
+                const TanhNear near(in, up);
 #pragma unroll
                 for (int i = 0; i < W; i += 2) {
                     const float2 t = near({s[i], s[i + 1]});
@@ -464,7 +469,8 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
                 v = c & 1 ? float2{v4.z, v4.w} : float2{v4.x, v4.y};
             }
             float2 x;
-            if (c % 8 == 1 || c % 8 == 4 || c % 8 == 6) {  // 3 of 8 pairs: measured beside 2 and 4
+            // 3 of 8 pairs by the cubic; none where capping has filled its pipe already
+            if (!MOD && (c % 8 == 1 || c % 8 == 4 || c % 8 == 6)) {
                 float2 u;
                 if (I8 && !MOD) {
                     x = fma2({a, b}, k, ms2);
@@ -647,7 +653,7 @@ __device__ __forceinline__ bool stream_sync(Misc* mi, int stream, uint32_t& phas
 template <int FMT, bool MOD>
 __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, const Segment& g, int stream, uint32_t before,
                              uint32_t s_addr, uint32_t o_addr, uint32_t& tiles, uint32_t& tphase, uint32_t& votes,
-                             uint32_t& xphase) {
+                             uint32_t& xphase, bool wide_before) {
     constexpr bool I8 = FMT != kF16;
     constexpr int NT = kThinRows;
     const int r_in = threadIdx.x & 127, lane = threadIdx.x & 31, warp = r_in >> 5;
@@ -795,7 +801,22 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         if (!warp_wait(&mi->odone[stream][1], (tiles - 1) & 1, mi)) return false;
         tcgen05_fence_after();
     }
-    // join the two streams; a thread holds one channel of all rows now
+    if (wide_before && !softmax_sync(mi, xphase)) return false;  // the staging space was the warps' own
+    // Join the two streams; a thread holds one channel of all rows now. Stream
+    // 1 hands its sums over, stream 0 scales both to a row's common reference.
+    float* const other = reinterpret_cast<float*>(smem + Layout<FMT>::stage) + r_in;  // [row][channel]
+    if (stream == 1) {
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += 4) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (any) {
+                tmem_ld4(o_addr + r0, x);
+                tmem_wait_ld();
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) other[(r0 + c) * kHeadDim] = x[c];
+        }
+    }
     if (!stream_sync(mi, stream, tphase)) return false;
 #pragma unroll 1
     for (int r = warp; r < rows; r += 4) {
@@ -805,27 +826,25 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(kFull, t, d);
         if (lane == 0) sp->sum[stream][r] = t;
     }
+    if (r_in == 0) sp->unit[stream] = I8 && any ? fast_exp2(static_cast<float>(ev)) : 1.f;
     if (!softmax_sync(mi, xphase)) return false;
-    if (r_in < rows) {  // each stream's factors, and where the row goes
-        const float m0 = sp->ref[0][r_in], m1 = sp->ref[1][r_in], top = fmaxf(m0, m1);
-        const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
-        sp->down[stream][r_in] = (stream ? a1 : a0) * (I8 && any ? fast_exp2(static_cast<float>(ev)) : 1.f);
-        if (stream == 0) {
+    if (stream == 0) {
+        if (r_in < rows) {
+            const float m0 = sp->ref[0][r_in], m1 = sp->ref[1][r_in], top = fmaxf(m0, m1);
+            const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - top), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - top);
             const float sum = a0 * sp->sum[0][r_in] + a1 * sp->sum[1][r_in];
             const int tl = p.by_group(r_in);
             const uint32_t to = dest_row(p, g, g.tok0 + tl, g.head * p.group + r_in - tl * p.group, r_in);
             store_ml(p, g, to, top, sum);
-            sp->inv[r_in] = sum > 0.f ? 1.f / sum : 0.f;
+            const float inv = g.dest != kDirect ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
+            sp->down[0][r_in] = a0 * sp->unit[0] * inv;
+            sp->down[1][r_in] = a1 * sp->unit[1] * inv;
             sp->to[r_in] = to;
         }
-    }
-    if (!stream_sync(mi, stream, tphase)) return false;
-    float* const other = reinterpret_cast<float*>(smem + Layout<FMT>::stage) + r_in;  // [row][channel]
-    const int dest = g.dest;
+        if (!stream_sync(mi, stream, tphase)) return false;
+        const int dest = g.dest;
 #pragma unroll 1
-    for (int turn = 1; turn >= 0; --turn) {  // stream 1 hands over, stream 0 adds and stores
-#pragma unroll 1
-        for (int r0 = 0; stream == turn && r0 < rows; r0 += 4) {
+        for (int r0 = 0; r0 < rows; r0 += 4) {
             float x[4] = {0.f, 0.f, 0.f, 0.f};
             if (any) {
                 tmem_ld4(o_addr + r0, x);
@@ -835,23 +854,18 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
             for (int c = 0; c < 4; ++c) {
                 const int r = r0 + c;
                 if (r >= rows) break;
-                const float f = sp->down[stream][r];
-                float v = f > 0.f ? x[c] * f : 0.f;
-                if (turn) {
-                    other[r * kHeadDim] = v;
-                    continue;
-                }
-                v += other[r * kHeadDim];
+                const float f0 = sp->down[0][r], f1 = sp->down[1][r];
+                const float v = (f0 > 0.f ? x[c] * f0 : 0.f) + (f1 > 0.f ? other[r * kHeadDim] * f1 : 0.f);
                 const size_t e = static_cast<size_t>(sp->to[r]) * kHeadDim + r_in;
                 if (dest == kDirect)
-                    p.out[e] = __float2half_rn(v * sp->inv[r]);
+                    p.out[e] = __float2half_rn(v);
                 else
                     (dest == kSlot ? p.part : p.rowbuf)[e] = v;
             }
         }
-        if (turn == 0) fence_async_smem();  // queries may be copied over the space that was used here
-        if (!softmax_sync(mi, xphase)) return false;
     }
+    fence_async_smem();  // queries may be copied over the space that was used here
+    if (!softmax_sync(mi, xphase)) return false;
     tcgen05_fence_before();
     return true;
 }
@@ -877,7 +891,8 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
             const uint32_t b = before;
             before += g.t1 - g.t0;
             const bool ok =
-                thin_segment<FMT, MOD>(p, mi, smem, g, stream, b, s_addr, o_addr, tiles, tphase, votes, xphase);
+                thin_segment<FMT, MOD>(p, mi, smem, g, stream, b, s_addr, o_addr, tiles, tphase, votes, xphase,
+                                          wide_before);
             if (!ok) return;
             wide_before = false;
             warp_arrive(&mi->segempty[slot]);
@@ -1387,7 +1402,8 @@ __device__ void plan(const Params& p, Misc* mi) {
     for (int pass = 0; pass < 2; ++pass) {  // add up; then, in the thread that has it, find the CTA's first unit
 #pragma unroll 1
         for (int id = id0; id < id1; ++id) {
-            if (!make_unit(p, id, s)) continue;
+            // with one number per thread the first pass has left it in s
+            if ((pass == 0 || chunk > 1) && !make_unit(p, id, s)) continue;
             const int c = unit_cost(p, s);
             if (pass == 0) {
                 sum += c;
@@ -1653,7 +1669,8 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const __grid_constant__ 
     const int c0 = cu_at(k, lo, p.n_tokens);
     if (k.n_seq > 0 && tok >= c0 && tok < cu_at(k, lo + 1, p.n_tokens)) {
         const int at = (tok - c0) / unit;
-        const int2 u = p.units[static_cast<size_t>(c0 / unit + lo + at) * p.n_kv + h];
+        const int id = at == 0 ? lo : k.n_seq + c0 / unit + at - 1;
+        const int2 u = p.units[static_cast<size_t>(id) * p.n_kv + h];
         if (u.y < 0)
             j.add(p.row_ml, p.rowbuf, row, lane);
         else
@@ -1836,10 +1853,10 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.per = w.per;
     p.thin_per = kThinRows / p.group;
     // clocks measured per tile, in units of 600: wide 2400 (fp16) and 4800
-    // (INT8, converted on the way), paired 1800 and 3000, thin 1800 (what its bytes
-    // take from memory) and 2400; 5400 to start and finish a unit
+    // (INT8, converted on the way), paired 1800 and 3000, thin 2400; 7200 to start
+    // and finish a unit
     const bool int8 = a.fmt != kF16;
-    p.lead = 9;
+    p.lead = 12;
     p.weight[kWide] = int8 ? 8 : 4;
     p.weight[kPaired] = int8 ? 5 : 3;
     p.weight[kThin] = int8 ? 4 : 4;
