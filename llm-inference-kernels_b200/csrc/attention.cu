@@ -312,27 +312,6 @@ struct TanhNear {  // up tanh(in s) for |in s| <= 0.8, the factors folded into t
     }
 };
 
-// 2^x on the multiply-add pipe for x = 64 u - 56, u in [0, 1]: x splits into an
-// integer, added to the exponent, and a rest in [-1/2, 1/2], whose power is a
-// cubic, minimax in the relative error (7.5e-5, Remez exchange); the weights it
-// gives are rounded to fp16 (4.9e-4). The exponential unit alone takes as long
-// for a tile as its matrix instructions, so a part of the weights come from here.
-__device__ __forceinline__ float2 exp2_cubic(float2 u) {
-    constexpr float magic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, kept in the low bits
-    const float2 t = fma2(u, {64.f, 64.f}, {magic - 56.f, magic - 56.f});
-    const float2 back = fma2(t, {-1.f, -1.f}, {magic - 56.f, magic - 56.f});
-    const float2 r = fma2(u, {64.f, 64.f}, back);
-    float2 e = fma2({0.0551716685295105f, 0.0551716685295105f}, r, {0.2426111251115799f, 0.2426111251115799f});
-    e = fma2(e, r, {0.6932609677314758f, 0.6932609677314758f});
-    e = fma2(e, r, {0.9999280571937561f, 0.9999280571937561f});
-    return {__int_as_float(__float_as_int(e.x) + (__float_as_int(t.x) << 23)),
-            __int_as_float(__float_as_int(e.y) + (__float_as_int(t.y) << 23))};
-}
-__device__ __forceinline__ float fma_sat(float a, float b, float c) {
-    float d;
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -450,10 +429,10 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
     const float kf = MOD ? 1.f : p.kf;
 #pragma unroll 1
     for (bool again = false;; again = true) {
-        const float ms = m == -INFINITY ? 0.f : -m, ms_u = (ms + 56.f) * (1.f / 64.f);
+        const float ms = m == -INFINITY ? 0.f : -m;
         const float2 ms2 = {ms, ms};
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-        float over[2] = {-INFINITY, -INFINITY}, full = 0.f;
+        float over[2] = {-INFINITY, -INFINITY};
         uint32_t w[16];
         float4 k4{}, v4{};
 #pragma unroll
@@ -468,30 +447,16 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
                 k = c & 1 ? float2{k4.z, k4.w} : float2{k4.x, k4.y};
                 v = c & 1 ? float2{v4.z, v4.w} : float2{v4.x, v4.y};
             }
-            float2 x;
-            // 3 of 8 pairs by the cubic; none where capping has filled its pipe already
-            if (!MOD && (c % 8 == 1 || c % 8 == 4 || c % 8 == 6)) {
-                float2 u;
-                if (I8 && !MOD) {
-                    x = fma2({a, b}, k, ms2);
-                    u = {fma_sat(x.x, 1.f / 64.f, 56.f / 64.f), fma_sat(x.y, 1.f / 64.f, 56.f / 64.f)};
-                } else {
-                    u = {fma_sat(a, kf * (1.f / 64.f), ms_u), fma_sat(b, kf * (1.f / 64.f), ms_u)};
-                }
-                full = max3(full, u.x, u.y);
-                x = exp2_cubic(u);
-            } else {
-                x = fma2({a, b}, k, ms2);
-                over[c & 1] = max3(over[c & 1], x.x, x.y);
-                x.x = fast_exp2(x.x);
-                x.y = fast_exp2(x.y);
-            }
+            float2 x = MOD ? add2({a, b}, ms2) : fma2({a, b}, k, ms2);
+            over[c & 1] = max3(over[c & 1], x.x, x.y);
+            x.x = fast_exp2(x.x);
+            x.y = fast_exp2(x.y);
             sum[c & 1] = add2(sum[c & 1], x);
             if (I8) x = mul2(x, v);
             w[c % 16] = pack_f16(x.x, x.y);
             if (c % 16 == 15) tmem_st16(p_addr + c - 15, w);
         }
-        const bool low = fmaxf(over[0], over[1]) > kRaise || full >= 1.f || m == -INFINITY;
+        const bool low = fmaxf(over[0], over[1]) > kRaise || m == -INFINITY;
         if (again || !__any_sync(kFull, low || (I8 && v_exp > ev))) {
             const float2 all = add2(sum[0], sum[1]);
             l += all.x + all.y;
@@ -1373,17 +1338,22 @@ __device__ __forceinline__ int unit_cost(const Params& p, const Segment& s) {
 // The units, laid end to end, are split over `ctas` CTAs, the first `more` of
 // which take one more than the others. Each takes at least the heaviest tile's
 // weight, so that from a split unit's first CTA to its last all have a tile of it.
+// x / y; mostly both fit 32 bits, and 64-bit division is a long subroutine
+__device__ __forceinline__ long long divide(long long x, long long y) {
+    if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+    return x / y;
+}
 struct Split {
     long long each, more, ctas;
     __device__ Split(const Params& p, long long total, int heaviest)
-        : ctas(max(min(static_cast<long long>(p.grid), total / max(heaviest, 1)), 1LL)) {
-        each = total / ctas;
+        : ctas(max(min(static_cast<long long>(p.grid), divide(total, max(heaviest, 1))), 1LL)) {
+        each = divide(total, ctas);
         more = total - each * ctas;
     }
     __device__ long long start(long long cta) const { return cta * each + min(cta, more); }
     __device__ int owner(long long x) const {
         const long long edge = more * (each + 1);
-        return static_cast<int>(x < edge ? x / (each + 1) : more + (x - edge) / each);
+        return static_cast<int>(x < edge ? divide(x, each + 1) : more + divide(x - edge, each));
     }
 };
 
@@ -1852,14 +1822,14 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.group = p.n_heads / p.n_kv;
     p.per = w.per;
     p.thin_per = kThinRows / p.group;
-    // clocks measured per tile, in units of 600: wide 2400 (fp16) and 4800
-    // (INT8, converted on the way), paired 1800 and 3000, thin 2400; 7200 to start
-    // and finish a unit
+    // clocks measured per tile, in units of 270: wide 4300 (fp16) and 6500 (INT8,
+    // converted on the way), paired 2500 and 3800, thin 2700 (what its bytes take
+    // from memory) and 3800; 7500 to start and finish a unit
     const bool int8 = a.fmt != kF16;
-    p.lead = 12;
-    p.weight[kWide] = int8 ? 8 : 4;
-    p.weight[kPaired] = int8 ? 5 : 3;
-    p.weight[kThin] = int8 ? 4 : 4;
+    p.lead = 28;
+    p.weight[kWide] = int8 ? 24 : 16;
+    p.weight[kPaired] = int8 ? 14 : 9;
+    p.weight[kThin] = int8 ? 14 : 10;
     p.by_group = make_div(p.group);
     p.by_unit = make_div(w.unit);
     p.by_block = make_div(static_cast<uint32_t>(a.block_size));

@@ -7,8 +7,6 @@ times the softmax scale, n its keys:
   * the weights (times V's scale, in an INT8 cache) are rounded to fp16 once (half
     a step, 2^-11): 2^-11 A, and below 2^-14 by 2^-25 at most, at a largest weight of
     1 or more: n 2^-25 max|v|;
-  * a part of them comes from a cubic for 2^x that is 7.5e-5 off at most: 8e-5 A in
-    the sum of weights times values, as much in the sum of weights;
   * the result is rounded to fp16: 2^-11 |out|;
   * a score is an fp32 sum of 128 exact products in any order (128 2^-24 B),
     scaled, capped and biased by a few fp32 operations (8 2^-23 |score| and the
@@ -103,7 +101,7 @@ def reference(q, k, v, seen, dist, cap=0.0, slopes=None):
         near = near + torch.where(e > 1e-9, slopes.double()[:, None, None] * dist.double(), torch.zeros_like(s)).amax(
             -1, keepdim=True)
     d = 128 * 2.0 ** -24 * B + 8 * 2.0 ** -23 * near + cap * 2.0 ** -20
-    tol = A * (H11 + 2 * 8e-5 + 2 * torch.expm1(d)) + H11 * out.abs() + kk.shape[1] * 2.0 ** -25 * vv.abs().amax() + 1e-7
+    tol = A * (H11 + 2 * torch.expm1(d)) + H11 * out.abs() + kk.shape[1] * 2.0 ** -25 * vv.abs().amax() + 1e-7
     return out.transpose(0, 1), tol.transpose(0, 1)
 
 
