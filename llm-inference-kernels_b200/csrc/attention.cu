@@ -1511,6 +1511,8 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
         mbar_init(&mi->xbar, 8);
         mbar_init(&mi->drain, 1);
         mi->abort = 0;
+        mi->first = Segment{};  // stays so in a CTA without a share
+        mi->start_id = mi->start_head = mi->start_off = 0;
         fence_barrier_init();
         tma_prefetch_map(&maps.k);
         tma_prefetch_map(&maps.v);
