@@ -39,6 +39,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <mutex>
 
 #include "lik_internal.h"
@@ -165,7 +166,8 @@ struct Scales {  // INT8 caches, see convert_role
 // Thin units, in the second query tile's place.
 struct ThinRow {
     int lo, hi, fk;
-    float pos, slope;
+    int pos;
+    float slope;
 };
 struct ThinSpace {
     unsigned char w[2][kThinRows * 256];  // per stream: weights [2][row][64 positions], swizzled
@@ -214,11 +216,11 @@ __device__ __forceinline__ void regs_dec() {
 
 // Whole warp; every lane has observed the phase on return. False: give up
 // (this wait or another one of the CTA ran out; the kernel's end reports it).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Misc* m) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Misc* m, uint32_t polls = kPolls) {
 #pragma unroll 1
     for (uint32_t i = 0;; ++i) {
         if (__all_sync(kFull, mbar_try_wait(bar, parity))) return true;
-        if (i == kPolls) *reinterpret_cast<volatile int*>(&m->abort) = 1;
+        if (i == polls) *reinterpret_cast<volatile int*>(&m->abort) = 1;
         if (*reinterpret_cast<volatile int*>(&m->abort)) return false;
     }
 }
@@ -287,9 +289,12 @@ __device__ bool make_unit(const Params& p, int id, Segment& s) {
 // ---- softmax of one stream -----------------------------------------------------
 
 struct Row {  // what one softmax thread's row sees
-    int lo, hi, fk, pfx;
-    float pos, slope;
+    int lo, hi, fk, pfx, pos;
+    float slope;
 };
+
+// 1 / a row's sum of weights: 0 where it saw nothing; what is not finite stays so.
+__device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 __device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
     return 1.0f - 2.0f * fast_rcp(1.0f + fast_exp2(t * (2.0f * kLog2e)));
@@ -411,7 +416,7 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
             }
         }
         if (p.slopes) {
-            const float from = static_cast<float>(j0) - row.pos;
+            const float from = static_cast<float>(j0 - row.pos);
 #pragma unroll
             for (int i = 0; i < W; ++i) s[i] = fmaf(-row.slope, fabsf(from + static_cast<float>(i)), s[i]);
         }
@@ -628,13 +633,13 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
     const int rows = g.ntok * p.group, pfx = g.pfx;
     if (r_in < NT) {  // both streams write the same
         const int tl = p.by_group(r_in), tok = g.tok0 + tl;
-        ThinRow q = {0, -1, 0, 0.f, 0.f};
+        ThinRow q = {0, -1, 0, 0, 0.f};
         if (r_in < rows) {
             const int pos = ks.extra ? max(ks.extra[tok], 0) + g.ctx - 1 : g.pos0 + tl;
             q.fk = p.first_keys ? max(p.first_keys[tok], 0) : 0;
             q.lo = max(p.window > 0 ? max(pos - p.window + 1, 0) : 0, q.fk);
             q.hi = ks.causal ? min(pos, g.ctx - 1) : g.ctx - 1;
-            q.pos = static_cast<float>(pos);
+            q.pos = pos;
             if (MOD && p.slopes) q.slope = p.slopes[g.head * p.group + r_in - tl * p.group] * kLog2e;
         }
         sp->row[r_in] = q;
@@ -684,7 +689,7 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
                 x[c] *= kx;
                 if (MOD && p.cap > 0.f) x[c] = p.cap * kLog2e * tanh_exp(x[c]);
                 if (MOD && p.slopes)
-                    x[c] = fmaf(-sp->row[r0 + c].slope, fabsf(static_cast<float>(j) - sp->row[r0 + c].pos), x[c]);
+                    x[c] = fmaf(-sp->row[r0 + c].slope, fabsf(static_cast<float>(j - sp->row[r0 + c].pos)), x[c]);
                 if (!whole || r0 + c >= rows) {
                     const ThinRow& q = sp->row[r0 + c];
                     if (!((j >= q.lo && j <= q.hi) || (j >= q.fk && j < pfx && r0 + c < rows))) x[c] = -INFINITY;
@@ -801,7 +806,7 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
             const int tl = p.by_group(r_in);
             const uint32_t to = dest_row(p, g, g.tok0 + tl, g.head * p.group + r_in - tl * p.group, r_in);
             store_ml(p, g, to, top, sum);
-            const float inv = g.dest != kDirect ? 1.f : sum > 0.f ? 1.f / sum : 0.f;
+            const float inv = g.dest != kDirect ? 1.f : over_sum(sum);
             sp->down[0][r_in] = a0 * sp->unit[0] * inv;
             sp->down[1][r_in] = a1 * sp->unit[1] * inv;
             sp->to[r_in] = to;
@@ -820,7 +825,7 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
                 const int r = r0 + c;
                 if (r >= rows) break;
                 const float f0 = sp->down[0][r], f1 = sp->down[1][r];
-                const float v = (f0 > 0.f ? x[c] * f0 : 0.f) + (f1 > 0.f ? other[r * kHeadDim] * f1 : 0.f);
+                const float v = (f0 != 0.f ? x[c] * f0 : 0.f) + (f1 != 0.f ? other[r * kHeadDim] * f1 : 0.f);
                 const size_t e = static_cast<size_t>(sp->to[r]) * kHeadDim + r_in;
                 if (dest == kDirect)
                     p.out[e] = __float2half_rn(v);
@@ -869,14 +874,14 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
         const int tl = tl0 + (wide ? stream * p.per : 0);
         const bool live = tl < g.ntok && tl0 < p.per;
         const int tok = g.tok0 + tl;
-        Row row{0, 0x7fffffff, 0, 0, 0.f, 0.f};  // a row that is not live keeps every column: nothing reads it
+        Row row{0, 0x7fffffff, 0, 0, 0, 0.f};  // a row that is not live keeps every column: nothing reads it
         if (live) {
             const int pos = g.pos0 + tl + (ks.extra ? max(ks.extra[tok], 0) + g.ctx - 1 - (g.pos0 + tl) : 0);
             row.fk = p.first_keys ? max(p.first_keys[tok], 0) : 0;
             row.lo = max(p.window > 0 ? max(pos - p.window + 1, 0) : 0, row.fk);
             row.hi = ks.causal ? min(pos, g.ctx - 1) : g.ctx - 1;
             row.pfx = g.pfx;
-            row.pos = static_cast<float>(pos);
+            row.pos = pos;
             if (MOD && p.slopes) row.slope = p.slopes[hr] * kLog2e;
         }
         float m = -INFINITY, l = 0.f;
@@ -889,14 +894,14 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
             if (!warp_wait(&mi->odone[stream][1], (tiles - 1) & 1, mi)) return;
             tcgen05_fence_after();
         }
-        if (m == -INFINITY) l = 0.f;
-        const float m2 = l > 0.f ? m : -INFINITY;
+        // l is 0 for a row that saw nothing, NaN if a score was
+        const float m2 = l == 0.f ? -INFINITY : fmaxf(m, -FLT_MAX);
         if (wide) {
             const uint32_t row_at = live ? dest_row(p, g, tok, hr, tl * p.group + hr - g.head * p.group) : ~0u;
             if (live) store_ml(p, g, row_at, m2, l);
             if (g.dest == kDirect)
                 store_wide<FMT, true>(stage, reinterpret_cast<unsigned char*>(p.out), o_addr, mine > 0, row_at,
-                                      l > 0.f ? unit_v / l : 0.f);
+                                      unit_v * over_sum(l));
             else
                 store_wide<FMT, false>(stage, reinterpret_cast<unsigned char*>(g.dest == kSlot ? p.part : p.rowbuf),
                                        o_addr, mine > 0, row_at, unit_v);
@@ -959,7 +964,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
                     if (d0 == 0 && c4 == 0) store_ml(p, g, at, mx, sum);
                     const size_t e = static_cast<size_t>(at) * kHeadDim + d0 + 4 * c4;
                     if (g.dest == kDirect) {
-                        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                        const float inv = over_sum(sum);
                         *reinterpret_cast<uint2*>(p.out + e) = {pack_f16(v.x * inv, v.y * inv), pack_f16(v.z * inv, v.w * inv)};
                     } else {
                         *reinterpret_cast<float4*>((g.dest == kSlot ? p.part : p.rowbuf) + e) = v;
@@ -1379,10 +1384,10 @@ __device__ void plan(const Params& p, Misc* mi) {
                 sum += c;
                 heaviest = max(heaviest, p.weight[s.mode]);
             } else if (a - at < static_cast<long long>(c) * p.n_kv) {
-                const uint32_t rest = static_cast<uint32_t>(a - at);
+                const long long rest = a - at;
                 mi->start_id = id;
-                mi->start_head = rest / c;
-                mi->start_off = rest % c;
+                mi->start_head = static_cast<int>(divide(rest, c));
+                mi->start_off = static_cast<int>(rest - static_cast<long long>(mi->start_head) * c);
                 mi->first = s;
                 break;
             } else {
@@ -1443,7 +1448,8 @@ __device__ void schedule_role(const Params& p, Misc* mi) {
         const bool last = left <= 0;
         if (last || t1 > t0) {
             const bool whole = t0 == 0 && t1 == tiles;
-            if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi)) break;
+            // a whole segment may pass, seconds for one over millions of keys
+            if (k >= kSegs && !warp_wait(&mi->segempty[slot], (k / kSegs - 1) & 1, mi, kPolls * 64)) break;
             if (lane == 0) {
                 s.valid = !last;
                 s.head = head;
@@ -1571,7 +1577,7 @@ struct Join {
     float4 v = {0.f, 0.f, 0.f, 0.f};
     __device__ void add(const float2* ml, const float* part, size_t r, int lane) {
         const float2 e = ml[r];
-        if (e.y <= 0.f) return;
+        if (e.y == 0.f) return;
         const float4 o = *reinterpret_cast<const float4*>(part + r * kHeadDim + lane * 4);
         const float up = fmaxf(m, e.x);
         const float a = m == -INFINITY ? 0.f : fast_exp2(m - up), b = fast_exp2(e.x - up);
@@ -1587,7 +1593,7 @@ struct Join {
             add(p.part_ml, p.part, static_cast<size_t>(2 * c + (c == first)) * p.slot_rows + unit_row, lane);
     }
     __device__ void store(const Params& p, size_t row, int lane) {
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = over_sum(l);
         uint2 u;
         u.x = pack_f16(v.x * inv, v.y * inv);
         u.y = pack_f16(v.z * inv, v.w * inv);

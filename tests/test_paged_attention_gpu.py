@@ -206,6 +206,54 @@ def test_rows_that_see_nothing_and_empty_sequences(L, kv):
 
 
 @pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("nq,ctx", [(1, 300), (1, 30000), (3, 500), (20, 500), (20, 9000), (64, 700), (300, 5000)])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_a_query_that_is_not_finite_is_its_own_rows_matter(L, kv, nq, ctx, what):
+    H, Hkv, bad_head = 8, 2, 5
+    g = torch.Generator().manual_seed(nq + ctx)
+    pool = Pool(g, kv, -(-ctx // 64) + 1, Hkv, 64)
+    table = pool.give([ctx])
+    q = rand(g, nq, H, 128)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    run = lambda x: L.paged_attention(x, pool.cache["k"], pool.cache["v"], table, i32([ctx]), i32([0, nq]), SCALE,  # noqa: E731
+                                      **pool.args())
+    dirty = q.clone()
+    dirty[nq // 2, bad_head, 7] = what
+    got = run(dirty)
+    assert torch.isnan(got[nq // 2, bad_head]).all()
+    p = torch.arange(ctx - nq, ctx, device="cuda")[:, None]
+    seen = torch.arange(ctx, device="cuda")[None] <= p
+    ref, tol = reference(q, pool.rows("k", table[0], ctx), pool.rows("v", table[0], ctx), seen, None)
+    others = torch.ones(nq, H, dtype=torch.bool, device="cuda")
+    others[nq // 2, bad_head] = False
+    check(got[others], ref[others], tol[others])
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("nq", [1, 20, 64])
+def test_distances_stay_exact_far_out(L, kv, nq):
+    """Past 2^24 positions a position is no fp32 number; the distances that count are."""
+    ctx, bs, width = (1 << 24) + 9 * 128 + 3, 128, (1 << 17) + 10
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, kv, 12, 1, bs)
+    near = pool.give([10 * bs - 125])[0]                  # the last ten pages hold the last 1155 positions
+    assert (ctx - 1) // bs - 9 == width - 10
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    table[0, width - 10:] = near
+    m = 9 * bs + 3
+    q = rand(g, nq, 2, 128)
+    slopes = torch.tensor([0.5, 0.03], device="cuda")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([ctx]), i32([0, nq]), SCALE, window=900,
+                            alibi_slopes=slopes, **pool.args())
+    p = torch.arange(m - nq, m, device="cuda")[:, None]
+    j = torch.arange(m, device="cuda")[None]
+    ref, tol = reference(q, pool.rows("k", near, m), pool.rows("v", near, m), (j <= p) & (j > p - 900), (p - j).abs(),
+                         slopes=slopes)
+    check(got, ref, tol)
+
+
+@pytest.mark.parametrize("kv", KV)
 def test_rows_of_no_sequence(L, kv):
     got, cu = run_case(L, kv, 8, 2, [5, 70], [50, 70], 16, lead=3, pad=4)
     assert (got[:3] == 0).all() and (got[-4:] == 0).all()
