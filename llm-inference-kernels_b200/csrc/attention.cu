@@ -22,7 +22,7 @@
 //     key tile;
 //   paired units (up to 128 rows): both streams hold the same rows and take
 //     alternate key tiles, their states are joined at the unit's end;
-//   thin units (up to 32 rows, single tokens among them): paired, and with the
+//   thin units (up to 16 rows, single tokens among them): paired, and with the
 //     operands exchanged, scores [position][row] = K q^T and sums
 //     [channel][row] = V^T w^T, so that few rows mean a small matrix product
 //     instead of a padded one and a tile's softmax is one position per thread.
@@ -33,8 +33,23 @@
 //
 // fp16 caches go from the pool to swizzled shared memory by tensor-map copies,
 // one box per run of positions inside a page. INT8 caches arrive as codes and
-// scales; four more warps write the codes as fp16 integers into the same
-// swizzled tiles, and the softmax applies the scales in fp32.
+// scales; two more warpgroups, one for K and one for V, write the codes as fp16
+// integers into the same swizzled tiles, and the softmax applies the scales in
+// fp32.
+//
+// What bounds it, measured (32 query heads on 8 KV heads; warps 0-7 softmax, 8
+// copies of K and q, 9 matrix instructions, 10 schedule, 11 copies of V):
+//   wide, 4096 causal tokens: the softmax. 154 us in fp16, 894 TFLOP/s, the
+//     tensor pipe busy half of the time; a tile's two steps take 4300 clocks, of
+//     which the exponentials alone are 2048 (32768 of them, 16 per clock on an SM).
+//     Capped scores 252 us (the polynomial), INT8 215 (scales, and one tile of K
+//     and of V in place of two);
+//   thin, 16 requests of 8192: memory. 93 us in fp16, 5.8 TB/s. INT8 103 us: its
+//     codes pass shared memory four times (copied in, read, written as fp16, read
+//     by the matrix unit), 1500 of a tile's 3200 clocks;
+//   a few tiles per CTA: the way there. 13 us for one request of 512: finding
+//     the share 5000 clocks, the first copies 3000, the unit's end 2500, and the
+//     joining kernel.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -1869,7 +1884,7 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
             continue;
         }
         const cuuint64_t dims[3] = {kHeadDim, static_cast<cuuint64_t>(a.n_heads), static_cast<cuuint64_t>(a.n_tokens)};
-        const cuuint64_t strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(a.q_token_stride) * 2};
+        const cuuint64_t strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(a.n_tokens > 1 ? a.q_token_stride : a.n_heads * kHeadDim) * 2};
         const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(toks)};
         if (!encode(&maps.q[i], CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, a.q, dims, strides, box, true, err)) return LIK_ERR_CUDA;
     }

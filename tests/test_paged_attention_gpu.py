@@ -395,6 +395,22 @@ def test_bad_table_entries_are_reported_and_read_as_zeros(L, kv):
                                   seen[:, :150].long()))
 
 
+def test_an_error_on_another_stream_is_reported(L):
+    g = torch.Generator().manual_seed(5)
+    pool = Pool(g, "fp16", 8, 1, 16)
+    table = pool.give([100])
+    table[0, 2] = 1 << 20
+    q = rand(g, 1, 4, 128)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    ctx, cu = i32([100]), i32([0, 1])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, ctx, cu, SCALE)
+    with pytest.raises(RuntimeError):
+        L.check_device_errors()
+    L.check_device_errors()
+
+
 def test_offsets_that_do_not_ascend_stay_in_bounds(L):
     """Token offsets and lengths out of range are clamped: no access outside the tensors, other rows unharmed."""
     g = torch.Generator().manual_seed(7)
