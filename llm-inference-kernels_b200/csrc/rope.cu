@@ -16,7 +16,7 @@
 // Bound by memory: every row is read and written once. One block holds 32 rows
 // (heads) of 128 channels of a token, or of a few tokens, an 8-lane group each;
 // its first threads work out the tokens' cosines and sines while the rows arrive.
-// 8192 tokens of 32 + 8 + 8 heads into fp16 caches take 39 us (5.1 TB/s), 2047
+// 8192 tokens of 32 + 8 + 8 heads into fp16 caches take 36 us (5.6 TB/s), 2047
 // into INT8 21 us, where a row's maximum is waited for before its codes; 8
 // tokens 1.9 us on the GPU, less than their launch takes the host.
 // Angles take a 64-bit product and range reduction: positions of 10^5 and more
@@ -87,6 +87,15 @@ __device__ __forceinline__ void store_cache_row(int format, const Raw16& raw, lo
     }
 }
 
+// Where frequency f's cosine and sine lie: lane l reads those of 8 l .. 8 l + 7 two
+// at a time, and the eight lanes' reads then fill one run of 128 bytes (8192
+// tokens: 35.8 us; 39.3 with them in order, where half the banks' reads collided).
+// kHalvesAny reads them one by one.
+template <int PAIRS>
+__device__ __forceinline__ int turn_at(int f) {
+    return PAIRS == kHalvesAny ? f : (f & 6) * 8 + (f >> 3) * 2 + (f & 1);
+}
+
 // PAIRS kHalves: the frequencies fill whole 16-byte chunks (r a multiple of
 // 8), so lane l < r / 8 holds chunks l and l + r / 8, both halves of its pairs;
 // the other lanes hold the chunks that pass. kHalvesAny (any r) and
@@ -95,7 +104,7 @@ __device__ __forceinline__ void store_cache_row(int format, const Raw16& raw, lo
 // one only where both caches are fp16.
 template <int PAIRS, int TOK>
 __global__ void __launch_bounds__(256, TOK == 1 ? 8 : 6) rope_append_kernel(const __grid_constant__ RopeParams p) {
-    __shared__ float2 turn[TOK][kMaxFreqs];  // cosine, sine
+    __shared__ __align__(16) float2 turn[TOK][kMaxFreqs];  // cosine, sine; see turn_at
     const long long tok0 = static_cast<long long>(blockIdx.x) * TOK;
     const int l = threadIdx.x & 7;
     const unsigned mask = 0xFFu << (threadIdx.x & 24);
@@ -129,7 +138,7 @@ __global__ void __launch_bounds__(256, TOK == 1 ? 8 : 6) rope_append_kernel(cons
                                  static_cast<double>(p.inv_freq[f]) * per_turn;
             float s, co;
             sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &co);
-            turn[t][f] = {co, s};
+            turn[t][turn_at<PAIRS>(f)] = {co, s};
         }
     }
     __syncthreads();
@@ -146,13 +155,19 @@ __global__ void __launch_bounds__(256, TOK == 1 ? 8 : 6) rope_append_kernel(cons
             if (PAIRS == kHalves) {
                 if (l < c) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) rotate2(a[i], b[i], cs[8 * l + 2 * i], cs[8 * l + 2 * i + 1]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 u = *reinterpret_cast<const float4*>(cs + turn_at<PAIRS>(8 * l + 2 * i));
+                        rotate2(a[i], b[i], {u.x, u.y}, {u.z, u.w});
+                    }
                 }
             } else if (PAIRS == kNeighbours) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (8 * l + i < p.freqs) a[i] = rotate1(a[i], cs[8 * l + i]);
-                    if (8 * l + 4 + i < p.freqs) b[i] = rotate1(b[i], cs[8 * l + 4 + i]);
+                    const float4 u = *reinterpret_cast<const float4*>(cs + turn_at<PAIRS>(8 * l + 2 * i));
+                    uint32_t& x = i < 2 ? a[2 * i] : b[2 * i - 4];
+                    uint32_t& y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+                    if (8 * l + 2 * i < p.freqs) x = rotate1(x, {u.x, u.y});
+                    if (8 * l + 2 * i + 1 < p.freqs) y = rotate1(y, {u.z, u.w});
                 }
             } else {
                 // a pair's other channel sits in another lane: read it once more
@@ -166,7 +181,7 @@ __global__ void __launch_bounds__(256, TOK == 1 ? 8 : 6) rope_append_kernel(cons
                         const bool first = ch < p.freqs;
                         const float x = __half2float(h[i]);
                         const float y = __half2float(row_at[first ? ch + p.freqs : ch - p.freqs]);
-                        const float2 u = cs[first ? ch : ch - p.freqs];
+                        const float2 u = cs[turn_at<PAIRS>(first ? ch : ch - p.freqs)];
                         h[i] = __float2half_rn(first ? __fsub_rn(__fmul_rn(x, u.x), __fmul_rn(y, u.y))
                                                      : __fadd_rn(__fmul_rn(x, u.x), __fmul_rn(y, u.y)));
                     }
@@ -227,9 +242,9 @@ void launch_tokens(const RopeParams& p, cudaStream_t stream) {
 
 // kTokens tokens per block keep more rows in flight. It pays where the work is
 // copying and there are tokens enough for every SM: 32 + 8 + 8 heads, fp16
-// caches, 37.3 instead of 41.3 us for 8000 tokens (5.3 TB/s), 20.9 instead of
-// 21.5 for 4000, the same for 2000 and fewer. Two tokens or four were slower
-// (39.4, 38.5). Rows that are quantized wait for their reductions, one token
+// caches, 35.3 instead of 37.3 us for 8000 tokens, 17.3 instead of 18.8 for
+// 4000, the same for 2000 and fewer. Two tokens were slower (36.0), and four for
+// 4000 tokens (18.8). Rows that are quantized wait for their reductions, one token
 // after the other: 8000 tokens into INT8 took 76 us with four tokens per block
 // and 67 with one (55.9 with the registers held to 32, eight blocks on an SM).
 template <int PAIRS>
