@@ -49,6 +49,11 @@ CASES = [
     (50, 5, 5, 1, None, False, 16),
     (29, 16, 16, 8, [2, 2, 2, 2], False, 1),
     (300, 71, 1, 48, [0, 48], False, 128),
+    # enough rows for several tokens per block, the last block short or full
+    (3199, 40, 8, 64, [16, 24, 24], False, 64),
+    (3200, 40, 8, 24, None, False, 16),
+    (3201, 40, 8, 31, None, True, 48),
+    (3200, 40, 8, 31, None, False, 48),
 ]
 
 
@@ -126,3 +131,27 @@ def test_captured_append_replays_with_other_positions(L):
     assert torch.equal(out, want)
     live = slots[slots >= 0]
     assert torch.equal(cache[live // 16, :, live % 16], c2[live // 16, :, live % 16])
+
+
+@pytest.mark.parametrize("n,r,interleaved", [(5, 64, False), (5, 31, True), (5, 31, False), (3200, 64, False),
+                                             (3200, 24, False), (3200, 31, True), (3200, 31, False)])
+def test_queries_rotated_in_place(L, n, r, interleaved):
+    import ctypes
+
+    from llmik_cuda import cabi
+    lib = cabi.lib()
+    g = torch.Generator().manual_seed(n + r)
+    q, k = torch.randn(n, 40, 128, generator=g).half().cuda(), torch.randn(n, 8, 128, generator=g).half().cuda()
+    pos, slots = torch.randint(0, 100000, (n,), generator=g).cuda(), torch.arange(n).cuda()
+    inv = (10000.0 ** (-torch.arange(r).double() / r)).float().cuda()
+    blocks = -(-n // 16)
+    caches = [torch.zeros(blocks, 8, 16, 128, dtype=torch.float16, device="cuda") for _ in range(4)]
+    want = L.paged_append_rope(q, k, k, pos, inv, slots, caches[0], caches[1], interleaved=interleaved)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    torch.cuda.synchronize()
+    st = lib.lik_paged_append_rope(0, 0, p(q), 40 * 128, p(k), 8 * 128, p(k), 8 * 128, p(pos), 1, None, p(inv), r,
+                                   int(interleaved), p(slots), p(q), n, 40, 8, 128, p(caches[2]), None, p(caches[3]),
+                                   None, None, blocks, 16, None)
+    torch.cuda.synchronize()
+    assert st == 0
+    assert torch.equal(q, want) and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
