@@ -573,7 +573,7 @@ lik_status lik_attention_shared_prefix(int kv_format, const void* q, int64_t q_t
                                        float softmax_scale, float softcap, const float* alibi_slopes, void* workspace,
                                        size_t workspace_bytes, void* stream) {
     if (n_groups < 1 && batch > 0) return fail(LIK_ERR_INVALID_ARGUMENT, "need at least one prefix group");
-    if (batch > 0 && (!prefix_tables || !prefix_lens || !block_tables || !context_lens))
+    if (batch > 0 && (!prefix_tables || !prefix_lens || (max_blocks_per_seq > 0 && !block_tables) || !context_lens))
         return fail(LIK_ERR_INVALID_ARGUMENT, "null block table or lengths");
     AttentionArgs a;
     a.fmt = kv_format;

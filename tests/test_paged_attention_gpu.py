@@ -491,6 +491,22 @@ def test_shared_prefix_equals_attention_over_joined_tables(L):
     assert ((a.float() - b.float()).abs() <= 2 * (2 * H11 * k)).all()
 
 
+def test_shared_prefix_without_own_pages(L):
+    """Own tables of no columns: every request has its group's prefix alone."""
+    g = torch.Generator().manual_seed(8)
+    pool = Pool(g, "fp16", 20, 2, 16)
+    pt = pool.give([200, 31])
+    q = rand(g, 5, 8, 128)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    run = lambda own, lens: L.paged_shared_prefix_attention(  # noqa: E731
+        q, pool.cache["k"], pool.cache["v"], pt, i32([200, 31]), i32([0, 3, 5]), own, i32(lens), SCALE)
+    none = torch.empty(5, 0, dtype=torch.int32, device="cuda")
+    want = run(torch.zeros(5, 1, dtype=torch.int32, device="cuda"), [0] * 5)
+    assert torch.isfinite(want).all() and want.abs().sum() > 0
+    assert torch.equal(run(none, [0] * 5), want)
+    assert torch.equal(run(none, [7] * 5)[:3].isfinite(), want[:3].isfinite())   # lengths are cut to the tables
+
+
 # ---------------------------------------------------------------- a serving step
 
 def test_append_prompt_and_decode_together(L):
