@@ -1600,12 +1600,41 @@ struct Join {
         l = l * a + e.y * b;
         v = {v.x * a + o.x * b, v.y * a + o.y * b, v.z * a + o.z * b, v.w * a + o.w * b};
     }
+    // The partial states of a unit's row in the CTAs first .. last. A lane reads
+    // one CTA's state, then the sums come four at a time: one after the other, each
+    // behind its state, they took 2 us per CTA for a unit that 18 CTAs share.
     // A CTA that gave up (a wait ran out) may have left its entries unwritten:
     // what is out of range is left out, and the error word has told.
     __device__ void add_slots(const Params& p, int first, int last, int unit_row, int lane) {
         if (first < 0 || last >= p.grid || unit_row >= p.slot_rows) return;
-        for (int c = first; c <= last; ++c)
-            add(p.part_ml, p.part, static_cast<size_t>(2 * c + (c == first)) * p.slot_rows + unit_row, lane);
+        auto slot = [&](int c) { return static_cast<size_t>(2 * c + (c == first)) * p.slot_rows + unit_row; };
+        for (int c0 = first; c0 <= last; c0 += 32) {
+            const int n = min(32, last - c0 + 1);
+            const float2 e = lane < n ? p.part_ml[slot(c0 + lane)] : float2{-INFINITY, 0.f};
+            float up = e.y == 0.f ? -INFINITY : e.x, sum;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) up = fmaxf(up, __shfl_xor_sync(kFull, up, d));
+            up = fmaxf(up, m);
+            const float a = m == -INFINITY ? 0.f : fast_exp2(m - up), f = e.y == 0.f ? 0.f : fast_exp2(e.x - up);
+            sum = e.y * f;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+            m = up;
+            l = l * a + sum;
+            v = {v.x * a, v.y * a, v.z * a, v.w * a};
+            for (int i = 0; i < n; i += 4) {
+                float4 o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    o[k] = *reinterpret_cast<const float4*>(p.part + slot(c0 + min(i + k, n - 1)) * kHeadDim + lane * 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float b = __shfl_sync(kFull, f, (i + k) & 31);
+                    if (i + k < n && b != 0.f)
+                        v = {v.x + o[k].x * b, v.y + o[k].y * b, v.z + o[k].z * b, v.w + o[k].w * b};
+                }
+            }
+        }
     }
     __device__ void store(const Params& p, size_t row, int lane) {
         const float inv = over_sum(l);
