@@ -1602,7 +1602,7 @@ struct Join {
     }
     // The partial states of a unit's row in the CTAs first .. last. A lane reads
     // one CTA's state, then the sums come four at a time: one after the other, each
-    // behind its state, they took 2 us per CTA for a unit that 18 CTAs share.
+    // behind its state, a unit that 18 CTAs share took 53 us in place of 32.
     // A CTA that gave up (a wait ran out) may have left its entries unwritten:
     // what is out of range is left out, and the error word has told.
     __device__ void add_slots(const Params& p, int first, int last, int unit_row, int lane) {
@@ -1811,7 +1811,9 @@ lik_status launch(const Maps& maps, const Params& p, cudaStream_t stream, std::s
                 cfg.gridDim = dim3(static_cast<unsigned>((rows + 7) / 8));
                 e = cudaLaunchKernelEx(&cfg, join_rows_kernel, p);
             } else {
-                cfg.gridDim = dim3(p.grid, static_cast<unsigned>((p.slot_rows + 31) / 32));
+                // two rows per warp: four took 32 us in place of 27 for 42 tokens over 1798
+                // keys, one 161 us in place of 153 for a prompt of 4096 (blocks with nothing to do)
+                cfg.gridDim = dim3(p.grid, static_cast<unsigned>((p.slot_rows + 15) / 16));
                 e = cudaLaunchKernelEx(&cfg, join_split_kernel, p);
             }
         }
