@@ -111,7 +111,7 @@ struct KeySet {
 
 struct Params {
     KeySet set[2];
-    int n_sets;
+    int n_sets, extra_most;  // `extra` counts up to extra_most: the lengths are cut to their tables
     const int* prefix_lens;
     const int* first_keys;
     const float* slopes;
@@ -650,7 +650,7 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         const int tl = p.by_group(r_in), tok = g.tok0 + tl;
         ThinRow q = {0, -1, 0, 0, 0.f};
         if (r_in < rows) {
-            const int pos = ks.extra ? max(ks.extra[tok], 0) + g.ctx - 1 : g.pos0 + tl;
+            const int pos = ks.extra ? clampi(ks.extra[tok], 0, p.extra_most) + g.ctx - 1 : g.pos0 + tl;
             q.fk = p.first_keys ? max(p.first_keys[tok], 0) : 0;
             q.lo = max(p.window > 0 ? max(pos - p.window + 1, 0) : 0, q.fk);
             q.hi = ks.causal ? min(pos, g.ctx - 1) : g.ctx - 1;
@@ -891,7 +891,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
         const int tok = g.tok0 + tl;
         Row row{0, 0x7fffffff, 0, 0, 0, 0.f};  // a row that is not live keeps every column: nothing reads it
         if (live) {
-            const int pos = g.pos0 + tl + (ks.extra ? max(ks.extra[tok], 0) + g.ctx - 1 - (g.pos0 + tl) : 0);
+            const int pos = ks.extra ? clampi(ks.extra[tok], 0, p.extra_most) + g.ctx - 1 : g.pos0 + tl;
             row.fk = p.first_keys ? max(p.first_keys[tok], 0) : 0;
             row.lo = max(p.window > 0 ? max(pos - p.window + 1, 0) : 0, row.fk);
             row.hi = ks.causal ? min(pos, g.ctx - 1) : g.ctx - 1;
@@ -1859,6 +1859,7 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
         p.set[1] = {nullptr, a.context_lens, a.block_tables, nullptr, static_cast<int>(a.n_tokens),
                     static_cast<int>(a.max_blocks), w.n_ids1, 0};
         p.n_sets = 2;
+        p.extra_most = static_cast<int>(a.max_blocks * a.block_size);
     } else {
         p.set[0] = {a.cu_seqlens, a.context_lens, a.block_tables, nullptr, static_cast<int>(a.n_seqs),
                     static_cast<int>(a.max_blocks), w.n_ids0, a.causal ? 1 : 0};
