@@ -78,9 +78,14 @@ constexpr int kSegs = 4;
 constexpr int kThinRows = 16;
 constexpr uint32_t kTmem = 0;                    // first column of tensor memory
 constexpr float kLog2e = 1.4426950408889634f;
-// The running maximum is raised only past this many powers of two, so most
-// tiles leave the accumulator alone; weights stay below 2^8 in fp16.
-constexpr float kRaise = 8.0f;
+// The reference of a row's weights is put kLift powers of two below its maximum
+// and raised only where a score lies more than kRaise above it, so most tiles
+// leave the accumulator alone. In fp16 the weights then reach from 2^15 down: a
+// row's largest is 2^7 or more, what lies 2^-21 below it and less is subnormal and
+// loses 2^-32 of the largest at most (2^-25 with the reference at the maximum,
+// where 32768 keys of weight 2^-25.5 vanished altogether).
+constexpr float kLift = 7.0f;
+constexpr float kRaise = 15.0f;
 constexpr uint32_t kPolls = 1u << 18;            // a poll sleeps for a few microseconds at most
 
 enum Mode : int { kWide = 0, kPaired = 1, kThin = 2 };
@@ -381,10 +386,10 @@ __device__ __forceinline__ void cap_far(float up, float kf, uint32_t s_addr, con
 // One step: the softmax of W score columns at s_addr, keys from j0, into W fp16
 // weights at p_addr. `m` is the row's reference, in powers of two. The weights
 // are worked out with the reference so far; only where a score turns out to lie
-// more than 2^8 above it (in the first step of a unit, rarely later) the
-// maximum is searched for, the reference raised to it and the weights worked
-// out again. Searched for ahead of the weights it held up every step by a
-// quarter. Weights stay below 2^8, which fp16 holds.
+// more than 2^kRaise above it (in the first step of a unit, rarely later) the
+// maximum is searched for, the reference raised and the weights worked out
+// again. Searched for ahead of the weights it held up every step by a quarter.
+// Weights stay below 2^15, which fp16 holds.
 //
 // INT8: ks holds kf times K's scales, vs V's scales divided by 2^v_exp, the
 // largest so far; the sums are in units of 2^ev. The matrix instructions see the
@@ -490,7 +495,7 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
             top = max3(top, s[i] * k.x, s[i + 1] * k.y);
             top = max3(top, s[i + 2] * k.z, s[i + 3] * k.w);
         }
-        const float up = fmaxf(m, top);
+        const float up = fmaxf(m, top - kLift);
         const float f = m == -INFINITY ? 0.f : fast_exp2(m - up);
         m = up;
         l *= f;
@@ -719,7 +724,7 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
         if (lane == 0) *reinterpret_cast<volatile int*>(flag + warp) = low;
         if (!stream_sync(mi, stream, tphase)) return false;
         const volatile int* f = flag;
-        if (f[0] | f[1] | f[2] | f[3]) {  // raise the references to the tile's maxima
+        if (f[0] | f[1] | f[2] | f[3]) {  // raise the references by the tile's maxima
 #pragma unroll 1
             for (int r0 = 0; r0 < rows; r0 += 4) {
                 float x[4];
@@ -735,8 +740,9 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
             if (!stream_sync(mi, stream, tphase)) return false;
             if (r_in < rows) {
                 const float old = ref[r_in];
-                const float up = fmaxf(max3(old, sp->top[stream][0][r_in], sp->top[stream][1][r_in]),
-                                       fmaxf(sp->top[stream][2][r_in], sp->top[stream][3][r_in]));
+                const float top = fmaxf(fmaxf(sp->top[stream][0][r_in], sp->top[stream][1][r_in]),
+                                        fmaxf(sp->top[stream][2][r_in], sp->top[stream][3][r_in]));
+                const float up = fmaxf(old, top - kLift);
                 sp->down[stream][r_in] = old == -INFINITY ? 0.f : fast_exp2(old - up);
                 ref[r_in] = up;
             }

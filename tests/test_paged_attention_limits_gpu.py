@@ -62,3 +62,62 @@ def test_lengths_without_own_pages_count_nothing(L, alibi):
     want = run(torch.zeros(5, 1, dtype=torch.int32, device="cuda"), [0] * 5)
     assert torch.isfinite(want).all() and want.abs().sum() > 0
     assert torch.equal(run(torch.empty(5, 0, dtype=torch.int32, device="cuda"), [7, 0, INT_MAX, -3, 1]), want)
+
+
+# ---------------------------------------------------------------- small weights
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("nq", [1, 20, 64])
+def test_many_keys_far_below_the_largest_weight(L, kv, nq):
+    """One key 2^25.5 above 32767 others, which carry the whole value: they must not be lost. Sequences enough for
+    every unit's keys to pass one CTA (all on the same pages)."""
+    ctx, bs, seqs = 32768, 128, 300 if nq < 64 else 150
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, kv, ctx // bs, 1, bs)
+    for x in "kv":
+        pool.exact[x].zero_()
+    if kv == "int8":
+        pool.s_all["k"].fill_(0.25)
+        pool.s_all["v"].fill_(2.0 ** -6)
+    pool.exact["v"][:] = 1.0 if kv == "fp16" else 64
+    table = [pool.free[-1 - i] for i in range(ctx // bs)]
+    pool.exact["v"][table[0], :, 0] = 0
+    pool.exact["k"][table[0], :, 0, 0] = 25.0 if kv == "fp16" else 100
+    table = pool.give([ctx])
+    q = torch.zeros(seqs * nq, 4, 128, dtype=torch.float16, device="cuda")
+    q[..., 0] = 8.0                                        # 8 * 25 * SCALE = 17.68 = 25.5 ln 2
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table.expand(seqs, -1).contiguous(), i32([ctx] * seqs),
+                            i32([nq * i for i in range(seqs + 1)]), SCALE, **pool.args())
+    p = torch.arange(ctx - nq, ctx, device="cuda")[:, None]
+    seen = torch.arange(ctx, device="cuda")[None] <= p
+    ref, tol = reference(q[:nq], pool.rows("k", table[0], ctx), pool.rows("v", table[0], ctx), seen, None)
+    tol = tol - ctx * 2.0 ** -25 + ctx * 2.0 ** (-32 if kv == "fp16" else -31)    # max |v| is 1
+    assert (tol < 0.1 * ref).all()
+    check(got.view(seqs, nq, 4, 128), ref[None], tol[None])
+
+
+@pytest.mark.parametrize("nq", [1, 20, 64])
+def test_a_large_v_scale_leaves_the_others_their_digits(L, nq):
+    """INT8: a hardly weighted row with a scale 2^21 times the others'. Alike weights: an element is off by 2^-32
+    times 127 times the power of two above the largest scale, besides the rounding of each weight."""
+    ctx, bs = 300, 16
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, "int8", 40, 1, bs)
+    pool.exact["k"].zero_()
+    pool.s_all["k"].fill_(0.5)
+    pool.exact["v"].copy_(torch.randint(60, 128, pool.exact["v"].shape, generator=g, dtype=torch.int8))
+    pool.s_all["v"].fill_(2.0 ** -15.5)
+    first = pool.free[-1]
+    pool.exact["k"][first, :, 3, 0] = -100                 # 8 * -50 * SCALE: a weight of 2^-51
+    pool.s_all["v"][first, :, 3] = 60.0
+    table = pool.give([ctx])
+    q = torch.zeros(nq, 4, 128, dtype=torch.float16, device="cuda")
+    q[..., 0] = 8.0
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([ctx]), i32([0, nq]), SCALE, causal=False,
+                            **pool.args())
+    seen = torch.ones(nq, ctx, dtype=torch.bool, device="cuda")
+    v = pool.rows("v", table[0], ctx)
+    ref, tol = reference(q, pool.rows("k", table[0], ctx), v, seen, None)
+    tol = tol - ctx * 2.0 ** -25 * v.abs().amax() + 2.0 ** -32 * 127 * 64
+    assert (tol < 0.01 * ref).all()
+    check(got, ref, tol)
