@@ -276,6 +276,7 @@ size_t lik_attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t 
  *
  *   score(p, j) = softmax_scale q.k_j                 (> 0)
  *   if softcap > 0: score = softcap * tanh(score / softcap)
+ *     (softcap < 1e30 and softmax_scale / softcap < 1e30)
  *   if alibi_slopes (fp32 [n_heads]): score -= slope * |p - j|
  *   visible: j < context_lens[b], j >= first_keys[token] (int32 [n_tokens], may
  *     be NULL: the start of the token's document; within a sequence it does not

@@ -316,26 +316,31 @@ struct Row {  // what one softmax thread's row sees
 // 1 / a row's sum of weights: 0 where it saw nothing; what is not finite stays so.
 __device__ __forceinline__ float over_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
-__device__ __forceinline__ float tanh_exp(float t) {  // 1 - 2 / (1 + e^2t)
-    return 1.0f - 2.0f * fast_rcp(1.0f + fast_exp2(t * (2.0f * kLog2e)));
-}
-// tanh on [-0.8, 0.8] as an odd polynomial of degree 9, minimax in the absolute
-// error (3.5e-7): Remez exchange on tanh(t) / t over t^2, weighted by t.
-constexpr float kTanhNear = 0.8f;
-struct TanhNear {  // up tanh(in s) for |in s| <= 0.8, the factors folded into the coefficients
+// tanh on [-0.7, 0.7] as an odd polynomial of degree 9 with linear coefficient 1,
+// minimax in the relative error (3.5e-7): Remez exchange on tanh(t) / t over t^2.
+// A capped score is so within a few fp32 roundings of its own, however loose the cap.
+constexpr float kTanhNear = 0.7f;
+constexpr float kTanh3 = -0.33331084995633364f, kTanh5 = 0.13287660176553176f, kTanh7 = -0.05101637469806898f,
+                kTanh9 = 0.013938170996101448f;
+struct TanhNear {  // up tanh(t) for |t| <= 0.7
     float2 c[5];
-    __device__ __forceinline__ TanhNear(float in, float up) {
-        const float k[5] = {0.9999951124191284f, -0.3331742584705353f, 0.13186219334602356f, -0.04826131463050842f,
-                            0.01146465539932251f};
-        float f = up * in;
+    __device__ __forceinline__ explicit TanhNear(float up) {
+        const float k[5] = {1.0f, kTanh3, kTanh5, kTanh7, kTanh9};
 #pragma unroll
-        for (int i = 0; i < 5; ++i, f *= in * in) c[i] = {k[i] * f, k[i] * f};
+        for (int i = 0; i < 5; ++i) c[i] = {k[i] * up, k[i] * up};
     }
-    __device__ __forceinline__ float2 operator()(float2 s) const {
-        const float2 y = mul2(s, s);
-        return mul2(fma2(fma2(fma2(fma2(c[4], y, c[3]), y, c[2]), y, c[1]), y, c[0]), s);
+    __device__ __forceinline__ float2 operator()(float2 t) const {
+        const float2 y = mul2(t, t);
+        return mul2(fma2(fma2(fma2(fma2(c[4], y, c[3]), y, c[2]), y, c[1]), y, c[0]), t);
     }
 };
+// tanh of any t: the polynomial, or 1 - 2 / (1 + e^2t), which cancels near zero
+__device__ __forceinline__ float tanh_any(float t) {
+    const float y = t * t;
+    const float near = t * fmaf(fmaf(fmaf(fmaf(kTanh9, y, kTanh7), y, kTanh5), y, kTanh3), y, 1.0f);
+    const float far = 1.0f - 2.0f * fast_rcp(1.0f + fast_exp2(t * (2.0f * kLog2e)));
+    return fabsf(t) <= kTanhNear ? near : far;
+}
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -360,7 +365,7 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi) {  // bits lo .
     return from & to;
 }
 
-// W scores that are not near zero, capped in place: up tanh(k s), 16 columns at
+// W scores that are not all near zero, capped in place: up tanh(k s), 16 columns at
 // a time (rolled: this code beside the step's own would crowd the instruction
 // cache, and capped scores are mostly near).
 template <int W, bool I8>
@@ -373,10 +378,10 @@ __device__ __forceinline__ void cap_far(float up, float kf, uint32_t s_addr, con
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const float4 k = I8 ? load_scales(ks + (i0 + i) / 4) : float4{kf, kf, kf, kf};
-            s[i] = up * tanh_exp(s[i] * k.x);
-            s[i + 1] = up * tanh_exp(s[i + 1] * k.y);
-            s[i + 2] = up * tanh_exp(s[i + 2] * k.z);
-            s[i + 3] = up * tanh_exp(s[i + 3] * k.w);
+            s[i] = up * tanh_any(s[i] * k.x);
+            s[i + 1] = up * tanh_any(s[i + 1] * k.y);
+            s[i + 2] = up * tanh_any(s[i + 2] * k.z);
+            s[i + 3] = up * tanh_any(s[i + 3] * k.w);
         }
         tmem_st16(s_addr + i0, reinterpret_cast<const uint32_t*>(s));
     }
@@ -403,25 +408,23 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
 #pragma unroll
     for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
     tmem_wait_ld();
-    if (MOD) {  // scores to powers of two
-        if (I8 || p.cap == 0.f) {
+    if (MOD) {  // scores to powers of two, or tanh's arguments
 #pragma unroll
-            for (int i = 0; i < W; i += 4) {
-                const float4 k = I8 ? load_scales(ks + i / 4) : float4{p.kf, p.kf, p.kf, p.kf};
-                const float2 a = mul2({s[i], s[i + 1]}, {k.x, k.y}), b = mul2({s[i + 2], s[i + 3]}, {k.z, k.w});
-                s[i] = a.x;
-                s[i + 1] = a.y;
-                s[i + 2] = b.x;
-                s[i + 3] = b.y;
-            }
+        for (int i = 0; i < W; i += 4) {
+            const float4 k = I8 ? load_scales(ks + i / 4) : float4{p.kf, p.kf, p.kf, p.kf};
+            const float2 a = mul2({s[i], s[i + 1]}, {k.x, k.y}), b = mul2({s[i + 2], s[i + 3]}, {k.z, k.w});
+            s[i] = a.x;
+            s[i + 1] = a.y;
+            s[i + 2] = b.x;
+            s[i + 3] = b.y;
         }
         if (p.cap > 0.f) {
-            const float up = p.cap * kLog2e, in = I8 ? 1.f : p.kf;
+            const float up = p.cap * kLog2e;
             float far[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < W; i += 2) far[i / 2 & 3] = max3_abs(far[i / 2 & 3], s[i], s[i + 1]);
-            if (__all_sync(kFull, fmaxf(max3(far[0], far[1], far[2]), far[3]) * in <= kTanhNear)) {
-                const TanhNear near(in, up);
+            if (__all_sync(kFull, fmaxf(max3(far[0], far[1], far[2]), far[3]) <= kTanhNear)) {
+                const TanhNear near(up);
 #pragma unroll
                 for (int i = 0; i < W; i += 2) {
                     const float2 t = near({s[i], s[i + 1]});
@@ -707,7 +710,7 @@ __device__ bool thin_segment(const Params& p, Misc* mi, unsigned char* smem, con
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 x[c] *= kx;
-                if (MOD && p.cap > 0.f) x[c] = p.cap * kLog2e * tanh_exp(x[c]);
+                if (MOD && p.cap > 0.f) x[c] = p.cap * kLog2e * tanh_any(x[c]);
                 if (MOD && p.slopes)
                     x[c] = fmaf(-sp->row[r0 + c].slope, fabsf(static_cast<float>(j - sp->row[r0 + c].pos)), x[c]);
                 if (!whole || r0 + c >= rows) {
@@ -1297,7 +1300,7 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
             const float sc = mine_seen ? __half2float(scale[t]) : 0.f;
             if (!is_v) {
                 // never zero: a hidden key's score is -inf times this
-                scales->k[at][t] = mine_seen ? fmaxf(sc * p.kf, 1e-30f) : 1.f;
+                scales->k[at][t] = mine_seen ? fmaxf(sc * p.kf, FLT_MIN) : 1.f;
             } else {
                 const int r4 = lane * 4;
                 const uint2 raw = *reinterpret_cast<const uint2*>(scale + r4);

@@ -506,6 +506,8 @@ static lik_status check_attention(const AttentionArgs& a, int64_t head_dim) {
         return fail(LIK_ERR_INVALID_ARGUMENT, "softmax_scale must be positive and finite");
     if (!(a.softcap >= 0.f) || !(a.softcap < 1e30f))
         return fail(LIK_ERR_INVALID_ARGUMENT, "softcap must be finite and >= 0 (0: none)");
+    if (a.softcap > 0.f && !(a.softmax_scale / a.softcap < 1e30f))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "softcap must be above softmax_scale / 1e30");
     if (a.window < 0 || a.window > (int64_t{1} << 30)) return fail(LIK_ERR_INVALID_ARGUMENT, "window out of range");
     if (a.block_size <= 0 || a.block_size % 16 != 0 || a.block_size > (1 << 20))
         return fail(LIK_ERR_INVALID_ARGUMENT, "block_size must be a positive multiple of 16");

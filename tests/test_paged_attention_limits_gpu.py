@@ -121,3 +121,59 @@ def test_a_large_v_scale_leaves_the_others_their_digits(L, nq):
     tol = tol - ctx * 2.0 ** -25 * v.abs().amax() + 2.0 ** -32 * 127 * 64
     assert (tol < 0.01 * ref).all()
     check(got, ref, tol)
+
+
+# ---------------------------------------------------------------- loose and tight caps
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e29])
+@pytest.mark.parametrize("nq", [1, 20, 64])
+@pytest.mark.parametrize("far", [False, True])
+def test_loose_caps_keep_the_score(L, kv, cap, nq, far):
+    """Scores of single products (exact in fp32), so that a capped score is off by its own fp32 roundings: some ten of
+    half a step (2^-24) and the polynomial's 2^-23.7, less than 8 * 2^-23 |score|. `far`: among them keys whose scores
+    lie at twice the cap below zero, where they have no weight."""
+    ctx, bs, q0 = 700, 16, 512.0
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, kv, 50, 1, bs)
+    c = 8.0 + torch.randint(0, 9, pool.exact["k"].shape[:3], generator=g).float() / 2      # scores of 5.7 to 8.5
+    off = (torch.rand(c.shape, generator=g) < 0.03) if far and cap < 1e20 else torch.zeros(c.shape, dtype=torch.bool)
+    down = -2 * cap / (q0 * SCALE) if cap < 1e20 else 0.0
+    pool.exact["k"].zero_()
+    if kv == "fp16":
+        pool.exact["k"][..., 0] = torch.where(off, torch.full_like(c, down), c / 64).half().cuda()
+    else:
+        pool.exact["k"][..., 0] = torch.where(off, torch.full_like(c, -127.0), c * 8).to(torch.int8).cuda()
+        pool.s_all["k"][:] = torch.where(off, torch.full_like(c, -down / 127), torch.full_like(c, 2.0 ** -9)).half().cuda()
+    table = pool.give([ctx])
+    q = torch.zeros(nq, 4, 128, dtype=torch.float16, device="cuda")
+    q[..., 0] = q0
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([ctx]), i32([0, nq]), SCALE, softcap=cap,
+                            causal=False, **pool.args())
+    k, v = pool.rows("k", table[0], ctx), pool.rows("v", table[0], ctx)
+    s = q0 * k[0, :, 0] * SCALE
+    s = cap * torch.tanh(s / cap)
+    w = torch.exp(s - s.max())
+    d = 8 * 2.0 ** -23 * s[w > 1e-9].abs().max()
+    ref, A = (w @ v[0]) / w.sum(), (w @ v[0].abs()) / w.sum()
+    tol = A * (H11 + 2 * torch.expm1(d)) + H11 * ref.abs() + ctx * 2.0 ** -31 * v.abs().max() + 1e-7
+    check(got, ref.expand(nq, 4, 128), tol.expand(nq, 4, 128))
+
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("cap", [1e-7, 1e-25])
+@pytest.mark.parametrize("nq", [1, 20, 64])
+def test_tight_caps(L, kv, cap, nq):
+    """Every key weighs the same, scores of zero among them (the first sequence's)."""
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, kv, 40, 2, 16)
+    table = pool.give([300, 200])
+    q = rand(g, 2 * nq, 8, 128)
+    q[:nq] = 0
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([300, 200]), i32([0, nq, 2 * nq]), SCALE,
+                            softcap=cap, **pool.args())
+    for b, m in enumerate([300, 200]):
+        p = torch.arange(m - nq, m, device="cuda")[:, None]
+        ref, tol = reference(q[b * nq:(b + 1) * nq], pool.rows("k", table[b], m), pool.rows("v", table[b], m),
+                             torch.arange(m, device="cuda")[None] <= p, None, cap)
+        check(got[b * nq:(b + 1) * nq], ref, tol)
