@@ -288,10 +288,11 @@ size_t lik_attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t 
  * cu_seqlens_q[0], from cu_seqlens_q[n_seqs] on) are left as they are, or set
  * to zero with zero_tail != 0. Keys and values that no query of a sequence
  * sees (page ends, what left the window) may hold anything, and the table
- * entries of pages with none that is seen are not read; a value that some query sees must be
- * finite. A table entry outside [0, num_blocks) that is reached reads as zero
- * keys and values, and LIK_ERR_DEVICE_BAD_BLOCK is recorded
- * (lik_attention_check). Requires n_heads / n_kv_heads <= 128 and fewer than
+ * entries of pages with none that is seen are not read; a value (and its scale)
+ * that some query sees must be finite, a key or its scale that is NaN makes the
+ * rows that see it NaN. Scales may have either sign. A table entry outside
+ * [0, num_blocks) that is reached reads as zero keys and values, and
+ * LIK_ERR_DEVICE_BAD_BLOCK is recorded (lik_attention_check). Requires n_heads / n_kv_heads <= 128 and fewer than
  * 2^31 - 128 rows in the cache (num_blocks * n_kv_heads * block_size).
  * Lengths and offsets are read on the device: a captured call may be replayed
  * with others. */

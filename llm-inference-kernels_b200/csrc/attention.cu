@@ -180,6 +180,7 @@ static_assert(sizeof(Misc) <= 2048, "the barrier block must fit behind the tiles
 
 struct Scales {  // INT8 caches, see convert_role
     float k[kScales][kTile], v[kScales][kTile];
+    float ones[kTile / 2];
     int v_exp[kScales];
 };
 
@@ -209,8 +210,8 @@ struct Layout {
     static constexpr int stage = raw + (FMT == kF16 ? 0 : 2 * kRaw * (kRawBytes + 256));
     static constexpr int stage_bytes = FMT == kF16 ? 32768 : 16384;
     static constexpr int scales = stage + stage_bytes;
-    static constexpr int misc = scales + (FMT == kF16 ? 0 : 4352);
-    static_assert(sizeof(Scales) <= 4352, "scales");
+    static constexpr int misc = scales + (FMT == kF16 ? 0 : 4368);
+    static_assert(sizeof(Scales) <= 4368, "scales");
     static constexpr int bytes = misc + 2048;
     static constexpr int threads = FMT == kF16 ? 384 : 640;
     // registers per thread: launched with `base`, then moved between the
@@ -398,12 +399,13 @@ __device__ __forceinline__ void cap_far(float up, float kf, uint32_t s_addr, con
 //
 // INT8: ks holds kf times K's scales, vs V's scales divided by 2^v_exp, the
 // largest so far; the sums are in units of 2^ev. The matrix instructions see the
-// exact codes.
+// exact codes. Scales may have any sign or be no number: they are applied before
+// a key is hidden, and `ones` stands in for them afterwards.
 template <int W, bool I8, bool MOD>
 __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Row& row, uint32_t s_addr, uint32_t p_addr,
                                              uint32_t o_addr, int j0, bool have_sums, uint64_t* odone, uint32_t odone_parity,
-                                             const float4* ks, const float4* vs, int v_exp, float& m, float& l,
-                                             int& ev) {
+                                             const float4* ks, const float4* vs, const float4* ones, int v_exp, float& m,
+                                             float& l, int& ev) {
     float s[W];
 #pragma unroll
     for (int i = 0; i < W; i += 32) tmem_ld32(s_addr + i, s + i);
@@ -446,6 +448,17 @@ __device__ __forceinline__ bool softmax_step(const Params& p, Misc* mi, const Ro
     }
     const bool whole = (j0 >= row.lo && j0 + W - 1 <= row.hi) || (j0 >= row.fk && j0 + W <= row.pfx);
     if (__any_sync(kFull, !whole)) {
+        if (I8 && !MOD) {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                const float4 k = load_scales(ks + i / 4);
+                s[i] *= k.x;
+                s[i + 1] *= k.y;
+                s[i + 2] *= k.z;
+                s[i + 3] *= k.w;
+            }
+            ks = ones;
+        }
 #pragma unroll
         for (int i = 0; i < W; i += 32) {
             const int j = j0 + i;
@@ -552,7 +565,8 @@ __device__ __forceinline__ bool softmax_run(const Params& p, Misc* mi, const Sca
             const float4* ks = reinterpret_cast<const float4*>(scales->k[st] + c);
             if (!softmax_step<W, I8, MOD>(p, mi, row, s_addr + c, s_addr + c / 2, o_addr, j0 + c, i > i0 || c > 0,
                                      c > 0 ? &mi->odone[stream][0] : nullptr, halves & 1, ks,
-                                     reinterpret_cast<const float4*>(scales->v[st] + c), v_exp, m, l, ev))
+                                     reinterpret_cast<const float4*>(scales->v[st] + c),
+                                     reinterpret_cast<const float4*>(scales->ones), v_exp, m, l, ev))
                 return false;
             tmem_wait_st();
             tcgen05_fence_before();
@@ -1299,18 +1313,17 @@ __device__ void convert_role(const Params& p, Misc* mi, unsigned char* smem, boo
             const bool mine_seen = all || seen(t);
             const float sc = mine_seen ? __half2float(scale[t]) : 0.f;
             if (!is_v) {
-                // never zero: a hidden key's score is -inf times this
-                scales->k[at][t] = mine_seen ? fmaxf(sc * p.kf, FLT_MIN) : 1.f;
+                scales->k[at][t] = sc * p.kf;
             } else {
                 const int r4 = lane * 4;
                 const uint2 raw = *reinterpret_cast<const uint2*>(scale + r4);
-                const float2 a = __half22float2(as_h2(raw.x)), b = __half22float2(as_h2(raw.y));
+                const float2 a = __half22float2(__habs2(as_h2(raw.x))), b = __half22float2(__habs2(as_h2(raw.y)));
                 float most = fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y));
                 if (!all)
                     most = fmaxf(fmaxf(seen(r4) ? a.x : 0.f, seen(r4 + 1) ? a.y : 0.f),
                                  fmaxf(seen(r4 + 2) ? b.x : 0.f, seen(r4 + 3) ? b.y : 0.f));
                 const uint32_t bits = __reduce_max_sync(kFull, __float_as_uint(most));
-                top = max(top, static_cast<int>(bits >> 23) - 126);
+                top = max(top, min(static_cast<int>(bits >> 23) - 126, 17));  // 17: no finite scale
                 scales->v[at][t] = sc * __int_as_float((127 - top) << 23);
                 scales->v_exp[at] = top;
                 warp_arrive(&mi->vscale[at]);
@@ -1551,6 +1564,7 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     grid_dependency_wait();
     grid_launch_dependents();
     plan<Lay::threads>(p, mi);
+    if (FMT != kF16 && threadIdx.x < kTile / 2) reinterpret_cast<Scales*>(smem + Lay::scales)->ones[threadIdx.x] = 1.f;
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();

@@ -177,3 +177,40 @@ def test_tight_caps(L, kv, cap, nq):
         ref, tol = reference(q[b * nq:(b + 1) * nq], pool.rows("k", table[b], m), pool.rows("v", table[b], m),
                              torch.arange(m, device="cuda")[None] <= p, None, cap)
         check(got[b * nq:(b + 1) * nq], ref, tol)
+
+
+# ---------------------------------------------------------------- scales of any sign, and none
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("nq,ctx", [(1, 300), (3, 40), (20, 500), (64, 700), (300, 900)])
+def test_scales_of_either_sign(L, nq, ctx, cap):
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, "int8", -(-ctx // 16) + 1, 2, 16)
+    for x in "kv":
+        s = pool.s_all[x]
+        s *= torch.where(torch.rand(s.shape, generator=g) < 0.5, -1.0, 1.0).half().cuda()
+        s[torch.rand(s.shape, generator=g).cuda() < 0.05] = 0.0
+    table = pool.give([ctx])
+    q = rand(g, nq, 8, 128)
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([ctx]), i32([0, nq]), SCALE, softcap=cap,
+                            window=max(ctx // 3, 1), **pool.args())
+    p = torch.arange(ctx - nq, ctx, device="cuda")[:, None]
+    j = torch.arange(ctx, device="cuda")[None]
+    check(got, *reference(q, pool.rows("k", table[0], ctx), pool.rows("v", table[0], ctx),
+                          (j <= p) & (j > p - max(ctx // 3, 1)), None, cap))
+
+
+@pytest.mark.parametrize("side", ["k", "v"])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("nq,ctx", [(1, 300), (1, 30000), (20, 500), (64, 700), (300, 900)])
+def test_a_scale_that_is_not_a_number_reaches_the_rows_that_see_it(L, side, nq, ctx, cap):
+    g = torch.Generator().manual_seed(nq)
+    pool = Pool(g, "int8", 2 * (-(-ctx // 64)) + 1, 2, 64)
+    pool.exact["v"][pool.exact["v"] == 0] = 1
+    bad, good = pool.give([ctx]), pool.give([ctx])
+    pool.scale[side][bad[0, 0], 1, 5] = math.nan           # a key that every row of the first sequence sees
+    q = rand(g, 2 * nq, 8, 128)
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], torch.cat([bad, good]), i32([ctx, ctx]), i32([0, nq, 2 * nq]),
+                            SCALE, softcap=cap, **pool.args())
+    assert torch.isnan(got[:nq, 4:]).all()
+    assert torch.isfinite(got[:nq, :4]).all() and torch.isfinite(got[nq:]).all()
