@@ -289,7 +289,7 @@ __device__ bool make_unit(const Params& p, int id, Segment& s) {
     s.ctx = static_cast<int>(min(static_cast<long long>(max(k.ctx[b], 0)),
                                  static_cast<long long>(k.width) * p.block_size));
     s.pos0 = s.ctx - n + at;
-    s.pfx = p.prefix_lens && s.set == 0 ? min(p.prefix_lens[b], s.ctx) : 0;
+    s.pfx = p.prefix_lens && s.set == 0 ? clampi(p.prefix_lens[b], 0, s.ctx) : 0;
     const int fk = p.first_keys ? max(p.first_keys[s.tok0], 0) : 0;  // they do not decrease
     s.fk = fk;
     s.vlo = p.window > 0 ? max(s.pos0 - p.window + 1, fk) : fk;

@@ -214,3 +214,22 @@ def test_a_scale_that_is_not_a_number_reaches_the_rows_that_see_it(L, side, nq, 
                             SCALE, softcap=cap, **pool.args())
     assert torch.isnan(got[:nq, 4:]).all()
     assert torch.isfinite(got[:nq, :4]).all() and torch.isfinite(got[nq:]).all()
+
+
+# ---------------------------------------------------------------- prefixes out of range
+
+@pytest.mark.parametrize("kv", KV)
+@pytest.mark.parametrize("nq", [1, 20, 64])
+def test_prefixes_below_zero_show_nothing(L, kv, nq):
+    g = torch.Generator().manual_seed(nq)
+    ctx = 300
+    pool = Pool(g, kv, 80, 2, 16)
+    table = pool.give([ctx] * 3)
+    q = rand(g, 3 * nq, 8, 128)
+    got = L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([ctx] * 3), i32([0, nq, 2 * nq, 3 * nq]), SCALE,
+                            window=100, prefix_lens=i32([-INT_MAX - 1, -INT_MAX, -5]), **pool.args())
+    p = torch.arange(ctx - nq, ctx, device="cuda")[:, None]
+    j = torch.arange(ctx, device="cuda")[None]
+    for b in range(3):
+        check(got[b * nq:(b + 1) * nq], *reference(q[b * nq:(b + 1) * nq], pool.rows("k", table[b], ctx),
+                                                   pool.rows("v", table[b], ctx), (j <= p) & (j > p - 100), None))
