@@ -98,6 +98,15 @@ lik_status lik_selftest_leave_timeout(int64_t polls, void* workspace, size_t wor
  * (synchronizes `stream`); the CUDA context stays usable. */
 lik_status lik_selftest_bounded_wait(int64_t polls, int* device_error, void* stream);
 
+/* Failure-detection self test of the attention kernel: in the calling thread's
+ * next attention call the barriers of one step of every block expect one arrival
+ * more than there is, so that its wait runs out: 1 copies of the queries, 2 K
+ * tiles, 3 V tiles, 4 scores, 5 weights, 6 sums, 7 the schedule, 8 copies of
+ * INT8 codes (0: none). The blocks must wait out what they have in flight and
+ * return (in a second or two); their results are void, lik_attention_check reports
+ * LIK_ERR_DEVICE_TIMEOUT once, and later calls are as ever. */
+lik_status lik_selftest_attention_timeout(int64_t what);
+
 /* ---- decode attention (single query token per sequence) -------------- */
 
 /* fp16 KV. Replaces launch_decode_attention_splitk

@@ -90,6 +90,10 @@ constexpr uint32_t kPolls = 1u << 18;            // a poll sleeps for a few micr
 
 enum Mode : int { kWide = 0, kPaired = 1, kThin = 2 };
 enum Dest : int { kDirect = 0, kSlot = 1, kRowBuf = 2 };
+// Self test: the step whose barriers expect one arrival more than there is.
+enum Stall : int {
+    kNoStall, kStallQuery, kStallK, kStallV, kStallScores, kStallWeights, kStallSums, kStallSegment, kStallRaw
+};
 
 // Division of 0 <= x < 2^31 by a launch constant (the round-up method of
 // Granlund and Montgomery): a multiplication instead of some thirty
@@ -133,6 +137,7 @@ struct Params {
     int shared;      // every unit's result goes through the joining kernel
     int zero_tail;
     int slot_rows, grid;
+    int stall;       // self test: the step whose wait runs out (Stall)
     float* part;     // [2 grid][slot_rows][128]
     float2* part_ml; // [2 grid][slot_rows] (maximum in powers of two, sum)
     int4* split;     // [grid] first token, tokens, head, last CTA (-1: none) of the unit split from this CTA on
@@ -1153,7 +1158,7 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
     const int sub = FMT == kF16 ? lane >> 1 & 7 : lane & 7;          // this lane's box
     const int part = FMT == kF16 ? lane & 1 : lane >> 3 & 1;         // half of the channels; codes or scales
     const bool mine = sub < subs && lane < 16;
-    uint32_t pos = 0, q_seg = 0;  // tiles and query loads so far
+    uint32_t pos = 0, q_seg = 0;  // tiles and query loads issued so far
     uint32_t thin = 0;            // 1 + the last thin segment
     uint64_t* const fulls = FMT == kF16 ? mi->full[is_v] : mi->rfull[is_v];
     uint64_t* const empties = FMT == kF16 ? mi->empty[is_v] : mi->rempty[is_v];
@@ -1194,7 +1199,6 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
             if (!is_v) {
                 // queries: the last segment's score tiles are done with them
                 if (q_seg > 0 && !warp_wait(&mi->qempty, (q_seg - 1) & 1, mi)) break;
-                ++q_seg;
                 if (mode == kWide && thin && k - (thin - 1) < kSegs &&
                     !warp_wait(&mi->segempty[(thin - 1) % kSegs], ((thin - 1) / kSegs) & 1, mi))
                     break;  // a thin segment still uses the second tile's place
@@ -1206,13 +1210,14 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
                     tma_load_3d(smem + c * kTileBytes + half * kHalfTile, &maps.q[mode == kThin], half * 64,
                                 head * p.group, tok0 + c * toks, &mi->qfull);
                 }
+                ++q_seg;
             }
             const int L = mode == kWide ? 1 : 2;
 #pragma unroll 1
             for (int i = -L; i < n; ++i) {
                 const int it = is_v ? i : i + L;  // this warp's tile now
                 if (it < 0 || it >= n) continue;
-                const uint32_t e = pos++;
+                const uint32_t e = pos;
                 if (it << sub_shift >> 5 != batch) {
                     ++batch;
                     rows = place(ahead, batch);
@@ -1249,19 +1254,23 @@ __device__ void copy_role(const Params& p, Misc* mi, unsigned char* smem, const 
                                        (is_v ? p.v_scale : p.k_scale) + row, p.box_rows * 2, full);
                 }
                 __syncwarp();
+                ++pos;
             }
         }
         if (!ok) break;
         if (mode == kThin) thin = k + 1;
         warp_arrive(&mi->segempty[slot]);
     }
-    // Leave no copy in flight: after an abort nobody else waits for them.
-    if (*reinterpret_cast<volatile int*>(&mi->abort)) {
-        for (uint32_t e = pos > ring ? pos - ring : 0; e < pos; ++e)
-            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&fulls[e % ring], (e / ring) & 1); ++i) {}
-        if (q_seg > 0)
-            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->qfull, (q_seg - 1) & 1); ++i) {}
-    }
+    // Leave no copy in flight: if a wait runs out, here or in another warp and
+    // later, nobody else waits for them. A slot's earlier copy was done before its
+    // latest one was issued, and none is issued afterwards, so each parity names it.
+#pragma unroll 1
+    for (uint32_t e = pos > ring ? pos - ring : 0; e < pos; ++e)
+#pragma unroll 1
+        for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&fulls[e % ring], (e / ring) & 1); ++i) {}
+    if (q_seg > 0)
+#pragma unroll 1
+        for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->qfull, (q_seg - 1) & 1); ++i) {}
 }
 
 // ---- INT8 conversion -------------------------------------------------------------
@@ -1526,27 +1535,28 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
     const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         const int readers = FMT == kF16 ? 11 : 19;  // warps that read a segment
+        auto late = [&](Stall what) { return p.stall == what ? 1 : 0; };
         for (int v = 0; v < 2; ++v) {
             for (int i = 0; i < kMaxRing; ++i) {
-                mbar_init(&mi->full[v][i], FMT == kF16 ? 1 : 4);
+                mbar_init(&mi->full[v][i], (FMT == kF16 ? 1 : 4) + late(v ? kStallV : kStallK));
                 mbar_init(&mi->empty[v][i], 1);
             }
         }
         for (int i = 0; i < 2 * kRaw; ++i) {
-            mbar_init(&mi->rfull[0][i], 1);
+            mbar_init(&mi->rfull[0][i], 1 + late(kStallRaw));
             mbar_init(&mi->rempty[0][i], 4);
         }
-        mbar_init(&mi->qfull, 1);
+        mbar_init(&mi->qfull, 1 + late(kStallQuery));
         mbar_init(&mi->qempty, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&mi->sfull[i], 1);
+            mbar_init(&mi->sfull[i], 1 + late(kStallScores));
             for (int h = 0; h < 2; ++h) {
-                mbar_init(&mi->pready[i][h], 4);
-                mbar_init(&mi->odone[i][h], 1);
+                mbar_init(&mi->pready[i][h], 4 + late(kStallWeights));
+                mbar_init(&mi->odone[i][h], 1 + late(kStallSums));
             }
         }
         for (int i = 0; i < kSegs; ++i) {
-            mbar_init(&mi->segfull[i], 1);
+            mbar_init(&mi->segfull[i], 1 + late(kStallSegment));
             mbar_init(&mi->segempty[i], readers);
         }
         for (int i = 0; i < kScales; ++i) mbar_init(&mi->vscale[i], 4);
@@ -1584,10 +1594,10 @@ __global__ void __launch_bounds__(Layout<FMT>::threads, 1)
             copy_role<FMT>(p, mi, smem, maps, true);
         } else if (warp == 9) {
             mma_role<FMT>(p, mi, smem);
-            if (*reinterpret_cast<volatile int*>(&mi->abort)) {  // wait out what is still running
-                mma_commit(&mi->drain, elect_one());
-                for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->drain, 0); ++i) {}
-            }
+            __syncwarp();
+            mma_commit(&mi->drain, elect_one());  // leave no product running, as for the copies
+#pragma unroll 1
+            for (uint32_t i = 0; i < kPolls && !mbar_try_wait(&mi->drain, 0); ++i) {}
         } else if (warp == 10) {
             schedule_role(p, mi);
         }
@@ -1673,7 +1683,8 @@ __global__ void __launch_bounds__(256) join_split_kernel(const __grid_constant__
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 u = p.split[blockIdx.x];
-    if (u.w >= 0 && u.x >= 0 && u.y >= 0 && u.x + u.y <= p.n_tokens && u.y <= 2 * (kTile / p.group) && u.z >= 0 &&
+    // (entries that a CTA which gave up never wrote hold anything)
+    if (u.w >= 0 && u.x >= 0 && u.y >= 0 && u.y <= 2 * (kTile / p.group) && u.x <= p.n_tokens - u.y && u.z >= 0 &&
         u.z < p.n_kv) {
         const int rows = u.y * p.group;
         for (int r = blockIdx.y * 8 + warp; r < rows; r += gridDim.y * 8) {
@@ -1848,7 +1859,11 @@ lik_status launch(const Maps& maps, const Params& p, cudaStream_t stream, std::s
     return LIK_OK;
 }
 
+thread_local int next_stall = kNoStall;
+
 }  // namespace
+
+void stall_next_attention(int what) { next_stall = what; }
 
 size_t attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t n_kv, int64_t n_groups, bool shared,
                                  int sm_count) {
@@ -1923,6 +1938,8 @@ lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::st
     p.zero_tail = a.zero_tail;
     p.slot_rows = w.slot_rows;
     p.grid = di.sm_count;
+    p.stall = next_stall;
+    next_stall = kNoStall;
     unsigned char* ws = static_cast<unsigned char*>(a.workspace);
     p.part = reinterpret_cast<float*>(ws + w.part);
     p.part_ml = reinterpret_cast<float2*>(ws + w.ml);

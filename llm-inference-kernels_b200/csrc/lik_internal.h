@@ -87,6 +87,8 @@ lik_status launch_rope_append(const RopeAppendArgs& a, cudaStream_t stream, std:
 size_t attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t n_kv, int64_t n_groups, bool shared,
                                  int sm_count);
 lik_status launch_attention(const AttentionArgs& a, cudaStream_t stream, std::string& err);
+// Self test: in this thread's next attention launch a wait runs out (lik_selftest_attention_timeout).
+void stall_next_attention(int what);
 // Device address of the attention kernels' error word on the current device.
 void* attention_error_word(std::string& err);
 

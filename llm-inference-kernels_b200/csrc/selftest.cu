@@ -103,3 +103,12 @@ extern "C" lik_status lik_selftest_leave_timeout(int64_t polls, void* workspace,
     }
     return LIK_OK;
 }
+
+extern "C" lik_status lik_selftest_attention_timeout(int64_t what) {
+    if (what < 0 || what > 8) {
+        lik::set_last_error("what must be in [0, 8]");
+        return LIK_ERR_INVALID_ARGUMENT;
+    }
+    lik::stall_next_attention(static_cast<int>(what));
+    return LIK_OK;
+}

@@ -233,3 +233,56 @@ def test_prefixes_below_zero_show_nothing(L, kv, nq):
     for b in range(3):
         check(got[b * nq:(b + 1) * nq], *reference(q[b * nq:(b + 1) * nq], pool.rows("k", table[b], ctx),
                                                    pool.rows("v", table[b], ctx), (j <= p) & (j > p - 100), None))
+
+
+# ---------------------------------------------------------------- a wait that runs out
+
+SHAPES = {"wide": ([300], [900]), "paired": ([20], [9000]), "thin": ([1, 1, 1], [300, 20000, 5]),
+          "mixed": ([1, 40, 300, 2], [700, 40, 2000, 130])}
+STEPS = ([("fp16", i, "mixed") for i in range(1, 8)] + [("int8", i, "mixed") for i in range(1, 9)] +
+         [("fp16", 3, "thin"), ("int8", 8, "thin"), ("fp16", 5, "wide"), ("int8", 2, "paired")])
+
+
+@pytest.mark.parametrize("kv,step,shape", STEPS)
+def test_a_wait_that_runs_out_is_reported_and_over(L, kv, step, shape):
+    """One step of every block is never seen completed: the call returns, memory around the result and later calls
+    are untouched."""
+    from llmik_cuda import cabi
+    nq, ctx = SHAPES[shape]
+    g = torch.Generator().manual_seed(step)
+    pool = Pool(g, kv, sum(-(-c // 32) for c in ctx) + 1, 2, 32)
+    table = pool.give(ctx)
+    n = sum(nq)
+    q = rand(g, n, 8, 128)
+    cu = i32([sum(nq[:i]) for i in range(len(nq) + 1)])
+    buf = torch.full((n + 20, 8, 128), 7.0, dtype=torch.float16, device="cuda")
+    call = lambda out=None: L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32(ctx), cu, SCALE, out=out,  # noqa: E731
+                                              **pool.args())
+    want = call()
+    L.check_device_errors()
+    cabi.call("lik_selftest_attention_timeout", step)
+    call(buf[10:-10])
+    with pytest.raises(RuntimeError, match="wait expired"):
+        L.check_device_errors()
+    assert (buf[:10] == 7).all() and (buf[-10:] == 7).all()
+    assert torch.equal(call(), want)
+    L.check_device_errors()
+
+
+@pytest.mark.parametrize("kv,step", [("fp16", 3), ("fp16", 7), ("int8", 5)])
+def test_a_wait_that_runs_out_over_a_shared_prefix(L, kv, step):
+    from llmik_cuda import cabi
+    g = torch.Generator().manual_seed(step)
+    pool = Pool(g, kv, 60, 2, 32)
+    pt, own = pool.give([700]), [1, 0, 40, 3, 100]
+    t = pool.give(own)
+    q = rand(g, 5, 8, 128)
+    call = lambda: L.paged_shared_prefix_attention(q, pool.cache["k"], pool.cache["v"], pt, i32([700]), i32([0, 5]), t,  # noqa: E731
+                                                   i32(own), SCALE, **pool.args())
+    want = call()
+    cabi.call("lik_selftest_attention_timeout", step)
+    call()
+    with pytest.raises(RuntimeError, match="wait expired"):
+        L.check_device_errors()
+    assert torch.equal(call(), want)
+    L.check_device_errors()
