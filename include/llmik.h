@@ -336,9 +336,10 @@ lik_status lik_attention_shared_prefix(
     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Read (and clear) the device error word of the two entry points above on the
- * current device, after the work queued on `stream` (synchronizes it):
+ * current device, which all streams share: waits for the device, then uses `stream`.
  * *device_error = 0 and LIK_OK when clean, else the code and status of
- * lik_workspace_check. */
+ * lik_workspace_check. An error recorded by another thread's call while the word
+ * is being read is reported with it or by the next check. */
 lik_status lik_attention_check(void* stream, int* device_error);
 
 /* ---- KV quantize / pack --------------------------------------------- */

@@ -596,7 +596,13 @@ lik_status lik_attention_check(void* stream, int* device_error) {
     std::string err;
     void* word = attention_error_word(err);
     if (!word) return fail(LIK_ERR_CUDA, err);
-    return check_error_word(word, sizeof(int), as_stream(stream), device_error);
+    // The word is the device's, not a stream's: wait for all that may write it, and
+    // for its clearing, lest that wipe out what a later call records.
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return fail(LIK_ERR_CUDA, std::string("error-word check: ") + cudaGetErrorString(e));
+    const lik_status s = check_error_word(word, sizeof(int), as_stream(stream), device_error);
+    e = cudaStreamSynchronize(as_stream(stream));
+    return e == cudaSuccess ? s : fail(LIK_ERR_CUDA, std::string("error-word check: ") + cudaGetErrorString(e));
 }
 
 }  // extern "C"

@@ -13,7 +13,6 @@
 
 #include <map>
 #include <mutex>
-#include <set>
 #include <tuple>
 
 #include "llmik.h"
@@ -49,37 +48,26 @@ at::Tensor& workspace(const at::Tensor& like, size_t bytes) {
     return t;
 }
 
-// Streams that attention ran on: its error word is one per device, and a check
-// has to wait for all of them.
-std::set<std::pair<int, void*>>& attention_streams() {
-    static std::set<std::pair<int, void*>> streams;
-    return streams;
-}
-
-// Failure detection for the torch ops: read the device error word of every
-// cached workspace of the current device (synchronizing each workspace's
-// stream), then attention's. A kernel whose bounded wait expired, or that met an out-of-range
-// block-table entry, left a code there and possibly unit counters that are
-// not zero; lik_workspace_check zeroes such a workspace again, and this op
-// then raises, so the failed step is reported and the next one starts clean.
+// Failure detection for the torch ops: read attention's error word (one per
+// device: this waits for all of the device's work, replayed graphs among it),
+// then that of every cached workspace of the current device. A kernel whose
+// bounded wait expired, or that met an out-of-range block-table entry, left a
+// code there and possibly unit counters that are not zero; lik_workspace_check
+// zeroes such a workspace again, and this op then raises, so the failed step is
+// reported and the next one starts clean.
 void check_device_errors() {
     const int dev = static_cast<int>(c10::cuda::current_device());
     std::string msg;
+    int code = 0;
+    lik_status st = lik_attention_check(cur_stream(), &code);
+    if (st != LIK_OK) msg = std::string(lik_status_string(st)) + ": " + lik_last_error();
     std::lock_guard<std::mutex> lock(ws_mutex());
     for (auto& kv : ws_cache()) {
         if (kv.first.first != dev || !kv.second.defined()) continue;
-        int code = 0;
-        const lik_status st =
-            lik_workspace_check(kv.second.data_ptr(), kv.second.numel(), kv.first.second, &code);
+        st = lik_workspace_check(kv.second.data_ptr(), kv.second.numel(), kv.first.second, &code);
         if (st != LIK_OK) msg += std::string(msg.empty() ? "" : "; ") + lik_status_string(st) + ": " + lik_last_error();
     }
-    for (const auto& used : attention_streams()) {
-        if (used.first != dev) continue;
-        int code = 0;
-        const lik_status st = lik_attention_check(used.second, &code);
-        if (st != LIK_OK) msg += std::string(msg.empty() ? "" : "; ") + lik_status_string(st) + ": " + lik_last_error();
-    }
-    TORCH_CHECK(msg.empty(), "decode kernel reported a device-side error (workspace reset): ", msg);
+    TORCH_CHECK(msg.empty(), "a kernel reported a device-side error (its scratch is reset): ", msg);
 }
 
 // Test hook for check_device_errors: leave, in the current stream's
@@ -673,10 +661,6 @@ AttnCommon attention_common(const at::Tensor& q, const at::Tensor& k_cache, cons
 // A workspace of this call alone: it comes from the caching allocator, so
 // captured graphs own theirs and calls on different streams share nothing.
 torch::Tensor attention_workspace(const at::Tensor& q, int64_t n_kv, int64_t groups) {
-    {
-        std::lock_guard<std::mutex> lock(ws_mutex());
-        attention_streams().insert({static_cast<int>(q.get_device()), cur_stream()});
-    }
     const size_t b = lik_attention_workspace_bytes(q.size(0), q.size(1), n_kv, groups);
     return torch::empty({static_cast<int64_t>(b)}, q.options().dtype(torch::kUInt8));
 }

@@ -286,3 +286,56 @@ def test_a_wait_that_runs_out_over_a_shared_prefix(L, kv, step):
         L.check_device_errors()
     assert torch.equal(call(), want)
     L.check_device_errors()
+
+
+# ---------------------------------------------------------------- errors
+
+def test_an_error_of_a_replay_on_a_new_stream_is_reported(L):
+    """A captured call's bad page is met by a replay on a stream that no eager call used, still running at the check."""
+    g = torch.Generator().manual_seed(5)
+    pool = Pool(g, "fp16", 8, 1, 16)
+    table = pool.give([100])
+    q = rand(g, 1, 4, 128)
+    ctx, cu = i32([100]), i32([0, 1])
+    call = lambda: L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, ctx, cu, SCALE)  # noqa: E731
+    want = call()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = call()
+    table[0, 2] = 1 << 20
+    torch.cuda.synchronize()
+    L.check_device_errors()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda._sleep(200_000_000)                     # about a tenth of a second of work ahead of the replay
+        gr.replay()
+    with pytest.raises(RuntimeError, match="out of range"):
+        L.check_device_errors()
+    L.check_device_errors()
+    table[0, 2] = table[0, 1]
+    gr.replay()
+    torch.cuda.synchronize()
+    L.check_device_errors()
+    assert torch.isfinite(out).all() and not torch.equal(out, want)
+
+
+def test_a_destroyed_stream_is_not_asked(L):
+    import ctypes
+    rt = ctypes.CDLL("libcudart.so.12")
+    g = torch.Generator().manual_seed(6)
+    pool = Pool(g, "fp16", 8, 1, 16)
+    table = pool.give([100])
+    q = rand(g, 1, 4, 128)
+    out = torch.empty_like(q)
+    call = lambda: L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([100]), i32([0, 1]), SCALE, out=out)  # noqa: E731
+    call()
+    want = out.clone()
+    handle = ctypes.c_void_p()
+    assert rt.cudaStreamCreate(ctypes.byref(handle)) == 0
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.ExternalStream(handle.value)):
+        call()
+    torch.cuda.synchronize()
+    assert rt.cudaStreamDestroy(handle) == 0
+    L.check_device_errors()
+    assert torch.equal(out, want)
