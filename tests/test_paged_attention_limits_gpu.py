@@ -235,6 +235,34 @@ def test_prefixes_below_zero_show_nothing(L, kv, nq):
                                                    pool.rows("v", table[b], ctx), (j <= p) & (j > p - 100), None))
 
 
+# ---------------------------------------------------------------- offsets out of range
+
+def test_offsets_out_of_range_leave_other_memory_alone(L):
+    """Offsets are cut to the tokens: rows of sequences that hold together are right, rows without positions zero,
+    rows of no sequence and the memory around the result as they were."""
+    g = torch.Generator().manual_seed(7)
+    pool = Pool(g, "fp16", 40, 2, 16)
+    table = pool.give([200, 150])
+    q = rand(g, 20, 8, 128)
+    k, v = pool.rows("k", table[0], 200), pool.rows("v", table[0], 200)
+    # offsets, rows of sequence 0 (200 positions), rows of sequence 1 (none), the others untouched
+    for cu, s0, s1 in (([0, 50, 20], (0, 20), (0, 0)), ([5, 3, 20], (0, 0), (3, 20)), ([-9, 10, 4000], (0, 10), (10, 20)),
+                       ([0, 0, 0], (0, 0), (0, 0)), ([7, 7, 9], (0, 0), (7, 9))):
+        buf = torch.full((60, 8, 128), 7.0, dtype=torch.float16, device="cuda")
+        out = buf[20:40]
+        L.paged_attention(q, pool.cache["k"], pool.cache["v"], table, i32([200, -3]), i32(cu), SCALE, out=out)
+        assert (buf[:20] == 7).all() and (buf[40:] == 7).all()
+        lo, hi = s0
+        if hi > lo:
+            p = torch.arange(200 - (hi - lo), 200, device="cuda")[:, None]
+            check(out[lo:hi], *reference(q[lo:hi], k, v, torch.arange(200, device="cuda")[None] <= p, None))
+        assert (out[s1[0]:s1[1]] == 0).all()
+        rest = torch.ones(20, dtype=torch.bool, device="cuda")
+        rest[lo:hi] = False
+        rest[s1[0]:s1[1]] = False
+        assert (out[rest] == 7).all()
+
+
 # ---------------------------------------------------------------- a wait that runs out
 
 SHAPES = {"wide": ([300], [900]), "paired": ([20], [9000]), "thin": ([1, 1, 1], [300, 20000, 5]),
