@@ -246,7 +246,7 @@ lik_status lik_paged_append(
  * q, q_out [n_tokens, n_heads, 128]; k, v [n_tokens, n_kv_heads, 128] fp16,
  * tokens *_token_stride elements apart (a multiple of 8; views of a fused
  * projection), q_out contiguous and, if q is contiguous too, possibly q
- * itself. slot_mapping as in lik_paged_append: a token whose slot is < 0 or >=
+ * itself (any other overlap with q, k or v is refused). slot_mapping as in lik_paged_append: a token whose slot is < 0 or >=
  * num_blocks * block_size is rotated but not stored; two tokens must not name
  * the same slot. k_format: 0 fp16 or 1 INT8 per token (k_scale); v_format: a
  * row_format of lik_paged_append (v_scale, v_zero). Keys are rounded to fp16
@@ -277,7 +277,8 @@ size_t lik_attention_workspace_bytes(int64_t n_tokens, int64_t n_heads, int64_t 
  * lik_decode_attention_paged.
  *
  * q [n_tokens, n_heads, 128] fp16, tokens q_token_stride elements apart (a
- * multiple of 8); out the same, contiguous. Sequence b owns tokens
+ * multiple of 8); out the same, contiguous, and apart from q or, if q is
+ * contiguous too, q itself. Sequence b owns tokens
  * cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 (int32 [n_seqs + 1], ascending) and
  * the first context_lens[b] positions of its table (int32 [n_seqs], clamped to
  * [0, block_size * max_blocks_per_seq]); its queries are the last of those

@@ -6,6 +6,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include "lik_device.cuh"
 #include "lik_internal.h"
@@ -436,6 +437,15 @@ lik_status lik_decode_attention_paged(int kv_format, const void* q, const void* 
     return run_decode(a, stream);
 }
 
+// Whether a contiguous result [n_tokens, heads, 128] lies over rows that are still
+// to be read, [n_tokens, heads_in, 128] with tokens `stride` elements apart. The
+// very same rows are no clash: each is read before it is written.
+static bool clashes(const void* out, int64_t heads, const void* in, int64_t heads_in, int64_t stride, int64_t n_tokens) {
+    if (out == in && heads == heads_in && (n_tokens == 1 || stride == heads * kHeadDim)) return false;
+    const __int128 o = reinterpret_cast<uintptr_t>(out), i = reinterpret_cast<uintptr_t>(in), n = n_tokens, row = kHeadDim * 2;
+    return o < i + (n - 1) * stride * 2 + heads_in * row && i < o + n * heads * row;
+}
+
 lik_status lik_paged_append_rope(int k_format, int v_format, const void* q, int64_t q_token_stride, const void* k,
                                  int64_t k_token_stride, const void* v, int64_t v_token_stride,
                                  const int64_t* positions, int64_t n_axes, const int64_t* sections,
@@ -473,6 +483,11 @@ lik_status lik_paged_append_rope(int k_format, int v_format, const void* q, int6
     for (const void* t : {q, k, v, static_cast<const void*>(q_out), static_cast<const void*>(k_cache),
                           static_cast<const void*>(v_cache)})
         if (!aligned16(t)) return fail(LIK_ERR_MISALIGNED, "q, k, v, q_out and the caches must be 16-byte aligned");
+    if (clashes(q_out, n_heads, q, n_heads, q_token_stride, n_tokens))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "q_out overlaps q without being q");
+    for (const auto& kv : {std::make_pair(k, k_token_stride), std::make_pair(v, v_token_stride)})
+        if (q_out == kv.first || clashes(q_out, n_heads, kv.first, n_kv_heads, kv.second, n_tokens))
+            return fail(LIK_ERR_INVALID_ARGUMENT, "q_out overlaps k or v");
     RopeAppendArgs a;
     a.q = q; a.k = k; a.v = v;
     a.positions = positions; a.inv_freq = inv_freq; a.slot_mapping = slot_mapping; a.q_out = q_out;
@@ -528,6 +543,8 @@ static lik_status check_attention(const AttentionArgs& a, int64_t head_dim) {
     if (a.fmt == kI8 && (!a.k_scale || !a.v_scale)) return fail(LIK_ERR_INVALID_ARGUMENT, "null scale pointer");
     for (const void* t : {a.q, a.k, a.v, static_cast<const void*>(a.out), a.k_scale, a.v_scale})
         if (!aligned16(t)) return fail(LIK_ERR_MISALIGNED, "q, out, caches and scales must be 16-byte aligned");
+    if (clashes(a.out, a.n_heads, a.q, a.n_heads, a.q_token_stride, a.n_tokens))
+        return fail(LIK_ERR_INVALID_ARGUMENT, "out overlaps q without being q");
     if (reinterpret_cast<uintptr_t>(a.workspace) & 255)
         return fail(LIK_ERR_MISALIGNED, "the workspace must be 256-byte aligned");
     return LIK_OK;

@@ -263,6 +263,26 @@ def test_offsets_out_of_range_leave_other_memory_alone(L):
         assert (out[rest] == 7).all()
 
 
+# ---------------------------------------------------------------- results in the queries' place
+
+@pytest.mark.parametrize("kv", KV)
+def test_results_may_take_the_place_of_their_queries(L, kv):
+    nq, ctx = [1, 300, 20, 2, 70], [5000, 900, 4000, 2, 100]
+    g = torch.Generator().manual_seed(1)
+    pool = Pool(g, kv, sum(-(-c // 32) for c in ctx) + 1, 2, 32)
+    table = pool.give(ctx)
+    q = rand(g, sum(nq), 8, 128)
+    cu = i32([sum(nq[:i]) for i in range(len(nq) + 1)])
+    call = lambda x, out: L.paged_attention(x, pool.cache["k"], pool.cache["v"], table, i32(ctx), cu, SCALE, out=out,  # noqa: E731
+                                            **pool.args())
+    want = call(q, None)
+    place = q.clone()
+    assert torch.equal(call(place, place), want)
+    buf = torch.cat([q, q])
+    with pytest.raises(RuntimeError, match="overlap"):
+        call(buf[:len(q)], buf[1:len(q) + 1])
+
+
 # ---------------------------------------------------------------- a wait that runs out
 
 SHAPES = {"wide": ([300], [900]), "paired": ([20], [9000]), "thin": ([1, 1, 1], [300, 20000, 5]),
