@@ -615,9 +615,7 @@ __device__ __forceinline__ void store_wide(unsigned char* stage, unsigned char* 
 #pragma unroll
         for (int i = 0; i < cols; ++i) o[i] = 0.f;
         if (any) {
-            if constexpr (cols == 8) {
-                tmem_ld8(o_addr + c, o);
-            } else if constexpr (cols == 16) {
+            if constexpr (cols == 16) {
                 tmem_ld16(o_addr + c, o);
             } else {
 #pragma unroll
@@ -954,17 +952,15 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
             if (wide_before && !softmax_sync(mi, xphase)) return;  // the staging space was the warps' own
             float2* ml = reinterpret_cast<float2*>(stage);
             float4* data = reinterpret_cast<float4*>(stage + 2048);
-            constexpr int states = 2, block = kTile;
-            const int rows = g.ntok * p.group, rr = r_in, state = stream;
+            const int rows = g.ntok * p.group;
             ml[threadIdx.x] = live ? float2{m2, l} : float2{-INFINITY, 0.f};
             if (!softmax_sync(mi, xphase)) return;
-            float top = -INFINITY;
-            top = fmaxf(ml[rr].x, ml[block + rr].x);
+            const float top = fmaxf(ml[r_in].x, ml[kTile + r_in].x);
             const float f = m2 == -INFINITY ? 0.f : fast_exp2(m2 - top) * unit_v;
-            int dc = 128;  // channels per pass: what fits the scratch space (states * rows <= 256)
-            while (states * rows * dc * 4 > Layout<FMT>::stage_bytes - 2048) dc >>= 1;
+            int dc = 128;  // channels per pass: what fits the scratch space (2 * rows <= 256)
+            while (2 * rows * dc * 4 > Layout<FMT>::stage_bytes - 2048) dc >>= 1;
             const int quads = dc / 4, spread = min(quads, 8) - 1;
-            float4* const mine_at = data + (state * rows + rr) * quads;
+            float4* const mine_at = data + (stream * rows + r_in) * quads;
 #pragma unroll 1
             for (int d0 = 0; d0 < kHeadDim; d0 += dc) {
 #pragma unroll 1
@@ -984,7 +980,7 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
                             if (x >= 0 && x < n) {
                                 float4 v = {o[4 * i] * f, o[4 * i + 1] * f, o[4 * i + 2] * f, o[4 * i + 3] * f};
                                 if (f == 0.f) v = {0.f, 0.f, 0.f, 0.f};
-                                mine_at[(c / 4 + x) ^ (rr & spread)] = v;
+                                mine_at[(c / 4 + x) ^ (r_in & spread)] = v;
                             }
                         }
                     }
@@ -993,15 +989,12 @@ __device__ void softmax_role(const Params& p, Misc* mi, unsigned char* smem) {
 #pragma unroll 1
                 for (int it = threadIdx.x; it < rows * quads; it += 256) {
                     const int r = it / quads, c4 = it - r * quads;
-                    float mx = -INFINITY, sum = 0.f;
-                    for (int t = 0; t < states; ++t) mx = fmaxf(mx, ml[t * block + r].x);
-                    float4 v = {0.f, 0.f, 0.f, 0.f};
-                    for (int t = 0; t < states; ++t) {
-                        const float2 e = ml[t * block + r];
-                        if (e.x > -INFINITY) sum += e.y * fast_exp2(e.x - mx);
-                        const float4 a = data[(t * rows + r) * quads + (c4 ^ (r & spread))];
-                        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-                    }
+                    const float2 e0 = ml[r], e1 = ml[kTile + r];
+                    const float mx = fmaxf(e0.x, e1.x);
+                    const float sum = (e0.x > -INFINITY ? e0.y * fast_exp2(e0.x - mx) : 0.f) +
+                                      (e1.x > -INFINITY ? e1.y * fast_exp2(e1.x - mx) : 0.f);
+                    const float4 a = data[r * quads + (c4 ^ (r & spread))], b = data[(rows + r) * quads + (c4 ^ (r & spread))];
+                    const float4 v = {a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w};
                     const int tk = p.by_group(r);
                     const uint32_t at = dest_row(p, g, g.tok0 + tk, g.head * p.group + r - tk * p.group, r);
                     if (d0 == 0 && c4 == 0) store_ml(p, g, at, mx, sum);
