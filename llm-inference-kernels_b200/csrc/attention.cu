@@ -39,15 +39,17 @@
 //
 // What bounds it, measured (32 query heads on 8 KV heads; warps 0-7 softmax, 8
 // copies of K and q, 9 matrix instructions, 10 schedule, 11 copies of V):
-//   wide, 4096 causal tokens: the softmax. 154 us in fp16, 894 TFLOP/s, the
-//     tensor pipe busy half of the time; a tile's two steps take 4300 clocks, of
-//     which the exponentials alone are 2048 (32768 of them, 16 per clock on an SM).
-//     Capped scores 252 us (the polynomial), INT8 215 (scales, and one tile of K
-//     and of V in place of two);
-//   thin, 16 requests of 8192: memory. 93 us in fp16, 5.8 TB/s. INT8 103 us: its
+//   wide, 4096 causal tokens: a chain of latencies. 173 us in fp16 under sustained
+//     load, 796 TFLOP/s, with no unit full: a tile's two steps take 4300 clocks,
+//     of which the exponentials are 2048 (32768 of them, 16 per clock on an SM),
+//     the tensor pipe is busy 47% of the time and the issue slots 34%. A stream's
+//     next scores overwrite its weights, so their product is issued behind both
+//     halves of the weighted sum, and its softmax warps wait meanwhile. Capped
+//     scores 227 us, INT8 218 (scales, and one tile of K and of V in place of two);
+//   thin, 16 requests of 8192: memory. 91 us in fp16, 5.9 TB/s. INT8 101 us: its
 //     codes pass shared memory four times (copied in, read, written as fp16, read
 //     by the matrix unit), 1500 of a tile's 3200 clocks;
-//   a few tiles per CTA: the way there. 13 us for one request of 512: finding
+//   a few tiles per CTA: the way there. 12 us for one request of 512: finding
 //     the share 5000 clocks, the first copies 3000, the unit's end 2500, and the
 //     joining kernel.
 #include <cuda_fp16.h>
@@ -1838,8 +1840,8 @@ lik_status launch(const Maps& maps, const Params& p, cudaStream_t stream, std::s
                 cfg.gridDim = dim3(static_cast<unsigned>((rows + 7) / 8));
                 e = cudaLaunchKernelEx(&cfg, join_rows_kernel, p);
             } else {
-                // two rows per warp: four took 32 us in place of 27 for 42 tokens over 1798
-                // keys, one 161 us in place of 153 for a prompt of 4096 (blocks with nothing to do)
+                // two rows per warp: four took 32 us in place of 27 for 42 tokens over 1798 keys,
+                // one 161 us in place of 153 for a prompt of 4096 after a pause (idle blocks)
                 cfg.gridDim = dim3(p.grid, static_cast<unsigned>((p.slot_rows + 15) / 16));
                 e = cudaLaunchKernelEx(&cfg, join_split_kernel, p);
             }
