@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -48,23 +49,32 @@ at::Tensor& workspace(const at::Tensor& like, size_t bytes) {
     return t;
 }
 
+// Devices that attention was called on.
+std::atomic<bool>* attention_used() {
+    static std::atomic<bool> used[64];
+    return used;
+}
+
 // Failure detection for the torch ops: read attention's error word (one per
-// device: this waits for all of the device's work, replayed graphs among it),
-// then that of every cached workspace of the current device. A kernel whose
-// bounded wait expired, or that met an out-of-range block-table entry, left a
-// code there and possibly unit counters that are not zero; lik_workspace_check
-// zeroes such a workspace again, and this op then raises, so the failed step is
-// reported and the next one starts clean.
+// device: where attention was ever called this waits for all of the device's
+// work, replayed graphs among it), then that of every cached workspace of the
+// current device (synchronizing each workspace's stream). A kernel whose bounded
+// wait expired, or that met an out-of-range block-table entry, left a code there
+// and possibly unit counters that are not zero; lik_workspace_check zeroes such a
+// workspace again, and this op then raises, so the failed step is reported and the
+// next one starts clean.
 void check_device_errors() {
     const int dev = static_cast<int>(c10::cuda::current_device());
     std::string msg;
     int code = 0;
-    lik_status st = lik_attention_check(cur_stream(), &code);
-    if (st != LIK_OK) msg = std::string(lik_status_string(st)) + ": " + lik_last_error();
+    if (attention_used()[dev & 63]) {
+        const lik_status st = lik_attention_check(cur_stream(), &code);
+        if (st != LIK_OK) msg = std::string(lik_status_string(st)) + ": " + lik_last_error();
+    }
     std::lock_guard<std::mutex> lock(ws_mutex());
     for (auto& kv : ws_cache()) {
         if (kv.first.first != dev || !kv.second.defined()) continue;
-        st = lik_workspace_check(kv.second.data_ptr(), kv.second.numel(), kv.first.second, &code);
+        const lik_status st = lik_workspace_check(kv.second.data_ptr(), kv.second.numel(), kv.first.second, &code);
         if (st != LIK_OK) msg += std::string(msg.empty() ? "" : "; ") + lik_status_string(st) + ": " + lik_last_error();
     }
     TORCH_CHECK(msg.empty(), "a kernel reported a device-side error (its scratch is reset): ", msg);
@@ -661,6 +671,7 @@ AttnCommon attention_common(const at::Tensor& q, const at::Tensor& k_cache, cons
 // A workspace of this call alone: it comes from the caching allocator, so
 // captured graphs own theirs and calls on different streams share nothing.
 torch::Tensor attention_workspace(const at::Tensor& q, int64_t n_kv, int64_t groups) {
+    attention_used()[q.get_device() & 63] = true;
     const size_t b = lik_attention_workspace_bytes(q.size(0), q.size(1), n_kv, groups);
     return torch::empty({static_cast<int64_t>(b)}, q.options().dtype(torch::kUInt8));
 }
